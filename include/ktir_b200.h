@@ -49,9 +49,11 @@ extern "C" {
 /* status word bits set by kernels */
 #define KTIR_STATUS_NEGATIVE_INDEX 1
 #define KTIR_STATUS_TIMEOUT 2
+#define KTIR_STATUS_BAD_INDEX 4   /* page, slot, position, length or offset out of range */
 
 enum KtirDtype { KTIR_F16 = 0, KTIR_F32 = 1, KTIR_I32 = 2, KTIR_I64 = 3, KTIR_BOOL = 4,
-                 KTIR_U32 = 5 /* arith.fptoui results (NumPy uint32 tiles) */ };
+                 KTIR_U32 = 5, /* arith.fptoui results (NumPy uint32 tiles) */
+                 KTIR_BF16 = 6 /* serving operators only */ };
 
 typedef struct {
   void* base[KTIR_MAX_BUFFERS];
@@ -411,6 +413,97 @@ int ktir_host_upload(const KtirHostXfer* x, int n, int device, void* stream);
  * the stream have completed. */
 int ktir_host_download(const KtirHostXfer* x, int n, const KtirHostCopy* extra, int m,
                        int device, void* stream);
+
+/* ---- serving operators: a paged key-value cache and the attention on it ----
+ *
+ * A paged cache is a pair of tensors K and V of elements (page, place, kv
+ * head, dim), the head vector contiguous, the other strides free (so a page
+ * may be stored token by token or head by head).  Slot s of the cache is
+ * place s % page_size of page s / page_size.  Element type f16 or bf16
+ * (dtype KTIR_F16 or KTIR_BF16) for all of q, k, v, caches and outputs; head
+ * vectors start on 16-byte boundaries (strides multiples of 8 elements).
+ * kv_heads divides heads: query head h reads kv head h / (heads / kv_heads).
+ * Index arrays are int32 in device memory; an index outside its range sets
+ * KTIR_STATUS_BAD_INDEX in *status and touches no memory.  (The reference's
+ * counterpart is its paged attention program, examples/triton-ktir/
+ * paged_attention.mlir, one indirect load per tile; it has no append.) */
+
+/* New tokens into the cache: k rotated by its position, and v, are written to
+ * slots[t] (negative: the token is padding and not written); q, when given,
+ * is rotated into q_out.  The rotation turns the pairs (x_i, x_{i+rot/2}), or
+ * (x_2i, x_2i+1) when interleaved, of a vector's first `rot` elements by
+ * table[position][i] = cos and table[position][rot/2 + i] = sin, in f32,
+ * rounded once; the elements after `rot` are copied.  rot = 0: plain copy, no
+ * positions or table needed.  The slots of one call are distinct. */
+typedef struct {
+  const void* q; const void* k; const void* v;   /* [tokens][heads][dim]; q may be null */
+  void* q_out;
+  void* k_cache; void* v_cache;
+  const int32_t* slots;
+  const int32_t* positions;
+  const float* table;            /* [table_rows][rot], rows table_stride apart */
+  int32_t* status;
+  int64_t tokens;
+  int64_t q_stride[2], k_stride[2], v_stride[2], qo_stride[2];   /* token, head */
+  int64_t kc_stride[3], vc_stride[3];                            /* page, place, head */
+  int64_t num_pages, page_size;
+  int64_t table_rows, table_stride;
+  int32_t heads, kv_heads, dim, rot;
+  int32_t interleaved, dtype;
+} KtirKvAppendDesc;
+int ktir_kv_append(const KtirKvAppendDesc* desc, void* stream);
+
+/* Attention of one new token per sequence over its cached keys: out[b][h] =
+ * softmax(scale q[b][h] . K) V over the lengths[b] first keys of the pages
+ * pages[b][0 ..].  A sequence of length 0 gives zeros (lse -inf).  lse, when
+ * given, receives the natural logarithm of each row's sum of exponentials,
+ * [batch][heads] f32.  dim 64 or 128.  workspace: device memory of at least
+ * ktir_paged_decode_workspace() bytes, zero before its first use and left so
+ * that the next call on the same stream may use it; two calls that may overlap
+ * need workspaces of their own. */
+typedef struct {
+  const void* q;                 /* [batch][heads][dim] */
+  const void* k_cache; const void* v_cache;
+  void* out;                     /* [batch][heads][dim] */
+  float* lse;
+  const int32_t* pages;          /* [batch][max_pages], rows page_row apart */
+  const int32_t* lengths;
+  void* workspace;
+  int32_t* status;
+  int64_t workspace_bytes;
+  int64_t batch, max_pages, page_row;
+  int64_t num_pages, page_size;
+  int64_t q_stride[2], out_stride[2];            /* sequence, head */
+  int64_t kc_stride[3], vc_stride[3];            /* page, place, head */
+  int32_t heads, kv_heads, dim, dtype;
+  float scale;
+  int32_t pad;
+} KtirPagedDecodeDesc;
+int64_t ktir_paged_decode_workspace(int64_t batch, int32_t heads, int32_t kv_heads, int32_t dim);
+int ktir_paged_decode(const KtirPagedDecodeDesc* desc, void* stream);
+
+/* Attention over packed prompts: sequence b's queries are tokens offsets[b] ..
+ * offsets[b+1]-1 of q, its keys tokens kv_offsets[b] .. kv_offsets[b+1]-1 of k
+ * and v (kv_offsets may be offsets itself).  Causal masks are aligned at the
+ * end: query i of n sees keys j <= i + m - n of m (m > n when the first part
+ * of the prompt was read earlier); a query that sees no key gives zeros (lse
+ * -inf).  lse as above, [tokens][heads].  dim 64 or 128; heads / kv_heads at
+ * most 128. */
+typedef struct {
+  const void* q;                 /* [tokens][heads][dim] */
+  const void* k; const void* v;  /* [kv_tokens][kv_heads][dim] */
+  void* out;                     /* [tokens][heads][dim] */
+  float* lse;
+  const int32_t* offsets;        /* [batch + 1] */
+  const int32_t* kv_offsets;     /* [batch + 1] */
+  int32_t* status;
+  int64_t batch, tokens, kv_tokens;
+  int64_t q_stride[2], k_stride[2], v_stride[2], out_stride[2];   /* token, head */
+  int32_t heads, kv_heads, dim, dtype;
+  float scale;
+  int32_t causal;
+} KtirPromptDesc;
+int ktir_prompt_attention(const KtirPromptDesc* desc, void* stream);
 
 #ifdef __cplusplus
 }

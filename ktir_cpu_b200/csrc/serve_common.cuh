@@ -1,0 +1,63 @@
+// Shared by the serving operators (kv_append.cu, paged_decode.cu,
+// prompt_attention.cu): element types, conversions and host-side checks.
+#pragma once
+
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+#include <cuda_runtime.h>
+#include <math.h>
+#include <stdint.h>
+
+#include "../../include/ktir_b200.h"
+
+int ktir_set_error(int code, const char* msg);
+
+namespace ktir {
+namespace serve {
+
+constexpr float LOG2E = 1.4426950408889634f;
+constexpr float LN2 = 0.6931471805599453f;
+
+template <typename T> struct Elem;
+template <> struct Elem<__half> {
+  static __device__ __forceinline__ float2 to2(uint32_t v) {
+    return __half22float2(*reinterpret_cast<const __half2*>(&v));
+  }
+  static __device__ __forceinline__ uint32_t from2(float a, float b) {   // round to nearest even
+    const __half2 h = __floats2half2_rn(a, b);
+    return *reinterpret_cast<const uint32_t*>(&h);
+  }
+};
+template <> struct Elem<__nv_bfloat16> {
+  static __device__ __forceinline__ float2 to2(uint32_t v) {
+    return make_float2(__uint_as_float(v << 16), __uint_as_float(v & 0xffff0000u));
+  }
+  static __device__ __forceinline__ uint32_t from2(float a, float b) {   // round to nearest even
+    const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
+    return *reinterpret_cast<const uint32_t*>(&h);
+  }
+};
+
+// 2^x on the special-function unit (relative error about 2^-22; -inf gives 0)
+__device__ __forceinline__ float ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+// -- host-side checks ---------------------------------------------------------
+inline bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
+
+// strides (elements) of axes with more than one entry keep head vectors on 16-byte boundaries
+inline bool vector_strides(const int64_t* stride, const int64_t* extent, int n) {
+  for (int i = 0; i < n; ++i)
+    if (extent[i] > 1 && ((stride[i] & 7) || stride[i] < 0)) return false;
+  return true;
+}
+
+inline int launched(const char* what) {
+  return cudaGetLastError() == cudaSuccess ? KTIR_OK : ktir_set_error(KTIR_ERR_CUDA, what);
+}
+
+}  // namespace serve
+}  // namespace ktir

@@ -24,9 +24,10 @@ MAX_INSTR = 64
 NREG = 12
 ARENA_SLOT = MAX_BUFFERS - 1
 
-F16, F32, I32, I64, BOOL, U32 = 0, 1, 2, 3, 4, 5
+F16, F32, I32, I64, BOOL, U32, BF16 = 0, 1, 2, 3, 4, 5, 6
 STATUS_NEGATIVE_INDEX = 1
 STATUS_TIMEOUT = 2
+STATUS_BAD_INDEX = 4
 
 _DT = {np.dtype(np.float16): F16, np.dtype(np.float32): F32, np.dtype(np.int32): I32,
        np.dtype(np.int64): I64, np.dtype(np.bool_): BOOL, np.dtype(np.uint32): U32}
@@ -139,13 +140,50 @@ class KtirHostCopy(C.Structure):
     _fields_ = [("dst", C.c_void_p), ("src", C.c_void_p), ("bytes", C.c_int64)]
 
 
+class KtirKvAppendDesc(C.Structure):
+    _fields_ = [("q", C.c_void_p), ("k", C.c_void_p), ("v", C.c_void_p), ("q_out", C.c_void_p),
+                ("k_cache", C.c_void_p), ("v_cache", C.c_void_p), ("slots", C.c_void_p),
+                ("positions", C.c_void_p), ("table", C.c_void_p), ("status", C.c_void_p),
+                ("tokens", C.c_int64), ("q_stride", C.c_int64 * 2), ("k_stride", C.c_int64 * 2),
+                ("v_stride", C.c_int64 * 2), ("qo_stride", C.c_int64 * 2),
+                ("kc_stride", C.c_int64 * 3), ("vc_stride", C.c_int64 * 3),
+                ("num_pages", C.c_int64), ("page_size", C.c_int64), ("table_rows", C.c_int64),
+                ("table_stride", C.c_int64), ("heads", C.c_int32), ("kv_heads", C.c_int32),
+                ("dim", C.c_int32), ("rot", C.c_int32), ("interleaved", C.c_int32),
+                ("dtype", C.c_int32)]
+
+
+class KtirPagedDecodeDesc(C.Structure):
+    _fields_ = [("q", C.c_void_p), ("k_cache", C.c_void_p), ("v_cache", C.c_void_p),
+                ("out", C.c_void_p), ("lse", C.c_void_p), ("pages", C.c_void_p),
+                ("lengths", C.c_void_p), ("workspace", C.c_void_p), ("status", C.c_void_p),
+                ("workspace_bytes", C.c_int64), ("batch", C.c_int64), ("max_pages", C.c_int64),
+                ("page_row", C.c_int64), ("num_pages", C.c_int64), ("page_size", C.c_int64),
+                ("q_stride", C.c_int64 * 2), ("out_stride", C.c_int64 * 2),
+                ("kc_stride", C.c_int64 * 3), ("vc_stride", C.c_int64 * 3),
+                ("heads", C.c_int32), ("kv_heads", C.c_int32), ("dim", C.c_int32),
+                ("dtype", C.c_int32), ("scale", C.c_float), ("pad", C.c_int32)]
+
+
+class KtirPromptDesc(C.Structure):
+    _fields_ = [("q", C.c_void_p), ("k", C.c_void_p), ("v", C.c_void_p), ("out", C.c_void_p),
+                ("lse", C.c_void_p), ("offsets", C.c_void_p), ("kv_offsets", C.c_void_p),
+                ("status", C.c_void_p), ("batch", C.c_int64), ("tokens", C.c_int64),
+                ("kv_tokens", C.c_int64), ("q_stride", C.c_int64 * 2),
+                ("k_stride", C.c_int64 * 2), ("v_stride", C.c_int64 * 2),
+                ("out_stride", C.c_int64 * 2), ("heads", C.c_int32), ("kv_heads", C.c_int32),
+                ("dim", C.c_int32), ("dtype", C.c_int32), ("scale", C.c_float),
+                ("causal", C.c_int32)]
+
+
 EXPORTS = ["ktir_version", "ktir_last_error", "ktir_device_count", "ktir_ew",
            "ktir_softmax_rows", "ktir_gather_rmw", "ktir_reduce", "ktir_matmul",
            "ktir_offsets", "ktir_indirect", "ktir_gemm_f16", "ktir_gemm_f16_blocked", "ktir_fmha_f16",
            "ktir_fmha_f16_part", "ktir_copy_blocks", "ktir_pack_kv", "ktir_bytes_delta",
            "ktir_wait_selftest", "ktir_host_threads", "ktir_host_upload", "ktir_host_download",
            "ktir_ipc_alloc", "ktir_ipc_open", "ktir_ipc_close", "ktir_ipc_free", "ktir_flag_set",
-           "ktir_flag_wait", "ktir_copy_async"]
+           "ktir_flag_wait", "ktir_copy_async", "ktir_kv_append", "ktir_paged_decode",
+           "ktir_prompt_attention"]
 
 _LIB: Optional[C.CDLL] = None
 
@@ -199,6 +237,11 @@ def load_library(build_if_missing: bool = False) -> C.CDLL:
     lib.ktir_host_upload.argtypes = [C.POINTER(KtirHostXfer), C.c_int, C.c_int, vp]
     lib.ktir_host_download.argtypes = [C.POINTER(KtirHostXfer), C.c_int, C.POINTER(KtirHostCopy),
                                        C.c_int, C.c_int, vp]
+    lib.ktir_kv_append.argtypes = [C.POINTER(KtirKvAppendDesc), vp]
+    lib.ktir_paged_decode.argtypes = [C.POINTER(KtirPagedDecodeDesc), vp]
+    lib.ktir_paged_decode_workspace.argtypes = [C.c_int64, C.c_int32, C.c_int32, C.c_int32]
+    lib.ktir_paged_decode_workspace.restype = C.c_int64
+    lib.ktir_prompt_attention.argtypes = [C.POINTER(KtirPromptDesc), vp]
     for name in EXPORTS:
         getattr(lib, name).restype = C.c_int if name != "ktir_last_error" else C.c_char_p
     _LIB = lib

@@ -1,0 +1,474 @@
+"""The serving operators (paged append, packed prompts, single-token decode)
+against plain 64-bit forms; bounds derived in serving_util.py."""
+
+import math
+import random
+
+import pytest
+
+import serving_util as S
+
+pytestmark = pytest.mark.gpu
+
+
+def _gen(seed):
+    import torch
+    return torch.Generator(device="cuda").manual_seed(seed)
+
+
+def _randn(gen, typ, *shape):
+    import torch
+    return torch.randn(*shape, generator=gen, device="cuda").to(S.dtype_of(typ))
+
+
+def _cache(gen, typ, pages, page, heads, dim, head_major):
+    if head_major:
+        return _randn(gen, typ, pages, heads, page, dim).transpose(1, 2)
+    return _randn(gen, typ, pages, page, heads, dim)
+
+
+# -- append -----------------------------------------------------------------------
+
+@pytest.mark.parametrize("typ,tokens,heads,kv_heads,dim,rot,page,interleaved,head_major", [
+    ("bf16", 1, 8, 2, 128, 128, 16, False, False),
+    ("f16", 37, 4, 4, 64, 32, 8, True, True),
+    ("bf16", 300, 6, 3, 96, 96, 24, False, True),
+    ("f16", 65, 40, 8, 128, 64, 1, False, False),
+    ("bf16", 9, 1, 1, 256, 16, 128, True, False),
+    ("f16", 12, 3, 1, 80, 0, 7, False, False),
+])
+def test_append(typ, tokens, heads, kv_heads, dim, rot, page, interleaved, head_major):
+    import torch
+    from ktir_cpu_b200 import check_status, kv_append, rotary_table
+    gen = _gen(tokens)
+    pages = tokens // page + 3
+    qkv = _randn(gen, typ, tokens, heads + 2 * kv_heads, dim)
+    q, k, v = qkv[:, :heads], qkv[:, heads:heads + kv_heads], qkv[:, heads + kv_heads:]
+    kc, vc = (_cache(gen, typ, pages, page, kv_heads, dim, head_major) for _ in range(2))
+    kc0, vc0 = kc.clone(), vc.clone()
+    slots = torch.randperm(pages * page, generator=gen, device="cuda")[:tokens].int()
+    if tokens > 1:
+        slots[::7] = -1
+    args = {}
+    if rot:
+        args = dict(table=rotary_table(5000, rot), interleaved=interleaved,
+                    positions=torch.randint(0, 5000, (tokens,), generator=gen, device="cuda").int())
+    q0 = qkv.clone()
+    out = kv_append(k, v, kc, vc, slots, q=q, **args)
+    check_status()
+    assert torch.equal(qkv, q0), "inputs changed"
+    def turned(x):
+        return S.rotate(x, args["table"], args["positions"], interleaved) if rot else (x.double(), torch.zeros_like(x, dtype=torch.float64))
+    want, bound = turned(q)
+    assert ((out.double() - want).abs() <= bound).all()
+    kept = slots >= 0
+    at = (slots[kept].long() // page, slots[kept].long() % page)
+    want, bound = turned(k)
+    assert ((kc[at].double() - want[kept]).abs() <= bound[kept]).all()
+    assert torch.equal(vc[at], v[kept])
+    kc0[at], vc0[at] = kc[at], vc[at]
+    assert torch.equal(kc, kc0) and torch.equal(vc, vc0), "another slot was written"
+
+
+def test_append_in_place_and_without_queries():
+    import torch
+    from ktir_cpu_b200 import check_status, kv_append, rotary_table
+    gen = _gen(3)
+    k, v, q = (_randn(gen, "bf16", 20, 4, 64) for _ in range(3))
+    caches = [torch.zeros(4, 8, 4, 64, dtype=torch.bfloat16, device="cuda") for _ in range(4)]
+    slots = torch.arange(20, dtype=torch.int32, device="cuda")
+    args = dict(positions=slots, table=rotary_table(64, 64))
+    out = kv_append(k, v, caches[0], caches[1], slots, q=q, **args)
+    same = q.clone()
+    assert kv_append(k, v, caches[2], caches[3], slots, q=same, q_out=same, **args) is same
+    assert torch.equal(out, same) and torch.equal(caches[0], caches[2]) and torch.equal(caches[1], caches[3])
+    caches[2].zero_()
+    assert kv_append(k, v, caches[2], caches[3], slots, **args) is None
+    assert torch.equal(caches[0], caches[2])
+    check_status()
+
+
+def test_append_reports_bad_indices():
+    import torch
+    from ktir_cpu_b200 import check_status, kv_append, rotary_table
+    gen = _gen(4)
+    k, v = (_randn(gen, "f16", 3, 2, 64) for _ in range(2))
+    kc, vc = (torch.zeros(2, 4, 2, 64, dtype=torch.float16, device="cuda") for _ in range(2))
+    index = lambda *x: torch.tensor(x, dtype=torch.int32, device="cuda")  # noqa: E731
+    kv_append(k, v, kc, vc, index(0, 8, 1))
+    with pytest.raises(IndexError):
+        check_status()
+    check_status()
+    kv_append(k, v, kc, vc, index(4, 5, 6), positions=index(0, 10, -1), table=rotary_table(10, 64))
+    with pytest.raises(IndexError):
+        check_status()
+    assert torch.equal(vc[1, 0], v[0]) and not vc[1, 1:].any()
+
+
+# -- decode -----------------------------------------------------------------------
+
+def _decode_inputs(typ, lengths, heads, kv_heads, dim, page, head_major=False, seed=0, scale_q=1.0):
+    import torch
+    gen = _gen(seed)
+    each = [-(-m // page) for m in lengths]
+    total = sum(each) + 2
+    kc, vc = (_cache(gen, typ, total, page, kv_heads, dim, head_major) for _ in range(2))
+    order = torch.randperm(total, generator=gen, device="cuda").int().cpu()
+    pages = torch.full((len(lengths), max(each + [1]) + 1), -7, dtype=torch.int32)
+    at = 0
+    for b, n in enumerate(each):
+        pages[b, :n] = order[at:at + n]
+        at += n
+    q = (_randn(gen, typ, len(lengths), heads, dim).float() * scale_q).to(S.dtype_of(typ))
+    return q, kc, vc, pages.cuda(), torch.tensor(lengths, dtype=torch.int32, device="cuda")
+
+
+def _check_decode(typ, q, kc, vc, pages, lengths, scale, out, lse):
+    S.decode(q, kc, vc, pages, lengths, scale,
+             lambda b, hs, want: S.check_rows(f"seq {b} heads {hs}", out[b, hs], want, typ, q.shape[2], lse[b, hs]))
+
+
+@pytest.mark.parametrize("typ,lengths,heads,kv_heads,dim,page,head_major", [
+    ("bf16", [1], 4, 1, 128, 16, False),
+    ("f16", [77], 32, 8, 128, 16, False),
+    ("bf16", [0, 1, 15, 16, 17, 0, 63, 64, 65, 130], 8, 2, 64, 16, True),
+    ("f16", [1000, 3, 257], 5, 5, 64, 24, False),
+    ("bf16", [513, 40], 12, 4, 128, 1, True),
+    ("f16", [70, 200], 48, 1, 128, 128, False),
+    ("bf16", [300, 5], 34, 2, 64, 7, False),
+    ("bf16", [9000], 8, 4, 128, 64, True),
+    ("f16", [20000, 10, 0], 16, 2, 128, 32, False),
+])
+def test_decode(typ, lengths, heads, kv_heads, dim, page, head_major):
+    from ktir_cpu_b200 import check_status, paged_decode
+    x = _decode_inputs(typ, lengths, heads, kv_heads, dim, page, head_major, seed=sum(lengths))
+    out, lse = paged_decode(*x, return_lse=True)
+    check_status()
+    _check_decode(typ, *x, dim ** -0.5, out, lse)
+
+
+def test_decode_many_sequences():
+    from ktir_cpu_b200 import check_status, paged_decode
+    rng = random.Random(5)
+    lengths = [rng.choice([0, 1, 2, 30, 64, 100, 300]) for _ in range(700)]
+    x = _decode_inputs("bf16", lengths, 4, 2, 64, 16, seed=9)
+    out, lse = paged_decode(*x, scale=0.3, return_lse=True)
+    check_status()
+    _check_decode("bf16", *x, 0.3, out, lse)
+
+
+@pytest.mark.parametrize("typ", ["bf16", "f16"])
+def test_decode_peaked_and_growing_scores(typ):
+    """Scores in the hundreds, the largest at the end: the running maximum moves
+    over and over, and most weights vanish."""
+    import torch
+    from ktir_cpu_b200 import check_status, paged_decode
+    q, kc, vc, pages, lengths = _decode_inputs(typ, [700, 2000], 8, 2, 128, 16, seed=2, scale_q=4.0)
+    ramp = torch.linspace(0.1, 3.0, 2000, device="cuda")
+    for b, m in enumerate(lengths.tolist()):
+        for i, p in enumerate(pages[b, :-(-m // 16)].tolist()):
+            kc[p] = (kc[p].float() * ramp[16 * i:16 * i + 16, None, None]).to(kc.dtype)
+    out, lse = paged_decode(q, kc, vc, pages, lengths, return_lse=True)
+    check_status()
+    _check_decode(typ, q, kc, vc, pages, lengths, 128 ** -0.5, out, lse)
+
+
+def test_decode_ignores_what_lies_past_the_length():
+    """Places past a sequence's length hold NaN and infinities."""
+    import torch
+    from ktir_cpu_b200 import check_status, paged_decode
+    q, kc, vc, pages, lengths = _decode_inputs("f16", [5, 33, 100, 0], 8, 2, 128, 32, seed=6)
+    clean = paged_decode(q, kc, vc, pages, lengths)
+    used = torch.zeros(kc.shape[:2], dtype=torch.bool, device="cuda")
+    for b, m in enumerate(lengths.tolist()):
+        for j in range(m):
+            used[int(pages[b, j // 32]), j % 32] = True
+    for i, bad in enumerate([math.nan, math.inf, -math.inf]):
+        kc[~used], vc[~used] = bad, bad
+        assert torch.equal(paged_decode(q, kc, vc, pages, lengths), clean), bad
+    check_status()
+
+
+def test_decode_strides_streams_and_repeats():
+    """Strided queries and outputs, another stream, calls of different sizes in turn,
+    and the same result every time."""
+    import torch
+    from ktir_cpu_b200 import check_status, paged_decode
+    small = _decode_inputs("bf16", [40, 900], 8, 2, 128, 16, seed=11)
+    large = _decode_inputs("bf16", [5000, 100, 7, 3000], 16, 4, 128, 16, seed=12)
+    a, b = paged_decode(*small), paged_decode(*large)
+    wide = torch.zeros(2, 8, 3, 128, dtype=torch.bfloat16, device="cuda")
+    wide[:, :, 1] = small[0]
+    into = torch.zeros_like(wide)
+    stream = torch.cuda.Stream()
+    stream.wait_stream(torch.cuda.current_stream())
+    for _ in range(20):
+        got = paged_decode(wide[:, :, 1], *small[1:], out=into[:, :, 2])
+        assert torch.equal(got, a) and not into[:, :, :2].any()
+        with torch.cuda.stream(stream):
+            other = paged_decode(*large)
+        stream.synchronize()
+        assert torch.equal(other, b) and torch.equal(paged_decode(*large), b)
+    check_status()
+
+
+def test_decode_in_a_graph():
+    import torch
+    from ktir_cpu_b200 import check_status, paged_decode
+    x = _decode_inputs("bf16", [3000, 17, 400], 16, 4, 128, 16, seed=13)
+    want = paged_decode(*x)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = paged_decode(*x)
+    for _ in range(3):
+        got.zero_()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(got, want)
+    x[4][1] = 5
+    graph.replay()
+    assert torch.equal(got, paged_decode(*x))
+    check_status()
+
+
+def test_decode_reports_bad_indices():
+    import torch
+    from ktir_cpu_b200 import check_status, paged_decode
+    for at, bad in [((3, (0, 1)), -1), ((3, (0, 1)), 1 << 20), ((4, (0,)), 500), ((4, (0,)), -3)]:
+        x = _decode_inputs("bf16", [40, 20], 4, 2, 64, 16, seed=14)
+        want = paged_decode(*x)
+        check_status()
+        x[at[0]][at[1]] = bad
+        got = paged_decode(*x)
+        with pytest.raises(IndexError):
+            check_status()
+        assert torch.equal(got[1], want[1])
+
+
+def test_decode_past_32_bits():
+    """Element offsets above 2^31 in the cache."""
+    import torch
+    from ktir_cpu_b200 import check_status, paged_decode
+    pages, page, hk, d = 66000, 16, 16, 128            # 2.16e9 elements, 4.3 GB each
+    kc, vc = (torch.zeros(pages, page, hk, d, dtype=torch.bfloat16, device="cuda") for _ in range(2))
+    gen = _gen(15)
+    last = [65999, 65990, 3]
+    for p in last:
+        kc[p], vc[p] = _randn(gen, "bf16", page, hk, d), _randn(gen, "bf16", page, hk, d)
+    q = _randn(gen, "bf16", 1, 16, d)
+    table = torch.tensor([last], dtype=torch.int32, device="cuda")
+    lengths = torch.tensor([41], dtype=torch.int32, device="cuda")
+    out, lse = paged_decode(q, kc, vc, table, lengths, return_lse=True)
+    check_status()
+    _check_decode("bf16", q, kc, vc, table, lengths, d ** -0.5, out, lse)
+
+
+# -- prompt -----------------------------------------------------------------------
+
+def _prompt_inputs(typ, new, keys, heads, kv_heads, dim, seed=0):
+    import torch
+    gen = _gen(seed)
+    q = _randn(gen, typ, sum(new), heads, dim)
+    kv = _randn(gen, typ, sum(keys), 2 * kv_heads, dim)
+    ends = lambda each: torch.tensor([0] + each, device="cuda").cumsum(0).int()  # noqa: E731
+    return q, kv[:, :kv_heads], kv[:, kv_heads:], ends(new), ends(keys)
+
+
+def _check_prompt(typ, q, k, v, offsets, kv_offsets, causal, scale, out, lse):
+    S.prompt(q, k, v, offsets, kv_offsets, causal, scale,
+             lambda ts, h, want: S.check_rows(f"tokens {ts} head {h}", out[ts, h], want, typ, q.shape[2], lse[ts, h]))
+
+
+@pytest.mark.parametrize("typ,new,keys,heads,kv_heads,dim,causal", [
+    ("bf16", [1], [1], 4, 1, 128, True),
+    ("f16", [19], [19], 32, 8, 128, True),
+    ("bf16", [0, 1, 127, 128, 129, 0, 255, 257, 0], None, 4, 2, 128, True),
+    ("f16", [300, 31, 64, 2], None, 5, 5, 64, True),
+    ("bf16", [200, 40], None, 12, 2, 64, False),
+    ("f16", [130, 77], None, 7, 1, 128, False),
+    ("bf16", [33, 5, 0, 100], [500, 5, 64, 101], 6, 2, 128, True),
+    ("f16", [17, 1, 20], [300, 129, 900], 3, 1, 64, True),
+    ("bf16", [50, 200, 9], [20, 60, 0], 4, 2, 64, True),      # rows that see no key
+    ("f16", [50, 9], [20, 0], 4, 2, 128, False),
+    ("bf16", [1030], None, 2, 1, 128, True),
+    ("bf16", [70, 3], None, 80, 1, 128, True),
+    ("f16", [5, 260], None, 128, 1, 64, True),
+    ("bf16", [2100, 600], None, 3, 3, 64, True),
+])
+def test_prompt(typ, new, keys, heads, kv_heads, dim, causal):
+    from ktir_cpu_b200 import check_status, prompt_attention
+    q, k, v, offsets, kv_offsets = _prompt_inputs(typ, new, keys or new, heads, kv_heads, dim, seed=sum(new))
+    out, lse = prompt_attention(q, k, v, offsets, kv_offsets=kv_offsets if keys else None, causal=causal,
+                                return_lse=True)
+    check_status()
+    _check_prompt(typ, q, k, v, offsets, kv_offsets, causal, dim ** -0.5, out, lse)
+
+
+def test_prompt_many_short():
+    from ktir_cpu_b200 import check_status, prompt_attention
+    rng = random.Random(8)
+    new = [rng.choice([0, 1, 2, 5, 17, 40]) for _ in range(500)]
+    x = _prompt_inputs("bf16", new, new, 2, 1, 64, seed=16)
+    out, lse = prompt_attention(*x[:4], scale=0.2, return_lse=True)
+    check_status()
+    _check_prompt("bf16", *x, True, 0.2, out, lse)
+
+
+@pytest.mark.parametrize("typ,dim", [("bf16", 128), ("f16", 64), ("f16", 128)])
+@pytest.mark.parametrize("rising", [True, False])
+def test_prompt_peaked_scores(typ, dim, rising):
+    """Large scores, rising or falling along the keys: the running maximum moves
+    over and over, or most later weights vanish."""
+    import torch
+    from ktir_cpu_b200 import check_status, prompt_attention
+    q, k, v, offsets, kv_offsets = _prompt_inputs(typ, [900, 300], [900, 300], 4, 2, dim, seed=17)
+    ramp = torch.linspace(0.1, 6.0, 1200, device="cuda")
+    k = (k.float() * (ramp if rising else ramp.flip(0))[:, None, None]).to(k.dtype)
+    out, lse = prompt_attention(q, k, v, offsets, return_lse=True)
+    check_status()
+    _check_prompt(typ, q, k, v, offsets, kv_offsets, True, dim ** -0.5, out, lse)
+
+
+def test_prompt_sequences_do_not_mix():
+    """NaN and infinities in one sequence reach no other."""
+    import torch
+    from ktir_cpu_b200 import check_status, prompt_attention
+    new = [70, 33, 150, 20]
+    q, k, v, offsets, _ = _prompt_inputs("bf16", new, new, 4, 2, 128, seed=18)
+    clean = prompt_attention(q, k, v, offsets)
+    for bad in [math.nan, math.inf, -math.inf]:
+        for lo, hi in [(0, 70), (103, 253)]:
+            q2, k2, v2 = q.clone(), k.clone(), v.clone()
+            q2[lo:hi], k2[lo:hi], v2[lo:hi] = bad, bad, bad
+            got = prompt_attention(q2, k2, v2, offsets)
+            assert torch.equal(got[:lo], clean[:lo]) and torch.equal(got[hi:], clean[hi:]), (bad, lo)
+    check_status()
+
+
+def test_prompt_infinite_keys_in_masked_places():
+    """A later key that is infinite or NaN moves no earlier row."""
+    import torch
+    from ktir_cpu_b200 import check_status, prompt_attention
+    q, k, v, offsets, _ = _prompt_inputs("bf16", [200], [200], 4, 2, 128, seed=19)
+    clean = prompt_attention(q, k, v, offsets)
+    for bad in [math.nan, math.inf]:
+        k2 = k.clone()
+        k2[150:] = bad
+        got = prompt_attention(q, k2, v, offsets)
+        assert torch.equal(got[:150], clean[:150])
+    check_status()
+
+
+def test_prompt_strides_out_and_graph():
+    import torch
+    from ktir_cpu_b200 import check_status, prompt_attention
+    q, k, v, offsets, kv_offsets = _prompt_inputs("f16", [140, 61], [140, 61], 6, 2, 64, seed=20)
+    want = prompt_attention(q, k, v, offsets)
+    # head-major memory, and outputs inside a larger buffer
+    q2, k2, v2 = (x.transpose(0, 1).contiguous().transpose(0, 1) for x in (q, k, v))
+    into = torch.zeros(201, 8, 128, dtype=torch.float16, device="cuda")
+    got = prompt_attention(q2, k2, v2, offsets, out=into[:, 1:7, 64:])
+    assert torch.equal(got, want)
+    assert not into[:, 0].any() and not into[:, 7].any() and not into[:, :, :64].any()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        again = prompt_attention(q, k, v, offsets)
+    for _ in range(3):
+        again.zero_()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(again, want)
+    # keys and values that all heads of a broadcast input share
+    one = k[:, :1].expand(-1, 2, -1)
+    assert torch.equal(prompt_attention(q, one, one, offsets),
+                       prompt_attention(q, one.contiguous(), one.contiguous(), offsets))
+    check_status()
+
+
+def test_prompt_reports_bad_offsets():
+    import torch
+    from ktir_cpu_b200 import check_status, prompt_attention
+    q, k, v, offsets, kv_offsets = _prompt_inputs("bf16", [40, 30], [50, 60], 2, 1, 64, seed=21)
+    for bad in ([0, 50, 111], [0, 50, 40], [-1, 50, 110]):
+        prompt_attention(q, k, v, offsets, kv_offsets=torch.tensor(bad, dtype=torch.int32, device="cuda"))
+        with pytest.raises(IndexError):
+            check_status()
+    prompt_attention(q, k, v, offsets, kv_offsets=kv_offsets)
+    check_status()
+
+
+# -- refusals with tensors on the GPU, and the pieces together ------------------------
+
+def test_refusals():
+    import torch
+    from ktir_cpu_b200 import kv_append, paged_decode, prompt_attention
+    q, kc, vc, pages, lengths = _decode_inputs("bf16", [40, 20], 4, 2, 64, 16, seed=22)
+    off = torch.tensor([0, 2], dtype=torch.int32, device="cuda")
+    k = kc[0, :2]
+    slots = off
+    for call, kind in [
+        (lambda: paged_decode(q.float(), kc, vc, pages, lengths), NotImplementedError),
+        (lambda: paged_decode(q, kc.half(), vc, pages, lengths), ValueError),
+        (lambda: paged_decode(q[:, :3], kc, vc, pages, lengths), ValueError),
+        (lambda: paged_decode(q, kc, vc, pages.long(), lengths), ValueError),
+        (lambda: paged_decode(q, kc, vc, pages, lengths[:1]), ValueError),
+        (lambda: paged_decode(q, kc, vc, pages, lengths.cpu()), ValueError),
+        (lambda: paged_decode(q, kc, vc, pages, lengths, scale=-1.0), NotImplementedError),
+        (lambda: paged_decode(q, kc, vc, pages, lengths, scale=math.nan), NotImplementedError),
+        (lambda: paged_decode(q[..., :32], kc[..., :32], vc[..., :32], pages, lengths), NotImplementedError),
+        (lambda: paged_decode(q.requires_grad_(), kc, vc, pages, lengths), RuntimeError),
+        (lambda: paged_decode(torch.zeros(2, 4, 65, dtype=q.dtype, device="cuda")[..., 1:], kc, vc, pages, lengths),
+         NotImplementedError),
+        (lambda: prompt_attention(k, k, k[:1], off), ValueError),
+        (lambda: prompt_attention(k, k[:1], k[:1], off), ValueError),
+        (lambda: prompt_attention(k, k, k, off[:1]), ValueError),
+        (lambda: prompt_attention(k, k, k, off, kv_offsets=off[:1]), ValueError),
+        (lambda: prompt_attention(k, k, k, off, out=k[:1]), ValueError),
+        (lambda: prompt_attention(k.transpose(1, 2), k, k, off), NotImplementedError),
+        (lambda: kv_append(k, k[:1], kc, vc, slots), ValueError),
+        (lambda: kv_append(k, k, kc, vc[:1], slots), ValueError),
+        (lambda: kv_append(k, k, kc, vc, slots.long()), ValueError),
+        (lambda: kv_append(k, k, kc, vc, slots, positions=slots), ValueError),
+        (lambda: kv_append(k, k, kc, vc, slots, positions=slots, table=torch.zeros(8, 24, device="cuda")),
+         NotImplementedError),
+        (lambda: kv_append(k, k, kc, vc, slots, q_out=k), ValueError),
+    ]:
+        with pytest.raises(kind):
+            call()
+        q.requires_grad_(False)
+
+
+def test_empty_calls():
+    import torch
+    from ktir_cpu_b200 import check_status, kv_append, paged_decode, prompt_attention
+    e = torch.zeros(0, 4, 64, dtype=torch.bfloat16, device="cuda")
+    c = torch.zeros(3, 8, 2, 64, dtype=torch.bfloat16, device="cuda")
+    none = torch.zeros(0, dtype=torch.int32, device="cuda")
+    assert paged_decode(e, c, c, none.view(0, 0), none).shape == (0, 4, 64)
+    off = torch.zeros(3, dtype=torch.int32, device="cuda")
+    assert prompt_attention(e, e[:, :2], e[:, :2], off).shape == (0, 4, 64)
+    kv_append(e[:, :2], e[:, :2], c, c.clone(), none)
+    check_status()
+
+
+def test_prompt_then_decode_agree():
+    """A prompt read in one pass, and the same tokens one at a time over the cache."""
+    import torch
+    from ktir_cpu_b200 import check_status, kv_append, paged_decode, prompt_attention, rotary_table
+    gen = _gen(23)
+    n, heads, kv_heads, dim, page = 70, 8, 2, 128, 16
+    q, k, v = _randn(gen, "bf16", n, heads, dim), _randn(gen, "bf16", n, kv_heads, dim), _randn(gen, "bf16", n, kv_heads, dim)
+    kc, vc = (torch.zeros(6, page, kv_heads, dim, dtype=torch.bfloat16, device="cuda") for _ in range(2))
+    pages = torch.tensor([[4, 0, 5, 2, 1]], dtype=torch.int32, device="cuda")
+    at = torch.arange(n, device="cuda")
+    slots = (pages[0].long()[at // page] * page + at % page).int()
+    args = dict(table=rotary_table(128, dim))
+    turned = kv_append(k, v, kc, vc, slots, q=q, positions=at.int(), **args)
+    keys = kc[slots.long() // page, slots.long() % page]
+    whole = prompt_attention(turned, keys, v, torch.tensor([0, n], dtype=torch.int32, device="cuda"))
+    # each side: one rounding of the output and one of the weights, both relative to at most max |v|
+    bound = 2 * 2 * S.U["bf16"] * float(v.abs().max()) * 1.01
+    for i in range(n):
+        one = paged_decode(turned[i:i + 1], kc, vc, pages, torch.tensor([i + 1], dtype=torch.int32, device="cuda"))
+        assert (one[0].double() - whole[i].double()).abs().max() <= bound
+    check_status()
