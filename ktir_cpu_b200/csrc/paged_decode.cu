@@ -3,8 +3,28 @@
 //   o = sum_j e^(x_j - m) v_j / l,   l = sum_j e^(x_j - m),   m = max_j x_j,
 //   x_j = scale q . k_j
 //
-// One warp per (sequence, head): the keys one after the other, m, l and o in
-// f32 registers (o scaled by e^(m - m') when the maximum moves to m').
+// Bound by memory: every cached key and value is read once and meets the g =
+// heads / kv_heads queries that share it, 2 g operations per byte.  So the
+// cache streams through shared memory in 16-byte asynchronous copies, and the
+// two products run on mma.sync (m16n8k16, up to 16 query heads as its rows; a
+// larger g takes several head tiles), which tcgen05's 64 or 128 rows would
+// leave mostly empty.
+//
+// Split over the cache: the 64-key tiles of all sequences form one list, cut
+// into equal stretches, one per group of CTAs; the CTAs of a group take the
+// head tiles over the same stretch (so a page's heads, neighbours in a
+// token-major cache, are read at the same time).  The work is even however the
+// lengths differ.  Within a CTA each of the four warps owns 16 keys of every
+// tile, with its own ring of copies in flight, its own running m, l and o: the
+// warps meet only where a sequence ends.  A stretch that holds part of a
+// sequence leaves (m, l, o) in the workspace, and the last of the CTAs that
+// share the sequence joins the parts in the order of the list (so the result
+// does not depend on which was last).
+//
+// Precision: scores, m, l and o in f32; the weights p are rounded to the
+// element type for the second product (as the values are), at most one half
+// ulp each.  m moves only when the maximum grows by more than 2^8, so p stays
+// below 2^8 and the largest p of a row is at least 1.
 #include "serve_common.cuh"
 
 using namespace ktir::serve;
@@ -12,75 +32,483 @@ using namespace ktir::serve;
 namespace {
 
 constexpr int WARPS = 4;
+constexpr int THREADS = WARPS * 32;
+constexpr int KPW = 16;                    // keys per warp and tile
+constexpr int TILE = WARPS * KPW;          // keys per tile
+constexpr int ROWS = 16;                   // query heads per head tile
+constexpr int CTAS_PER_SM = 2;
+constexpr int MAX_CTAS = 512;              // of a launch that splits sequences
+constexpr int MIN_TILES = 2;               // per stretch: both in flight at once
+constexpr float RESCALE_THRESHOLD = 8.0f;  // log2 units
+constexpr int PART_STRIDE = ROWS * (128 + 2);   // floats of a part: o, then (m, l) per row
+constexpr int64_t PARTS_BYTES = (int64_t)MAX_CTAS * 2 * PART_STRIDE * 4;
+
+struct DecodeParams {
+  KtirPagedDecodeDesc d;
+  int group;          // query heads per kv head
+  int htiles;         // head tiles per kv head
+  int ht;             // kv_heads * htiles
+  int groups;         // CTA groups of the launch
+  int page_shift;     // log2(page_size), or -1
+  float* parts;
+  int* counters;      // [batch][ht], zero between calls
+};
+
+template <typename T>
+__device__ __forceinline__ void mma16816(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1);
+template <>
+__device__ __forceinline__ void mma16816<__half>(float (&c)[4], const uint32_t (&a)[4], uint32_t b0,
+                                                 uint32_t b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, "
+      "{%0,%1,%2,%3};"
+      : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+template <>
+__device__ __forceinline__ void mma16816<__nv_bfloat16>(float (&c)[4], const uint32_t (&a)[4],
+                                                        uint32_t b0, uint32_t b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, "
+      "{%0,%1,%2,%3};"
+      : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+
+__device__ __forceinline__ void ldsm4(uint32_t (&r)[4], uint32_t addr) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+               : "r"(addr)
+               : "memory");
+}
+__device__ __forceinline__ void ldsm4t(uint32_t (&r)[4], uint32_t addr) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+               : "r"(addr)
+               : "memory");
+}
+// 16 bytes, or 16 zero bytes where `bytes` is 0 (nothing is read then)
+__device__ __forceinline__ void cp16(uint32_t dst, const void* src, int bytes) {
+  asm volatile("cp.async.cg.shared.global.L2::128B [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes)
+               : "memory");
+}
+__device__ __forceinline__ void cp_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void cp_wait() {
+  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+}
+
+// where a stretch stands: tile t of sequence b's nt tiles (len keys)
+struct Cursor {
+  long long b;
+  int t, nt, len;
+};
 
 template <typename T, int D>
-__global__ void __launch_bounds__(WARPS * 32)
-    k_paged_decode(const __grid_constant__ KtirPagedDecodeDesc d) {
-  constexpr int E = D / 32;            // elements per lane
-  const long long item = (long long)blockIdx.x * WARPS + (threadIdx.x >> 5);
-  if (item >= d.batch * d.heads) return;
-  const int lane = threadIdx.x & 31;
-  const long long b = item / d.heads;
-  const int h = (int)(item - b * d.heads);
-  const int g = h / (d.heads / d.kv_heads);
-  const float sl = d.scale * LOG2E;
-  int len = d.lengths[b];
-  if (len < 0 || len > d.max_pages * d.page_size) {
-    if (lane == 0) atomicOr(d.status, KTIR_STATUS_BAD_INDEX);
-    len = 0;
+struct Cfg {
+  static constexpr int CHUNKS = D / 8;                 // 16-byte pieces of a row
+  static constexpr int ROW_BYTES = D * 2;
+  static constexpr int HALF_STAGE = KPW * ROW_BYTES;   // K, then V
+  static constexpr int STAGE = 2 * HALF_STAGE;
+  static constexpr int STAGES = D == 128 ? 3 : 6;      // 24 KiB in flight per warp
+  static constexpr int RING = WARPS * STAGES * STAGE;
+  static constexpr int JOIN = 2 * ROWS * D * 4;        // two warps' outputs
+  static constexpr int SMEM = RING + JOIN;
+};
+
+template <typename T, int D>
+__global__ void __launch_bounds__(THREADS, CTAS_PER_SM)
+    k_paged_decode(const __grid_constant__ DecodeParams p) {
+  using C = Cfg<T, D>;
+  const KtirPagedDecodeDesc& d = p.d;
+  extern __shared__ __align__(128) uint8_t smem[];
+  __shared__ long long s_scan[WARPS];
+  __shared__ long long s_start[2];                     // sequence, tile in it
+  __shared__ float2 s_ml[WARPS][ROWS];
+  __shared__ int s_last;
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int grp = blockIdx.x / p.ht, ht = blockIdx.x - grp * p.ht;
+  const int kvh = ht / p.htiles, head0 = kvh * p.group + (ht - kvh * p.htiles) * ROWS;
+  const int nrows = min(ROWS, (kvh + 1) * p.group - head0);
+  const long long most = d.max_pages * d.page_size;
+
+  // tiles of a sequence; a length outside its range counts as 0
+  auto length_of = [&](long long b) -> int {
+    const int len = d.lengths[b];
+    return len < 0 || len > most ? 0 : len;
+  };
+
+  // this stretch of the list: an exclusive scan over runs of sequences
+  const long long per = (d.batch + THREADS - 1) / THREADS;
+  const long long r0 = min((long long)d.batch, tid * per), r1 = min((long long)d.batch, r0 + per);
+  long long mine = 0;
+  for (long long b = r0; b < r1; ++b) {
+    const int len = d.lengths[b];
+    if (len < 0 || len > most) {
+      if (blockIdx.x == 0) atomicOr(d.status, KTIR_STATUS_BAD_INDEX);
+    } else {
+      mine += (len + TILE - 1) / TILE;
+    }
   }
-  float q[E], o[E], m = -INFINITY, l = 0.f;
-  const T* qp = static_cast<const T*>(d.q) + b * d.q_stride[0] + h * d.q_stride[1] + lane * E;
+  long long incl = mine;
 #pragma unroll
-  for (int i = 0; i < E; i += 2) {
-    const float2 x = Elem<T>::to2(*reinterpret_cast<const uint32_t*>(qp + i));
-    q[i] = x.x * sl;
-    q[i + 1] = x.y * sl;
-    o[i] = o[i + 1] = 0.f;
+  for (int w = 1; w < 32; w <<= 1) {
+    const long long o = __shfl_up_sync(0xffffffffu, incl, w);
+    if (lane >= w) incl += o;
   }
-  for (int j = 0; j < len; ++j) {
-    const int page = d.pages[b * d.page_row + j / d.page_size];
-    if (page < 0 || page >= d.num_pages) {
-      if (lane == 0) atomicOr(d.status, KTIR_STATUS_BAD_INDEX);
+  if (lane == 31) s_scan[warp] = incl;
+  __syncthreads();
+  long long before = 0, total = 0;
+#pragma unroll
+  for (int w = 0; w < WARPS; ++w) {
+    if (w < warp) before += s_scan[w];
+    total += s_scan[w];
+  }
+  // sequences without keys give zeros
+  for (long long b = grp; b < d.batch; b += p.groups) {
+    if (length_of(b) == 0) {
+      for (int i = tid; i < nrows * C::CHUNKS; i += THREADS) {
+        const int r = i / C::CHUNKS, c = i - r * C::CHUNKS;
+        *reinterpret_cast<uint4*>(static_cast<T*>(d.out) + b * d.out_stride[0] +
+                                  (head0 + r) * d.out_stride[1] + c * 8) = make_uint4(0, 0, 0, 0);
+      }
+      if (d.lse && tid < nrows) d.lse[b * d.heads + head0 + tid] = -INFINITY;
+    }
+  }
+  const long long want = (total + MIN_TILES - 1) / MIN_TILES;
+  const long long ng = min((long long)p.groups, want);
+  if (grp >= ng) return;
+  const long long t_begin = total * grp / ng, t_end = total * (grp + 1) / ng;
+  const int n = (int)(t_end - t_begin);
+  const long long excl = before + incl - mine;
+  if (t_begin >= excl && t_begin < excl + mine) {
+    long long at = excl;
+    for (long long b = r0; b < r1; ++b) {
+      const int nt = (length_of(b) + TILE - 1) / TILE;
+      if (t_begin < at + nt) {
+        s_start[0] = b;
+        s_start[1] = t_begin - at;
+        break;
+      }
+      at += nt;
+    }
+  }
+  __syncthreads();
+
+  auto open = [&](Cursor& c, long long b) {   // the next sequence from b on that has keys
+    c.b = b;
+    c.t = 0;
+    while (c.b < d.batch - 1 && length_of(c.b) == 0) ++c.b;
+    c.len = length_of(c.b);
+    c.nt = (c.len + TILE - 1) / TILE;
+  };
+  auto step = [&](Cursor& c) {
+    if (++c.t == c.nt) open(c, c.b + 1);
+  };
+  Cursor get, use;
+  open(get, s_start[0]);
+  get.t = (int)s_start[1];
+  use = get;
+  long long base = t_begin - get.t;           // first tile of use's sequence in the list
+
+  const uint32_t ring = (uint32_t)__cvta_generic_to_shared(smem) + warp * (C::STAGES * C::STAGE);
+  float* join = reinterpret_cast<float*>(smem + C::RING);
+
+  // -- copies: lane l < 16 looks up key l of the warp's 16 one tile ahead ------
+  int page = -1, place = 0;
+  auto look = [&]() {                         // page and place for cursor `get`
+    const int key = get.t * TILE + warp * KPW + (lane & 15);
+    page = -1;
+    if (key < get.len) {
+      const int pi = p.page_shift >= 0 ? key >> p.page_shift : key / (int)d.page_size;
+      place = key - pi * (int)d.page_size;
+      page = d.pages[get.b * d.page_row + pi];
+      if (page < 0 || page >= d.num_pages) {
+        atomicOr(d.status, KTIR_STATUS_BAD_INDEX);
+        page = -1;
+      }
+    }
+  };
+  int got = 0;                                // tiles issued
+  auto issue = [&]() {
+    if (got < n) {
+      const uint32_t st = ring + (got % C::STAGES) * C::STAGE;
+      const long long ko = page < 0 ? -1 : page * d.kc_stride[0] + place * d.kc_stride[1] + kvh * d.kc_stride[2];
+      const long long vo = page < 0 ? -1 : page * d.vc_stride[0] + place * d.vc_stride[1] + kvh * d.vc_stride[2];
+      if (++got < n) {                        // the next tile's pages are on their way meanwhile
+        step(get);
+        look();
+      }
+      const int c = lane % C::CHUNKS;
+      constexpr int PER = 32 / C::CHUNKS;     // rows per instruction
+#pragma unroll
+      for (int i = 0; i < KPW / PER; ++i) {
+        const int r = i * PER + lane / C::CHUNKS;
+        const long long k = __shfl_sync(0xffffffffu, ko, r), v = __shfl_sync(0xffffffffu, vo, r);
+        const uint32_t dst = st + r * C::ROW_BYTES + ((c ^ (r & 7)) << 4);
+        cp16(dst, static_cast<const T*>(d.k_cache) + (k < 0 ? 0 : k + c * 8), k < 0 ? 0 : 16);
+        cp16(dst + C::HALF_STAGE, static_cast<const T*>(d.v_cache) + (v < 0 ? 0 : v + c * 8), v < 0 ? 0 : 16);
+      }
+    }
+    cp_commit();
+  };
+  look();
+#pragma unroll
+  for (int s = 0; s < C::STAGES - 1; ++s) issue();
+
+  uint32_t qa[D / 16][4];
+  float o[D / 8][4], m[2], l[2];
+  const float sl = d.scale * LOG2E;
+  const int row = lane >> 2, col = (lane & 3) * 2;
+
+  for (int i = 0; i < n; ++i) {
+    if (i == 0 || use.t == 0) {
+      // a sequence begins (or this stretch of it): its queries, and nothing summed yet
+      const T* q = static_cast<const T*>(d.q) + use.b * d.q_stride[0];
+#pragma unroll
+      for (int k = 0; k < D / 16; ++k)
+#pragma unroll
+        for (int x = 0; x < 4; ++x) {
+          const int r = row + (x & 1) * 8;
+          qa[k][x] = r < nrows ? *reinterpret_cast<const uint32_t*>(q + (head0 + r) * d.q_stride[1] + k * 16 +
+                                                                     (x >> 1) * 8 + col)
+                               : 0u;
+        }
+#pragma unroll
+      for (int k = 0; k < D / 8; ++k) o[k][0] = o[k][1] = o[k][2] = o[k][3] = 0.f;
+      m[0] = m[1] = -INFINITY;
+      l[0] = l[1] = 0.f;
+    }
+    cp_wait<C::STAGES - 2>();
+    __syncwarp();                             // every lane's copies of tile i, and its reads of tile i - 1
+    issue();
+    const uint32_t kt = ring + (i % C::STAGES) * C::STAGE, vt = kt + C::HALF_STAGE;
+
+    // x = q k^T for 16 keys: s[0] keys 0-7, s[1] keys 8-15
+    float s[2][4] = {};
+#pragma unroll
+    for (int k = 0; k < D / 16; ++k) {
+      uint32_t b[4];
+      const int r = (lane & 7) + ((lane >> 4) << 3), c = 2 * k + ((lane >> 3) & 1);
+      ldsm4(b, kt + r * C::ROW_BYTES + ((c ^ (r & 7)) << 4));
+      mma16816<T>(s[0], qa[k], b[0], b[1]);
+      mma16816<T>(s[1], qa[k], b[2], b[3]);
+    }
+    const int left = use.len - use.t * TILE - warp * KPW;      // keys of the 16 that exist
+#pragma unroll
+    for (int h = 0; h < 2; ++h)
+#pragma unroll
+      for (int x = 0; x < 4; ++x) {
+        s[h][x] = 8 * h + col + (x & 1) < left ? s[h][x] * sl : -INFINITY;
+      }
+    float top[2];
+#pragma unroll
+    for (int r = 0; r < 2; ++r) {
+      top[r] = fmaxf(fmaxf(s[0][2 * r], s[0][2 * r + 1]), fmaxf(s[1][2 * r], s[1][2 * r + 1]));
+      top[r] = fmaxf(top[r], __shfl_xor_sync(0xffffffffu, top[r], 1));
+      top[r] = fmaxf(top[r], __shfl_xor_sync(0xffffffffu, top[r], 2));
+    }
+    if (__any_sync(0xffffffffu, top[0] > m[0] + RESCALE_THRESHOLD || top[1] > m[1] + RESCALE_THRESHOLD)) {
+#pragma unroll
+      for (int r = 0; r < 2; ++r) {
+        const float mn = fmaxf(m[r], top[r]);
+        const float f = mn == -INFINITY ? 1.f : ex2(m[r] - mn);
+        m[r] = mn;
+        l[r] *= f;
+#pragma unroll
+        for (int k = 0; k < D / 8; ++k) {
+          o[k][2 * r] *= f;
+          o[k][2 * r + 1] *= f;
+        }
+      }
+    }
+    uint32_t pa[4];
+#pragma unroll
+    for (int r = 0; r < 2; ++r) {
+      const float sub = m[r] == -INFINITY ? 0.f : m[r];
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const float a = ex2(s[h][2 * r] - sub), b = ex2(s[h][2 * r + 1] - sub);
+        l[r] += a + b;
+        pa[2 * h + r] = Elem<T>::from2(a, b);
+      }
+    }
+    // o += p v
+#pragma unroll
+    for (int k = 0; k < D / 16; ++k) {
+      uint32_t b[4];
+      const int r = (lane & 7) + (((lane >> 3) & 1) << 3), c = 2 * k + (lane >> 4);
+      ldsm4t(b, vt + r * C::ROW_BYTES + ((c ^ (r & 7)) << 4));
+      mma16816<T>(o[2 * k], pa, b[0], b[1]);
+      mma16816<T>(o[2 * k + 1], pa, b[2], b[3]);
+    }
+
+    if (use.t + 1 < use.nt && i + 1 < n) {
+      ++use.t;
       continue;
     }
-    const long long place = j % d.page_size;
-    const T* k = static_cast<const T*>(d.k_cache) + page * d.kc_stride[0] + place * d.kc_stride[1] +
-                 g * d.kc_stride[2] + lane * E;
-    const T* v = static_cast<const T*>(d.v_cache) + page * d.vc_stride[0] + place * d.vc_stride[1] +
-                 g * d.vc_stride[2] + lane * E;
-    float x = 0.f;
+    // -- the sequence, or this stretch of it, ends: join the warps ---------------
 #pragma unroll
-    for (int i = 0; i < E; i += 2) {
-      const float2 kk = Elem<T>::to2(*reinterpret_cast<const uint32_t*>(k + i));
-      x += q[i] * kk.x + q[i + 1] * kk.y;
+    for (int r = 0; r < 2; ++r) {
+      l[r] += __shfl_xor_sync(0xffffffffu, l[r], 1);
+      l[r] += __shfl_xor_sync(0xffffffffu, l[r], 2);
     }
-#pragma unroll
-    for (int w = 16; w; w >>= 1) x += __shfl_xor_sync(0xffffffffu, x, w);
-    const float mn = fmaxf(m, x);
-    const float f = mn == -INFINITY ? 1.f : ex2(m - mn), e = mn == -INFINITY ? 0.f : ex2(x - mn);
-    m = mn;
-    l = l * f + e;
-#pragma unroll
-    for (int i = 0; i < E; i += 2) {
-      const float2 vv = Elem<T>::to2(*reinterpret_cast<const uint32_t*>(v + i));
-      o[i] = o[i] * f + e * vv.x;
-      o[i + 1] = o[i + 1] * f + e * vv.y;
+    if ((lane & 3) == 0) {
+      s_ml[warp][row] = make_float2(m[0], l[0]);
+      s_ml[warp][row + 8] = make_float2(m[1], l[1]);
     }
+    __syncthreads();
+    float mt[2], lt[2];
+#pragma unroll
+    for (int r = 0; r < 2; ++r) {
+      mt[r] = -INFINITY;
+#pragma unroll
+      for (int w = 0; w < WARPS; ++w) mt[r] = fmaxf(mt[r], s_ml[w][row + 8 * r].x);
+      const float sub = mt[r] == -INFINITY ? 0.f : mt[r];
+      lt[r] = 0.f;
+#pragma unroll
+      for (int w = 0; w < WARPS; ++w) lt[r] += s_ml[w][row + 8 * r].y * ex2(s_ml[w][row + 8 * r].x - sub);
+      const float f = ex2(m[r] - sub);
+#pragma unroll
+      for (int k = 0; k < D / 8; ++k) {
+        o[k][2 * r] *= f;
+        o[k][2 * r + 1] *= f;
+      }
+    }
+    auto put = [&](float* to) {
+#pragma unroll
+      for (int k = 0; k < D / 8; ++k)
+#pragma unroll
+        for (int r = 0; r < 2; ++r)
+          *reinterpret_cast<float2*>(to + (row + 8 * r) * D + k * 8 + col) = make_float2(o[k][2 * r], o[k][2 * r + 1]);
+    };
+    auto add = [&](const float* from) {
+#pragma unroll
+      for (int k = 0; k < D / 8; ++k)
+#pragma unroll
+        for (int r = 0; r < 2; ++r) {
+          const float2 x = *reinterpret_cast<const float2*>(from + (row + 8 * r) * D + k * 8 + col);
+          o[k][2 * r] += x.x;
+          o[k][2 * r + 1] += x.y;
+        }
+    };
+    if (warp >= 2) put(join + (warp - 2) * ROWS * D);
+    __syncthreads();
+    if (warp < 2) add(join + warp * ROWS * D);
+    if (warp == 1) put(join + ROWS * D);
+    __syncthreads();
+    const long long end = base + use.nt;
+    const bool whole = base >= t_begin && end <= t_end;
+    if (warp == 0) {
+      add(join + ROWS * D);
+      if (whole) {
+        T* out = static_cast<T*>(d.out) + use.b * d.out_stride[0];
+#pragma unroll
+        for (int r = 0; r < 2; ++r) {
+          if (row + 8 * r < nrows) {
+            const float inv = lt[r] == 0.f ? 0.f : 1.f / lt[r];   // every score -inf: nothing to weigh
+#pragma unroll
+            for (int k = 0; k < D / 8; ++k)
+              *reinterpret_cast<uint32_t*>(out + (head0 + row + 8 * r) * d.out_stride[1] + k * 8 + col) =
+                  Elem<T>::from2(o[k][2 * r] * inv, o[k][2 * r + 1] * inv);
+            if (d.lse && (lane & 3) == 0)
+              d.lse[use.b * d.heads + head0 + row + 8 * r] = (mt[r] + log2f(lt[r])) * LN2;
+          }
+        }
+      } else {
+        float* part = p.parts + ((long long)blockIdx.x * 2 + (base >= t_begin ? 1 : 0)) * PART_STRIDE;
+        put(part);
+        if ((lane & 3) == 0) {
+          float2* ml = reinterpret_cast<float2*>(part + ROWS * D);
+          ml[row] = make_float2(mt[0], lt[0]);
+          ml[row + 8] = make_float2(mt[1], lt[1]);
+        }
+        __threadfence();
+      }
+    }
+    if (!whole) {
+      // stretches that share the sequence: those of its first to its last tile
+      const long long g0 = ((base + 1) * ng - 1) / total, g1 = (end * ng - 1) / total;
+      __syncthreads();
+      if (tid == 0) {
+        int* counter = p.counters + use.b * p.ht + ht;
+        const int before = atomicAdd(counter, 1);
+        s_last = before == (int)(g1 - g0);
+        if (s_last) *counter = 0;
+        __threadfence();
+      }
+      __syncthreads();
+      if (s_last) {
+        for (int e = tid; e < nrows * (D / 4); e += THREADS) {
+          const int r = e / (D / 4), c = (e - r * (D / 4)) * 4;
+          float mm = -INFINITY, ll = 0.f;
+          float4 oo = make_float4(0.f, 0.f, 0.f, 0.f);
+          for (long long g = g0; g <= g1; ++g) {
+            // the first part ends its stretch, the others begin theirs
+            const bool begins = base >= total * g / ng;
+            const float* part = p.parts + ((g * p.ht + ht) * 2 + (begins ? 1 : 0)) * PART_STRIDE;
+            const float2 ml = __ldcg(reinterpret_cast<const float2*>(part + ROWS * D) + r);
+            const float4 x = __ldcg(reinterpret_cast<const float4*>(part + r * D + c));
+            const float mn = fmaxf(mm, ml.x);
+            const float sub = mn == -INFINITY ? 0.f : mn;
+            const float f = ex2(mm - sub), w = ex2(ml.x - sub);
+            mm = mn;
+            ll = ll * f + ml.y * w;
+            oo.x = oo.x * f + x.x * w;
+            oo.y = oo.y * f + x.y * w;
+            oo.z = oo.z * f + x.z * w;
+            oo.w = oo.w * f + x.w * w;
+          }
+          const float inv = ll == 0.f ? 0.f : 1.f / ll;
+          uint2 v;
+          v.x = Elem<T>::from2(oo.x * inv, oo.y * inv);
+          v.y = Elem<T>::from2(oo.z * inv, oo.w * inv);
+          *reinterpret_cast<uint2*>(static_cast<T*>(d.out) + use.b * d.out_stride[0] +
+                                    (head0 + r) * d.out_stride[1] + c) = v;
+          if (d.lse && c == 0) d.lse[use.b * d.heads + head0 + r] = (mm + log2f(ll)) * LN2;
+        }
+      }
+    }
+    base = end;
+    if (i + 1 < n) open(use, use.b + 1);
   }
-  const float inv = l > 0.f ? 1.f / l : 0.f;
-  T* out = static_cast<T*>(d.out) + b * d.out_stride[0] + h * d.out_stride[1] + lane * E;
-#pragma unroll
-  for (int i = 0; i < E; i += 2)
-    *reinterpret_cast<uint32_t*>(out + i) = Elem<T>::from2(o[i] * inv, o[i + 1] * inv);
-  if (d.lse && lane == 0) d.lse[b * d.heads + h] = l > 0.f ? (m + log2f(l)) * LN2 : -INFINITY;
+}
+
+template <typename T, int D>
+int launch(const DecodeParams& p, unsigned grid, cudaStream_t stream) {
+  // the attribute is per device
+  static bool ready[64] = {};
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64)
+    return ktir_set_error(KTIR_ERR_CUDA, "ktir_paged_decode: no usable current device");
+  if (!ready[dev]) {
+    if (cudaFuncSetAttribute(k_paged_decode<T, D>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                             Cfg<T, D>::SMEM) != cudaSuccess)
+      return ktir_set_error(KTIR_ERR_CUDA, "ktir_paged_decode: shared-memory attribute refused");
+    ready[dev] = true;
+  }
+  k_paged_decode<T, D><<<grid, THREADS, Cfg<T, D>::SMEM, stream>>>(p);
+  return launched("ktir_paged_decode: launch failed");
+}
+
+int sm_count() {
+  static int count[64] = {};
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return 0;
+  if (!count[dev] && cudaDeviceGetAttribute(&count[dev], cudaDevAttrMultiProcessorCount, dev) != cudaSuccess)
+    return 0;
+  return count[dev];
 }
 
 }  // namespace
 
 extern "C" int64_t ktir_paged_decode_workspace(int64_t batch, int32_t heads, int32_t kv_heads,
                                                int32_t dim) {
-  return batch > 0 && heads > 0 && kv_heads > 0 && dim > 0 ? 256 : 0;
+  if (batch < 1 || heads < 1 || kv_heads < 1 || dim < 1) return 0;
+  const int64_t htiles = (heads / kv_heads + ROWS - 1) / ROWS;
+  // the parts first, at a size of their own: the counters keep their places
+  // (and their zeros) between calls of different batches
+  return PARTS_BYTES + batch * kv_heads * htiles * 4;
 }
 
 extern "C" int ktir_paged_decode(const KtirPagedDecodeDesc* d, void* stream) {
@@ -96,7 +524,7 @@ extern "C" int ktir_paged_decode(const KtirPagedDecodeDesc* d, void* stream) {
   if (d->batch < 0 || d->heads < 1 || d->kv_heads < 1 || d->heads % d->kv_heads ||
       d->heads > (1 << 16) || d->batch > (1 << 24) || d->num_pages < 1 || d->page_size < 1 ||
       d->max_pages < 1 || d->num_pages > 0x7fffffffLL || d->page_size > 0x7fffffffLL ||
-      d->max_pages > 0x7fffffffLL)
+      d->max_pages > 0x7fffffffLL || d->max_pages * d->page_size > 0x7fffff00LL)
     return ktir_set_error(KTIR_ERR_ARG, "ktir_paged_decode: extent out of range");
   if (!(d->scale > 0.f) || !isfinite(d->scale))
     return ktir_set_error(KTIR_ERR_UNSUPPORTED, "ktir_paged_decode: needs a positive, finite scale");
@@ -109,15 +537,29 @@ extern "C" int ktir_paged_decode(const KtirPagedDecodeDesc* d, void* stream) {
                           "ktir_paged_decode: head vectors must start on 16-byte boundaries");
   if (d->workspace_bytes < ktir_paged_decode_workspace(d->batch, d->heads, d->kv_heads, d->dim))
     return ktir_set_error(KTIR_ERR_ARG, "ktir_paged_decode: workspace too small");
-  const unsigned grid = (unsigned)((d->batch * d->heads + WARPS - 1) / WARPS);
+  const int sms = sm_count();
+  if (sms < 1) return ktir_set_error(KTIR_ERR_CUDA, "ktir_paged_decode: no usable current device");
+  DecodeParams p;
+  p.d = *d;
+  p.group = d->heads / d->kv_heads;
+  p.htiles = (p.group + ROWS - 1) / ROWS;
+  p.ht = d->kv_heads * p.htiles;
+  p.parts = static_cast<float*>(d->workspace);
+  p.counters = reinterpret_cast<int*>(static_cast<char*>(d->workspace) + PARTS_BYTES);
+  p.page_shift = -1;
+  if ((d->page_size & (d->page_size - 1)) == 0)
+    for (p.page_shift = 0; (1LL << p.page_shift) < d->page_size; ++p.page_shift) {}
+  // one resident wave of CTAs, no more groups than the cache could have stretches
+  int slots = sms * CTAS_PER_SM;
+  if (slots > MAX_CTAS) slots = MAX_CTAS;
+  long long groups = slots / p.ht;
+  const __int128 tiles = (__int128)d->batch * ((d->max_pages * d->page_size + TILE - 1) / TILE);
+  if (groups > (tiles + MIN_TILES - 1) / MIN_TILES) groups = (long long)((tiles + MIN_TILES - 1) / MIN_TILES);
+  if (groups < 1) groups = 1;
+  p.groups = (int)groups;
+  const unsigned grid = (unsigned)(groups * p.ht);
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   const bool f16 = d->dtype == KTIR_F16;
-  if (d->dim == 64) {
-    if (f16) k_paged_decode<__half, 64><<<grid, WARPS * 32, 0, s>>>(*d);
-    else k_paged_decode<__nv_bfloat16, 64><<<grid, WARPS * 32, 0, s>>>(*d);
-  } else {
-    if (f16) k_paged_decode<__half, 128><<<grid, WARPS * 32, 0, s>>>(*d);
-    else k_paged_decode<__nv_bfloat16, 128><<<grid, WARPS * 32, 0, s>>>(*d);
-  }
-  return launched("ktir_paged_decode: launch failed");
+  if (d->dim == 64) return f16 ? launch<__half, 64>(p, grid, s) : launch<__nv_bfloat16, 64>(p, grid, s);
+  return f16 ? launch<__half, 128>(p, grid, s) : launch<__nv_bfloat16, 128>(p, grid, s);
 }
