@@ -477,10 +477,9 @@ __global__ void __launch_bounds__(THREADS, CTAS_PER_SM)
 template <typename T, int D>
 int launch(const DecodeParams& p, unsigned grid, cudaStream_t stream) {
   // the attribute is per device
-  static bool ready[64] = {};
-  int dev = 0;
-  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64)
-    return ktir_set_error(KTIR_ERR_CUDA, "ktir_paged_decode: no usable current device");
+  static bool ready[MAX_DEVICES] = {};
+  const int dev = current_device();
+  if (dev < 0) return ktir_set_error(KTIR_ERR_CUDA, "ktir_paged_decode: no usable current device");
   if (!ready[dev]) {
     if (cudaFuncSetAttribute(k_paged_decode<T, D>, cudaFuncAttributeMaxDynamicSharedMemorySize,
                              Cfg<T, D>::SMEM) != cudaSuccess)
@@ -489,15 +488,6 @@ int launch(const DecodeParams& p, unsigned grid, cudaStream_t stream) {
   }
   k_paged_decode<T, D><<<grid, THREADS, Cfg<T, D>::SMEM, stream>>>(p);
   return launched("ktir_paged_decode: launch failed");
-}
-
-int sm_count() {
-  static int count[64] = {};
-  int dev = 0;
-  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return 0;
-  if (!count[dev] && cudaDeviceGetAttribute(&count[dev], cudaDevAttrMultiProcessorCount, dev) != cudaSuccess)
-    return 0;
-  return count[dev];
 }
 
 }  // namespace

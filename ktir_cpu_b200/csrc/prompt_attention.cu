@@ -1,85 +1,686 @@
-// Attention over packed prompts with grouped heads.
+// Attention over packed prompts with grouped heads, on the tensor cores.
 //
 // Query i of a sequence's n sees keys j <= i + m - n of its m when causal, all
-// of them otherwise; o = softmax(scale q K^T) V over those.  One warp per
-// (token, head): the keys one after the other, running maximum, sum and output
-// in f32 registers.
+// of them otherwise; o = softmax(scale q K^T) V over those.
+//
+// Bound by the tensor pipe and, about as tightly, by the exponentials: a tile
+// of 128 rows x 128 keys costs 2 x 128^2 x dim products (1,024 cycles at dim
+// 128) and 128^2 exponentials (16 per cycle and SM: 1,024 cycles).  So a CTA
+// (one per SM, persistent) works on two row tiles at once, one in the softmax
+// while the other is in the tensor pipe.
+//
+// A row is a (token, head) pair: the g = heads / kv_heads queries that share a
+// kv head lie side by side, 128 / g tokens per tile, so that every row of a
+// tile uses the same K and V whatever g is, and a short prompt fills more of a
+// tile.
+//
+// Roles, meeting only at mbarriers:
+//   warps 0-3, 4-7  the softmax of row tile 0 and 1, one row per thread:
+//                   S from TMEM, mask, running maximum and sum, P = 2^(x - m)
+//                   rounded to the element type back over S's columns, and at
+//                   a tile's end O / l to memory
+//   warp 8 (MMA)    S_w(j) = Q_w K_j^T (128 x 128 x dim) and O_w += P_w(j) V_j,
+//                   P read from TMEM; per row tile and block: PV_w(j), then
+//                   S_w(j+1) over the columns that held P_w(j) (the tensor pipe
+//                   runs one thread's products in order)
+//   warp 9 (TMA)    Q tiles, and K_j, V_j through one ring
+//   warp 10         sets V's rows past the sequence's last key to zero (they
+//                   belong to another sequence; a weight of 0 does not cancel
+//                   an infinity there)
+//   warp 11         finds the next tile: tiles are taken in order of falling
+//                   key counts over all sequences, back and forth over the
+//                   CTAs, so that the last ones to finish are the shortest
+// TMEM: S_0 0..127, S_1 128..255, O_0 and O_1 from 256 on, dim columns each.
+// The running maximum moves only when a row's maximum exceeds it by more than
+// 2^8; O's rows are then rescaled in TMEM, which S_w(j)'s completion allows:
+// PV_w(j-1) was issued before it.
+// Precision: S, O, m and l in f32; P is rounded to the element type for the
+// second product (tcgen05 wants one type for both operands), half an ulp per
+// weight; l adds the unrounded weights.
+// Every wait is bounded; one that runs out raises the CTA's abort flag, every
+// role then leaves its loop, waits for its own copies and products, and the
+// CTA still frees its TMEM.
+#include <cuda.h>
+
 #include "serve_common.cuh"
+#include "tc_common.cuh"
 
 using namespace ktir::serve;
+using namespace ktir::tc;
 
 namespace {
 
-constexpr int WARPS = 4;
+constexpr int BQ = 128;              // rows of a row tile
+constexpr int BK = 128;              // keys of a block
+constexpr int THREADS = 384;
+constexpr int SCHED = 4;             // tiles announced ahead
+constexpr int SCHED_READERS = 11;    // 8 softmax warps, MMA, TMA, V's tail
+constexpr float RESCALE_THRESHOLD = 8.0f;   // log2 units
+constexpr uint32_t TMEM_COLS = 512;
+constexpr uint32_t O_COL = 256;
+
+template <int D>
+struct Cfg {
+  static constexpr int PANEL = BK * 128;            // 128 rows of 64 elements, 128-byte swizzle
+  static constexpr int PANELS = D / 64;
+  static constexpr int TILE = PANELS * PANEL;       // a Q tile, a K block or a V block
+  static constexpr int STAGES = D == 128 ? 5 : 10;
+  static constexpr int BYTES = (2 + STAGES) * TILE;
+};
+constexpr int MAX_STAGES = 10;
+
+struct Tile {
+  int stop;
+  int token;      // first token of the tile (of row tile 0)
+  int tokens;     // of the sequence from there on
+  int seen;       // keys that the first token sees (causal)
+  int keys;       // of the sequence
+  int key0;       // its first key
+  int head;       // kv head
+  int blocks[2];  // key blocks of each row tile
+};
+
+struct Shared {
+  uint64_t q_full[2], q_empty[2];
+  uint64_t full[MAX_STAGES], empty[MAX_STAGES];
+  uint64_t s_full[2], p_full[2], pv_done[2], o_free[2];
+  uint64_t tail[MAX_STAGES];        // a V block with rows past the last key has arrived
+  uint64_t drain;
+  uint64_t sched_full[SCHED], sched_empty[SCHED];
+  Tile tile[SCHED];
+  uint32_t tmem_base;
+  int abort_flag;
+};
+
+struct PromptParams {
+  KtirPromptDesc d;
+  int group;            // query heads per kv head
+  int tile_tokens;      // tokens of a row tile
+  int k_head_step, v_head_step, q_head_step;   // 0 where all heads share one vector
+};
+
+__device__ __forceinline__ void tma_load_3d(uint32_t dst, const CUtensorMap* map, uint32_t bar, int x, int y,
+                                            int z) {
+  asm volatile(
+      "cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes"
+      " [%0], [%1, {%2, %3, %4}], [%5];" ::"r"(dst),
+      "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(z), "r"(bar)
+      : "memory");
+}
+
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float d;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+  return d;
+}
+
+// two f32 in a 64-bit register, one instruction for both
+__device__ __forceinline__ uint64_t pack2(float a, float b) {
+  uint64_t r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+  return r;
+}
+__device__ __forceinline__ void unpack2(uint64_t v, float& a, float& b) {
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(v));
+}
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+
+// -- the order of tiles -----------------------------------------------------------
+// Tile i of a sequence (n tokens, m keys) holds tokens [i T, (i + 1) T), T = two row
+// tiles; its weight is the number of key blocks that its last token sees.  Tiles
+// are numbered by falling weight over all sequences; within a weight by
+// sequence, and each tile once per kv head.
+struct Seq {
+  int n, m, tiles;
+};
+
+__device__ __forceinline__ Seq sequence(const KtirPromptDesc& d, long long b, int T, bool& bad) {
+  const int q0 = d.offsets[b], q1 = d.offsets[b + 1], k0 = d.kv_offsets[b], k1 = d.kv_offsets[b + 1];
+  bad = q0 < 0 || q1 < q0 || q1 > d.tokens || k0 < 0 || k1 < k0 || k1 > d.kv_tokens;
+  Seq s;
+  s.n = bad ? 0 : q1 - q0;
+  s.m = bad ? 0 : k1 - k0;
+  s.tiles = (s.n + T - 1) / T;
+  return s;
+}
+
+// tiles of weight at least `w`: the last ones of the sequence
+__device__ __forceinline__ int heavier(const Seq& s, int w, int T, int causal) {
+  if (w <= 0) return s.tiles;
+  const int need = (w - 1) * BK;             // more than this many keys seen
+  if (s.m <= need) return 0;
+  if (!causal) return s.tiles;
+  const int x = need - (s.m - s.n);          // (i + 1) T > x
+  return x <= 0 ? s.tiles : s.tiles - x / T;
+}
+
+__device__ __forceinline__ int warp_sum(int v) {
+#pragma unroll
+  for (int w = 16; w; w >>= 1) v += __shfl_xor_sync(0xffffffffu, v, w);
+  return v;
+}
+
+__device__ int tiles_of_weight(const KtirPromptDesc& d, int w, int T, int lane) {
+  int c = 0;
+  for (long long b = lane; b < d.batch; b += 32) {
+    bool bad;
+    c += heavier(sequence(d, b, T, bad), w, T, d.causal);
+  }
+  return warp_sum(c);
+}
+
+// tile number `x` (0 = heaviest), by one warp
+__device__ void find_tile(const KtirPromptDesc& d, int x, int head, int T, int heaviest, int lane, Tile& t) {
+  int lo = 0, hi = heaviest + 1;             // count(lo) > x >= count(hi)
+  int above = 0;
+  while (hi - lo > 1) {
+    const int mid = (lo + hi) >> 1;
+    const int c = tiles_of_weight(d, mid, T, lane);
+    if (c > x) {
+      lo = mid;
+    } else {
+      hi = mid;
+      above = c;
+    }
+  }
+  int r = x - above;
+  for (long long b0 = 0; b0 < d.batch; b0 += 32) {
+    const long long b = b0 + lane;
+    Seq s = {0, 0, 0};
+    int first = 0, count = 0;
+    bool bad;
+    if (b < d.batch) {
+      s = sequence(d, b, T, bad);
+      const int c = heavier(s, lo, T, d.causal);
+      count = c - heavier(s, lo + 1, T, d.causal);
+      first = s.tiles - c;
+    }
+    int incl = count;
+#pragma unroll
+    for (int w = 1; w < 32; w <<= 1) {
+      const int o = __shfl_up_sync(0xffffffffu, incl, w);
+      if (lane >= w) incl += o;
+    }
+    const int all = __shfl_sync(0xffffffffu, incl, 31);
+    if (r >= all) {
+      r -= all;
+      continue;
+    }
+    if (r >= incl - count && r < incl) {
+      const int i = first + r - (incl - count), at = i * T, half = T / 2;
+      t.stop = 0;
+      t.token = d.offsets[b] + at;
+      t.tokens = s.n - at;
+      t.seen = at + s.m - s.n + 1;
+      t.keys = s.m;
+      t.key0 = d.kv_offsets[b];
+      t.head = head;
+      for (int w = 0; w < 2; ++w) {
+        const int here = min(half, t.tokens - w * half);       // tokens of the row tile
+        const int end = d.causal ? min(s.m, at + w * half + here + s.m - s.n) : s.m;
+        t.blocks[w] = here > 0 && end > 0 ? (end + BK - 1) / BK : 0;
+      }
+    }
+    break;
+  }
+}
 
 template <typename T, int D>
-__global__ void __launch_bounds__(WARPS * 32)
-    k_prompt_attention(const __grid_constant__ KtirPromptDesc d) {
-  constexpr int E = D / 32;            // elements per lane
-  const long long item = (long long)blockIdx.x * WARPS + (threadIdx.x >> 5);
-  if (item >= d.tokens * d.heads) return;
-  const int lane = threadIdx.x & 31;
-  const long long t = item / d.heads;
-  const int h = (int)(item - t * d.heads);
-  const int g = h / (d.heads / d.kv_heads);
-  const float sl = d.scale * LOG2E;
-  // the sequence whose stretch of tokens holds t
-  long long lo = 0, hi = d.batch;
-  while (hi - lo > 1) {
-    const long long mid = (lo + hi) >> 1;
-    if (d.offsets[mid] <= t) lo = mid;
-    else hi = mid;
-  }
-  const long long q0 = d.offsets[lo], q1 = d.offsets[lo + 1];
-  const long long k0 = d.kv_offsets[lo], k1 = d.kv_offsets[lo + 1];
-  long long seen = 0;
-  if (t >= q0 && t < q1) {
-    if (k0 < 0 || k1 < k0 || k1 > d.kv_tokens) {
-      if (lane == 0) atomicOr(d.status, KTIR_STATUS_BAD_INDEX);
-    } else {
-      seen = k1 - k0;
-      if (d.causal) seen = min(seen, max(0LL, t - q0 + 1 + (k1 - k0) - (q1 - q0)));
+__global__ void __launch_bounds__(THREADS, 1)
+    k_prompt_attention(const __grid_constant__ CUtensorMap tq, const __grid_constant__ CUtensorMap tk,
+                       const __grid_constant__ CUtensorMap tv, const __grid_constant__ PromptParams p) {
+  using C = Cfg<D>;
+  constexpr uint32_t TYPE = sizeof(T) == 2 && Elem<T>::BF16 ? (1u << 7) | (1u << 10) : 0u;
+  constexpr int STAGES = C::STAGES;
+  extern __shared__ uint8_t smem_raw[];
+  __shared__ Shared B;
+  const KtirPromptDesc& d = p.d;
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const uint32_t base = (smem_u32(smem_raw) + 1023u) & ~1023u;
+  const uint32_t sQ = base, ring = base + 2 * C::TILE;
+  volatile int* abort = &B.abort_flag;
+
+  if (tid == 0) {
+    B.abort_flag = 0;
+    for (int w = 0; w < 2; ++w) {
+      mbar_init(smem_u32(&B.q_full[w]), 1);
+      mbar_init(smem_u32(&B.q_empty[w]), 1);
+      mbar_init(smem_u32(&B.s_full[w]), 1);
+      mbar_init(smem_u32(&B.p_full[w]), 4);
+      mbar_init(smem_u32(&B.pv_done[w]), 1);
+      mbar_init(smem_u32(&B.o_free[w]), 4);
     }
-  } else if (lane == 0) {
-    atomicOr(d.status, KTIR_STATUS_BAD_INDEX);
-  }
-  float q[E], o[E], m = -INFINITY, l = 0.f;
-  const T* qp = static_cast<const T*>(d.q) + t * d.q_stride[0] + h * d.q_stride[1] + lane * E;
-#pragma unroll
-  for (int i = 0; i < E; i += 2) {
-    const float2 x = Elem<T>::to2(*reinterpret_cast<const uint32_t*>(qp + i));
-    q[i] = x.x * sl;
-    q[i + 1] = x.y * sl;
-    o[i] = o[i + 1] = 0.f;
-  }
-  const T* kp = static_cast<const T*>(d.k) + k0 * d.k_stride[0] + g * d.k_stride[1] + lane * E;
-  const T* vp = static_cast<const T*>(d.v) + k0 * d.v_stride[0] + g * d.v_stride[1] + lane * E;
-  for (long long j = 0; j < seen; ++j) {
-    float x = 0.f;
-#pragma unroll
-    for (int i = 0; i < E; i += 2) {
-      const float2 kk = Elem<T>::to2(*reinterpret_cast<const uint32_t*>(kp + j * d.k_stride[0] + i));
-      x += q[i] * kk.x + q[i + 1] * kk.y;
+    for (int s = 0; s < STAGES; ++s) {
+      mbar_init(smem_u32(&B.full[s]), 1);
+      mbar_init(smem_u32(&B.empty[s]), 1);
+      mbar_init(smem_u32(&B.tail[s]), 1);
     }
+    mbar_init(smem_u32(&B.drain), 1);
+    for (int s = 0; s < SCHED; ++s) {
+      mbar_init(smem_u32(&B.sched_full[s]), 1);
+      mbar_init(smem_u32(&B.sched_empty[s]), SCHED_READERS);
+    }
+    fence_barrier_init();
+  }
+  if (warp == 8) {
+    tmem_alloc(smem_u32(&B.tmem_base), TMEM_COLS);
+    tmem_relinquish();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = B.tmem_base;
+
+  // announced tiles, read by whole warps: false at the end (or on an abort)
+  auto next_tile = [&](int k, Tile& t) -> bool {
+    const int s = k % SCHED;
+    if (!__all_sync(0xffffffffu, mbar_wait(smem_u32(&B.sched_full[s]), (k / SCHED) & 1, abort))) return false;
+    t = B.tile[s];
+    __syncwarp();
+    if (lane == 0) mbar_arrive(smem_u32(&B.sched_empty[s]));
+    return !t.stop;
+  };
+
+  if (warp == 11) {
+    // ---------------- tile finder ----------------
+    const int span = 2 * p.tile_tokens;
+    int heaviest = 0, total = 0;
+    bool any_bad = false;
+    for (long long b = lane; b < d.batch; b += 32) {
+      bool bad;
+      const Seq s = sequence(d, b, span, bad);
+      any_bad |= bad;
+      if (s.n) heaviest = max(heaviest, (s.m + BK - 1) / BK);
+      total += s.tiles;
+    }
+    if (blockIdx.x == 0) {
+      if (lane == 0) any_bad |= d.offsets[0] != 0 || d.offsets[d.batch] != d.tokens;
+      if (any_bad) atomicOr(d.status, KTIR_STATUS_BAD_INDEX);
+    }
+    total = warp_sum(total);
 #pragma unroll
-    for (int w = 16; w; w >>= 1) x += __shfl_xor_sync(0xffffffffu, x, w);
-    const float mn = fmaxf(m, x);
-    const float f = mn == -INFINITY ? 1.f : ex2(m - mn), e = mn == -INFINITY ? 0.f : ex2(x - mn);
-    m = mn;
-    l = l * f + e;
+    for (int w = 16; w; w >>= 1) heaviest = max(heaviest, __shfl_xor_sync(0xffffffffu, heaviest, w));
+    const long long all = (long long)total * d.kv_heads;
+    for (int k = 0;; ++k) {
+      const long long x = (long long)k * gridDim.x + ((k & 1) ? gridDim.x - 1 - blockIdx.x : blockIdx.x);
+      const int s = k % SCHED;
+      if (k >= SCHED &&
+          !__all_sync(0xffffffffu, mbar_wait(smem_u32(&B.sched_empty[s]), (k / SCHED - 1) & 1, abort)))
+        break;
+      // back and forth, a CTA may have a tile in the last round after having none before it
+      const bool stop = (long long)k * gridDim.x >= all;
+      if (stop) {
+        if (lane == 0) B.tile[s].stop = 1;
+      } else if (x < all) {
+        find_tile(d, (int)(x / d.kv_heads), (int)(x % d.kv_heads), span, heaviest, lane, B.tile[s]);
+      } else if (lane == 0) {
+        Tile& t = B.tile[s];
+        t.stop = 0;
+        t.tokens = t.blocks[0] = t.blocks[1] = t.keys = 0;
+        t.token = t.key0 = t.head = 0;
+        t.seen = 0;
+      }
+      __syncwarp();
+      if (lane == 0) mbar_arrive(smem_u32(&B.sched_full[s]));
+      if (stop) break;
+    }
+  } else if (warp == 9) {
+    // ---------------- TMA ----------------
+    if (lane == 0) {
+      tma_prefetch_desc(&tq);
+      tma_prefetch_desc(&tk);
+      tma_prefetch_desc(&tv);
+    }
+    const uint32_t q_bytes = (uint32_t)(p.group * p.tile_tokens) * 128u * C::PANELS;
+    int loads = 0, q_loads[2] = {0, 0};
+    uint32_t was_tail = 0, tail_phase = 0;      // per ring stage: last load, next phase's parity
+    Tile t;
+    bool ok = true;
+    for (int k = 0; ok && next_tile(k, t); ++k) {
+      if (lane == 0) {
+        const int blocks = max(t.blocks[0], t.blocks[1]);
+        for (int j = 0; ok && j < blocks; ++j) {
+          if (j == 0) {
+            for (int w = 0; ok && w < 2; ++w) {
+              if (!t.blocks[w]) continue;
+              if (q_loads[w] && !mbar_wait(smem_u32(&B.q_empty[w]), (q_loads[w] - 1) & 1, abort)) {
+                ok = false;
+                break;
+              }
+              const uint32_t bar = smem_u32(&B.q_full[w]);
+              mbar_arrive_expect_tx(bar, q_bytes);
 #pragma unroll
-    for (int i = 0; i < E; i += 2) {
-      const float2 vv = Elem<T>::to2(*reinterpret_cast<const uint32_t*>(vp + j * d.v_stride[0] + i));
-      o[i] = o[i] * f + e * vv.x;
-      o[i + 1] = o[i + 1] * f + e * vv.y;
+              for (int c = 0; c < C::PANELS; ++c)
+                tma_load_3d(sQ + w * C::TILE + c * C::PANEL, &tq, bar, 64 * c, t.head * p.q_head_step,
+                            t.token + w * p.tile_tokens);
+              ++q_loads[w];
+            }
+          }
+          for (int kv = 0; ok && kv < 2; ++kv, ++loads) {
+            const int s = loads % STAGES;
+            if (loads >= STAGES && !mbar_wait(smem_u32(&B.empty[s]), (loads / STAGES - 1) & 1, abort)) {
+              ok = false;
+              break;
+            }
+            // V rows past the last key: warp 10 passes the block on when it has cleared them
+            const bool tail = kv && (j + 1) * BK > t.keys;
+            const uint32_t bar = smem_u32(tail ? &B.tail[s] : &B.full[s]);
+            was_tail = (was_tail & ~(1u << s)) | (tail ? 1u << s : 0u);
+            if (tail) tail_phase ^= 1u << s;
+            mbar_arrive_expect_tx(bar, C::TILE);
+#pragma unroll
+            for (int c = 0; c < C::PANELS; ++c)
+              tma_load_3d(ring + s * C::TILE + c * C::PANEL, kv ? &tv : &tk, bar, 64 * c,
+                          t.head * (kv ? p.v_head_step : p.k_head_step), t.key0 + j * BK);
+          }
+        }
+      }
+      ok = __shfl_sync(0xffffffffu, ok ? 1 : 0, 0) != 0;
+    }
+    if (lane == 0 && *abort) {
+      // leave no copy in flight
+      int none = 0;
+      for (int s = 0; s < STAGES && s < loads; ++s) {
+        if ((was_tail >> s) & 1) mbar_wait(smem_u32(&B.tail[s]), ((tail_phase >> s) & 1) ^ 1, &none);
+        else mbar_wait(smem_u32(&B.full[s]), ((loads - 1 - s) / STAGES) & 1, &none);
+      }
+      for (int w = 0; w < 2; ++w)
+        if (q_loads[w]) mbar_wait(smem_u32(&B.q_full[w]), (q_loads[w] - 1) & 1, &none);
+    }
+  } else if (warp == 10) {
+    // ---------------- V rows past the last key ----------------
+    int loads = 0;
+    uint32_t phase = 0;                                 // per ring stage
+    Tile t;
+    for (int k = 0; next_tile(k, t); ++k) {
+      const int blocks = max(t.blocks[0], t.blocks[1]);
+      const int left = t.keys - (blocks - 1) * BK;      // keys of the last block that exist
+      if (blocks && left < BK) {
+        const int at = loads + 2 * blocks - 1, s = at % STAGES;
+        if (!__all_sync(0xffffffffu, mbar_wait(smem_u32(&B.tail[s]), (phase >> s) & 1, abort))) break;
+        phase ^= 1u << s;
+        uint8_t* v = smem_raw + (ring + s * C::TILE - smem_u32(smem_raw));
+        // whole 128-byte rows of each panel: the swizzle permutes within a row
+        for (int i = left * 8 + lane; i < BK * 8; i += 32)
+#pragma unroll
+          for (int c = 0; c < C::PANELS; ++c)
+            *reinterpret_cast<uint4*>(v + c * C::PANEL + i * 16) = make_uint4(0, 0, 0, 0);
+        fence_proxy_async();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(smem_u32(&B.full[s]));
+      }
+      loads += 2 * blocks;
+    }
+  } else if (warp == 8) {
+    // ---------------- MMA ----------------
+    constexpr uint32_t idesc_s = idesc_f16(BQ, BK, 0, 0) | TYPE;     // Q and K both K-major
+    constexpr uint32_t idesc_pv = idesc_f16(BQ, D, 0, 1) | TYPE;     // P K-major, V MN-major
+    int loads = 0;
+    int n_q[2] = {0, 0}, n_p[2] = {0, 0}, n_o[2] = {0, 0};   // Q tiles, P blocks and O tiles so far
+    Tile t;
+    bool ok = true;
+    for (int k = 0; ok && next_tile(k, t); ++k) {
+      if (lane == 0) {
+        const int blocks = max(t.blocks[0], t.blocks[1]);
+        int full_seen = loads - 1;        // ring loads known to have arrived
+        auto arrived = [&](int at) -> bool {
+          for (; full_seen < at; ++full_seen)
+            if (!mbar_wait(smem_u32(&B.full[(full_seen + 1) % STAGES]), ((full_seen + 1) / STAGES) & 1, abort))
+              return false;
+          return true;
+        };
+        auto issue_s = [&](int w, int j) -> bool {
+          const int at = loads + 2 * j;
+          if (!arrived(at)) return false;
+          tc_fence_after();
+          const uint32_t q = sQ + w * C::TILE, kb = ring + (at % STAGES) * C::TILE;
+#pragma unroll
+          for (int kk = 0; kk < D / 16; ++kk) {
+            const uint32_t off = (kk >> 2) * C::PANEL + (kk & 3) * 32;
+            mma_f16(tmem + w * BK, sdesc_sw128(q + off, 16, 1024), sdesc_sw128(kb + off, 16, 1024), idesc_s,
+                    kk != 0);
+          }
+          mma_commit(smem_u32(&B.s_full[w]));
+          if (j + 1 == t.blocks[w]) mma_commit(smem_u32(&B.q_empty[w]));
+          // the last row tile to use K_j: tile 1, unless only tile 0 goes this far
+          if (w == 1 || j >= t.blocks[1]) mma_commit(smem_u32(&B.empty[at % STAGES]));
+          return true;
+        };
+        for (int w = 0; ok && w < 2; ++w) {
+          if (!t.blocks[w]) continue;
+          ok = mbar_wait(smem_u32(&B.q_full[w]), n_q[w] & 1, abort);
+          ++n_q[w];
+          ok = ok && issue_s(w, 0);
+        }
+        for (int j = 0; ok && j < blocks; ++j) {
+          for (int w = 0; ok && w < 2; ++w) {
+            if (j >= t.blocks[w]) continue;
+            const int at = loads + 2 * j + 1;
+            ok = mbar_wait(smem_u32(&B.p_full[w]), n_p[w] & 1, abort);
+            ++n_p[w];
+            if (ok && j == 0) {
+              if (n_o[w]) ok = mbar_wait(smem_u32(&B.o_free[w]), (n_o[w] - 1) & 1, abort);
+              ++n_o[w];
+            }
+            ok = ok && arrived(at);
+            if (!ok) break;
+            tc_fence_after();
+            const uint32_t v = ring + (at % STAGES) * C::TILE;
+#pragma unroll
+            for (int kk = 0; kk < BK / 16; ++kk)
+              mma_f16_ts(tmem + O_COL + w * D, tmem + w * BK + kk * 8,
+                         sdesc_sw128(v + kk * 16 * 128, C::PANEL, 1024), idesc_pv, (j | kk) != 0);
+            mma_commit(smem_u32(&B.pv_done[w]));
+            if (w == 1 || j >= t.blocks[1]) mma_commit(smem_u32(&B.empty[at % STAGES]));
+            if (j + 1 < t.blocks[w]) ok = issue_s(w, j + 1);
+          }
+        }
+        loads += 2 * blocks;
+      }
+      ok = __shfl_sync(0xffffffffu, ok ? 1 : 0, 0) != 0;
+    }
+    if (lane == 0 && *abort) {
+      int none = 0;
+      mma_commit(smem_u32(&B.drain));
+      mbar_wait(smem_u32(&B.drain), 0, &none);
+    }
+  } else {
+    // ---------------- softmax, one row per thread ----------------
+    const int w = warp >> 2;
+    const int row = tid & 127;
+    const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
+    const uint32_t S = tmem + lanes + w * BK, O = tmem + lanes + O_COL + w * D;
+    const int token = row / p.group;                 // of the row tile
+    const int head_in = row - token * p.group;
+    const bool real = token < p.tile_tokens;
+    const float c = d.scale * LOG2E;
+    int n_s = 0;
+    Tile t;
+    for (int k = 0; next_tile(k, t); ++k) {
+      const int at = w * p.tile_tokens + token;       // of the tile's tokens
+      const bool store = real && at < t.tokens;
+      const int blocks = t.blocks[w];
+      const int limit = d.causal ? t.seen + at : t.keys;                           // keys this row sees
+      const int least = d.causal ? t.seen + w * p.tile_tokens : t.keys;            // and the tile's first row
+      float m = -INFINITY, l = 0.f;
+      bool ok = true;
+      for (int j = 0; j < blocks; ++j) {
+        ok = __all_sync(0xffffffffu, mbar_wait(smem_u32(&B.s_full[w]), n_s & 1, abort));
+        if (!ok) break;
+        ++n_s;
+        tc_fence_after();
+        float s[BK];
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          uint32_t r[64];
+          tmem_ld64_wait(S + 64 * h, r);
+#pragma unroll
+          for (int i = 0; i < 64; ++i) s[64 * h + i] = __uint_as_float(r[i]);
+        }
+        if ((j + 1) * BK > least) {
+          const int left = limit - j * BK;
+#pragma unroll
+          for (int i = 0; i < BK; ++i)
+            if (i >= left) s[i] = -INFINITY;
+        }
+        float m8[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) m8[i] = fmaxf(s[i], s[8 + i]);
+#pragma unroll
+        for (int i = 16; i < BK; i += 16)
+#pragma unroll
+          for (int x = 0; x < 8; ++x) m8[x] = max3(m8[x], s[i + x], s[i + 8 + x]);
+        const float top = fmaxf(max3(m8[0], m8[1], m8[2]), fmaxf(max3(m8[3], m8[4], m8[5]), fmaxf(m8[6], m8[7]))) * c;
+        const bool move = top > m + RESCALE_THRESHOLD;     // also from -inf
+        if (__any_sync(0xffffffffu, move)) {
+          const float f = move ? ex2(m - top) : 1.f;
+          if (move) m = top;
+          l *= f;
+          if (j) {
+#pragma unroll 1
+            for (int i = 0; i < D; i += 32) {
+              uint32_t r[32];
+              tmem_ld32_wait(O + i, r);
+#pragma unroll
+              for (int x = 0; x < 32; ++x) r[x] = __float_as_uint(__uint_as_float(r[x]) * f);
+              tmem_st32_wait(O + i, r);
+            }
+          }
+        }
+        const float sub = m == -INFINITY ? 0.f : -m;
+        const uint64_t c2 = pack2(c, c), sub2 = pack2(sub, sub);
+        uint64_t l4[4] = {0, 0, 0, 0};
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          uint32_t r[32];
+#pragma unroll
+          for (int i = 0; i < 32; ++i) {
+            const int e = 64 * h + 2 * i;
+            float a, b;
+            unpack2(fma2(pack2(s[e], s[e + 1]), c2, sub2), a, b);
+            a = ex2(a);
+            b = ex2(b);
+            l4[i & 3] = add2(l4[i & 3], pack2(a, b));
+            r[i] = Elem<T>::from2(a, b);
+          }
+          tmem_st32_wait(S + 32 * h, r);
+        }
+        float a, b;
+        unpack2(add2(add2(l4[0], l4[1]), add2(l4[2], l4[3])), a, b);
+        l += a + b;
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(smem_u32(&B.p_full[w]));
+      }
+      if (!ok) break;
+      const long long tok = (long long)t.token + at;
+      const int head = t.head * p.group + head_in;
+      T* out = static_cast<T*>(d.out) + tok * d.out_stride[0] + head * d.out_stride[1];
+      if (blocks) {
+        // every PV of this row tile is complete
+        if (!__all_sync(0xffffffffu, mbar_wait(smem_u32(&B.pv_done[w]), (n_s - 1) & 1, abort))) break;
+        tc_fence_after();
+        const float inv = l == 0.f ? 0.f : 1.f / l;
+#pragma unroll 1
+        for (int i = 0; i < D; i += 32) {
+          uint32_t r[32];
+          tmem_ld32_wait(O + i, r);
+          if (store) {
+#pragma unroll
+            for (int x = 0; x < 32; x += 8) {
+              uint32_t v[4];
+#pragma unroll
+              for (int y = 0; y < 4; ++y)
+                v[y] = l == 0.f ? 0u
+                                : Elem<T>::from2(__uint_as_float(r[x + 2 * y]) * inv,
+                                                 __uint_as_float(r[x + 2 * y + 1]) * inv);
+              *reinterpret_cast<uint4*>(out + i + x) = make_uint4(v[0], v[1], v[2], v[3]);
+            }
+          }
+        }
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(smem_u32(&B.o_free[w]));
+      } else if (store) {
+#pragma unroll
+        for (int i = 0; i < D; i += 8) *reinterpret_cast<uint4*>(out + i) = make_uint4(0, 0, 0, 0);
+      }
+      if (store && d.lse) d.lse[tok * d.heads + head] = l == 0.f ? -INFINITY : (m + log2f(l)) * LN2;
     }
   }
-  const float inv = l > 0.f ? 1.f / l : 0.f;
-  T* out = static_cast<T*>(d.out) + t * d.out_stride[0] + h * d.out_stride[1] + lane * E;
-#pragma unroll
-  for (int i = 0; i < E; i += 2)
-    *reinterpret_cast<uint32_t*>(out + i) = Elem<T>::from2(o[i] * inv, o[i + 1] * inv);
-  if (d.lse && lane == 0) d.lse[t * d.heads + h] = l > 0.f ? (m + log2f(l)) * LN2 : -INFINITY;
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 8) {
+    tc_fence_after();
+    tmem_dealloc(tmem, TMEM_COLS);
+  }
+  if (tid == 0 && B.abort_flag) atomicOr(d.status, KTIR_STATUS_TIMEOUT);
+}
+
+typedef CUresult (*EncodeTiledFn)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*,
+                                  const cuuint64_t*, const cuuint32_t*, const cuuint32_t*,
+                                  CUtensorMapInterleave, CUtensorMapSwizzle, CUtensorMapL2promotion,
+                                  CUtensorMapFloatOOBfill);
+
+EncodeTiledFn encode_fn() {
+  static EncodeTiledFn fn = nullptr;
+  if (!fn) {
+    void* ptr = nullptr;
+    cudaDriverEntryPointQueryResult q;
+    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &ptr, cudaEnableDefault, &q) == cudaSuccess &&
+        q == cudaDriverEntryPointSuccess)
+      fn = reinterpret_cast<EncodeTiledFn>(ptr);
+  }
+  return fn;
+}
+
+// [tokens][heads][dim] in boxes of 64 elements x box_heads x box_tokens; *head_step
+// is 0 where all heads are one vector (an expanded axis has stride 0)
+bool make_map(CUtensorMap* m, const void* base, bool bf16, int dim, int64_t heads, int64_t tokens,
+              const int64_t stride[2], int box_heads, int box_tokens, int* head_step) {
+  EncodeTiledFn enc = encode_fn();
+  if (!enc) return false;
+  *head_step = box_heads;
+  if (heads > 1 && stride[1] == 0) {
+    if (box_heads > 1) return false;
+    heads = 1;
+    *head_step = 0;
+  }
+  cuuint64_t dims[3] = {(cuuint64_t)dim, (cuuint64_t)heads, (cuuint64_t)tokens};
+  // an axis with one entry has no stride of its own
+  cuuint64_t strides[2] = {(cuuint64_t)(heads > 1 ? stride[1] : dim) * 2, (cuuint64_t)(tokens > 1 ? stride[0] : heads * dim) * 2};
+  cuuint32_t box[3] = {64, (cuuint32_t)box_heads, (cuuint32_t)box_tokens};
+  cuuint32_t estr[3] = {1, 1, 1};
+  return enc(m, bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 3,
+             const_cast<void*>(base), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+             CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+             CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+template <typename T, int D>
+int launch(const CUtensorMap& tq, const CUtensorMap& tk, const CUtensorMap& tv, const PromptParams& p,
+           unsigned grid, cudaStream_t stream) {
+  constexpr int BYTES = Cfg<D>::BYTES + 1024;
+  static bool ready[MAX_DEVICES] = {};
+  const int dev = current_device();
+  if (dev < 0) return ktir_set_error(KTIR_ERR_CUDA, "ktir_prompt_attention: no usable current device");
+  if (!ready[dev]) {
+    if (cudaFuncSetAttribute(k_prompt_attention<T, D>, cudaFuncAttributeMaxDynamicSharedMemorySize, BYTES) !=
+        cudaSuccess)
+      return ktir_set_error(KTIR_ERR_CUDA, "ktir_prompt_attention: shared-memory attribute refused");
+    ready[dev] = true;
+  }
+  k_prompt_attention<T, D><<<grid, THREADS, BYTES, stream>>>(tq, tk, tv, p);
+  return launched("ktir_prompt_attention: launch failed");
 }
 
 }  // namespace
@@ -108,18 +709,30 @@ extern "C" int ktir_prompt_attention(const KtirPromptDesc* d, void* stream) {
       !aligned16(d->k) || !aligned16(d->v) || !aligned16(d->out))
     return ktir_set_error(KTIR_ERR_UNSUPPORTED,
                           "ktir_prompt_attention: head vectors must start on 16-byte boundaries");
-  const long long blocks = (d->tokens * d->heads + WARPS - 1) / WARPS;
-  if (blocks > 0x7fffffffLL)
-    return ktir_set_error(KTIR_ERR_UNSUPPORTED, "ktir_prompt_attention: too many rows");
-  const unsigned grid = (unsigned)blocks;
+  const bool bf16 = d->dtype == KTIR_BF16;
+  PromptParams p;
+  p.d = *d;
+  p.group = d->heads / d->kv_heads;
+  p.tile_tokens = BQ / p.group;
+  // without keys nothing is loaded, but the maps must be valid
+  const int64_t none[2] = {d->dim, d->dim};
+  const int64_t keys = d->kv_tokens > 0 ? d->kv_tokens : 1;
+  CUtensorMap tq, tk, tv;
+  if (!make_map(&tq, d->q, bf16, d->dim, d->heads, d->tokens, d->q_stride, p.group, p.tile_tokens,
+                &p.q_head_step) ||
+      !make_map(&tk, d->kv_tokens > 0 ? d->k : d->q, bf16, d->dim, d->kv_tokens > 0 ? d->kv_heads : 1, keys,
+                d->kv_tokens > 0 ? d->k_stride : none, 1, BK, &p.k_head_step) ||
+      !make_map(&tv, d->kv_tokens > 0 ? d->v : d->q, bf16, d->dim, d->kv_tokens > 0 ? d->kv_heads : 1, keys,
+                d->kv_tokens > 0 ? d->v_stride : none, 1, BK, &p.v_head_step))
+    return ktir_set_error(KTIR_ERR_UNSUPPORTED, "ktir_prompt_attention: strides that a tensor map does not take");
+  const int sms = sm_count();
+  if (sms < 1) return ktir_set_error(KTIR_ERR_CUDA, "ktir_prompt_attention: no usable current device");
+  // at most this many tiles: every sequence may end in a part of one
+  const long long tiles = (d->tokens / (2 * p.tile_tokens) + d->batch) * d->kv_heads;
+  if (tiles > 0x7fffffffLL) return ktir_set_error(KTIR_ERR_UNSUPPORTED, "ktir_prompt_attention: too many tiles");
+  const unsigned grid = (unsigned)(tiles < sms ? tiles : sms);
   cudaStream_t s = static_cast<cudaStream_t>(stream);
-  const bool f16 = d->dtype == KTIR_F16;
-  if (d->dim == 64) {
-    if (f16) k_prompt_attention<__half, 64><<<grid, WARPS * 32, 0, s>>>(*d);
-    else k_prompt_attention<__nv_bfloat16, 64><<<grid, WARPS * 32, 0, s>>>(*d);
-  } else {
-    if (f16) k_prompt_attention<__half, 128><<<grid, WARPS * 32, 0, s>>>(*d);
-    else k_prompt_attention<__nv_bfloat16, 128><<<grid, WARPS * 32, 0, s>>>(*d);
-  }
-  return launched("ktir_prompt_attention: launch failed");
+  if (d->dim == 64)
+    return bf16 ? launch<__nv_bfloat16, 64>(tq, tk, tv, p, grid, s) : launch<__half, 64>(tq, tk, tv, p, grid, s);
+  return bf16 ? launch<__nv_bfloat16, 128>(tq, tk, tv, p, grid, s) : launch<__half, 128>(tq, tk, tv, p, grid, s);
 }

@@ -20,6 +20,7 @@ constexpr float LN2 = 0.6931471805599453f;
 
 template <typename T> struct Elem;
 template <> struct Elem<__half> {
+  static constexpr bool BF16 = false;
   static __device__ __forceinline__ float2 to2(uint32_t v) {
     return __half22float2(*reinterpret_cast<const __half2*>(&v));
   }
@@ -29,6 +30,7 @@ template <> struct Elem<__half> {
   }
 };
 template <> struct Elem<__nv_bfloat16> {
+  static constexpr bool BF16 = true;
   static __device__ __forceinline__ float2 to2(uint32_t v) {
     return make_float2(__uint_as_float(v << 16), __uint_as_float(v & 0xffff0000u));
   }
@@ -53,6 +55,23 @@ inline bool vector_strides(const int64_t* stride, const int64_t* extent, int n) 
   for (int i = 0; i < n; ++i)
     if (extent[i] > 1 && ((stride[i] & 7) || stride[i] < 0)) return false;
   return true;
+}
+
+constexpr int MAX_DEVICES = 64;
+
+// the current device, or -1
+inline int current_device() {
+  int dev = 0;
+  return cudaGetDevice(&dev) == cudaSuccess && dev >= 0 && dev < MAX_DEVICES ? dev : -1;
+}
+
+inline int sm_count() {   // of the current device, 0 if there is none
+  static int count[MAX_DEVICES] = {};
+  const int dev = current_device();
+  if (dev < 0) return 0;
+  if (!count[dev] && cudaDeviceGetAttribute(&count[dev], cudaDevAttrMultiProcessorCount, dev) != cudaSuccess)
+    return 0;
+  return count[dev];
 }
 
 inline int launched(const char* what) {
