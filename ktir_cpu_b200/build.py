@@ -1,4 +1,5 @@
-"""Compile the CUDA library (libktir_b200.so) in-tree for sm_100a.
+"""Compile the CUDA library (libktir_b200.so) in-tree for sm_100a, and the
+serving operators' Python binding (_serving.so), which calls it.
 
     python -m ktir_cpu_b200.build          # or build() from Python
 
@@ -16,6 +17,8 @@ import sys
 HERE = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(HERE, "csrc")
 LIB = os.path.join(HERE, "libktir_b200.so")
+BINDING_SRC = os.path.join(CSRC, "serving_binding.cpp")
+BINDING = os.path.join(HERE, "_serving.so")
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
 
 
@@ -30,13 +33,42 @@ def sources():
     return sorted(glob.glob(os.path.join(CSRC, "*.cu")))
 
 
-def up_to_date() -> bool:
-    if not os.path.exists(LIB):
+def _newer(target, deps) -> bool:
+    if not os.path.exists(target):
         return False
-    t = os.path.getmtime(LIB)
-    deps = sources() + glob.glob(os.path.join(CSRC, "*.cuh")) + \
-        glob.glob(os.path.join(HERE, "..", "include", "*.h"))
+    t = os.path.getmtime(target)
     return all(os.path.getmtime(p) <= t for p in deps)
+
+
+def up_to_date() -> bool:
+    headers = glob.glob(os.path.join(HERE, "..", "include", "*.h"))
+    return _newer(LIB, sources() + glob.glob(os.path.join(CSRC, "*.cuh")) + headers) and \
+        _newer(BINDING, [BINDING_SRC] + headers)
+
+
+def _compile_binding():
+    """The binding's object file and the process that compiles it."""
+    import sysconfig
+    import torch
+    inc = os.path.join(os.path.dirname(torch.__file__), "include")
+    obj = os.path.join(HERE, "_build", "serving_binding.o")
+    includes = [inc, os.path.join(inc, "torch", "csrc", "api", "include"), sysconfig.get_paths()["include"],
+                os.path.join(os.path.dirname(os.path.dirname(os.path.realpath(_nvcc()))), "include")]
+    cmd = ["g++", "-O2", "-std=c++17", "-fPIC", "-Wall", "-c", BINDING_SRC, "-o", obj]
+    for p in includes:
+        cmd += ["-isystem", p]
+    return obj, subprocess.Popen(cmd, stdout=subprocess.PIPE, stderr=subprocess.STDOUT)
+
+
+def _link_binding(obj):
+    import torch
+    cmd = ["g++", "-shared", "-o", BINDING + ".tmp", obj, "-L", HERE, "-l:" + os.path.basename(LIB),
+           "-Wl,-rpath,$ORIGIN"]
+    cmd += ["-L", os.path.join(os.path.dirname(torch.__file__), "lib")]
+    # torch's libraries are in the process by the time the binding is imported
+    cmd += ["-ltorch_python", "-ltorch_cpu", "-ltorch", "-lc10", "-lc10_cuda"]
+    subprocess.check_call(cmd)
+    os.replace(BINDING + ".tmp", BINDING)
 
 
 def build(force: bool = False, verbose: bool = False) -> str:
@@ -55,6 +87,8 @@ def build(force: bool = False, verbose: bool = False) -> str:
             cmd.insert(1, "-Xptxas=-v")
         procs.append((src, subprocess.Popen(cmd, stdout=subprocess.PIPE, stderr=subprocess.STDOUT)))
         objs.append(obj)
+    binding_obj, binding = _compile_binding()
+    procs.append((BINDING_SRC, binding))
     failed = []
     for src, p in procs:
         out, _ = p.communicate()
@@ -67,6 +101,7 @@ def build(force: bool = False, verbose: bool = False) -> str:
     tmp_lib = LIB + ".tmp"
     subprocess.check_call([nvcc, *ARCH, "-shared", "-o", tmp_lib, *objs, "-lcudart"])
     os.replace(tmp_lib, LIB)
+    _link_binding(binding_obj)
     return LIB
 
 

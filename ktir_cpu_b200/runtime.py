@@ -192,6 +192,10 @@ def lib_path() -> str:
     return _build.LIB
 
 
+def binding_path() -> str:
+    return _build.BINDING
+
+
 def load_library(build_if_missing: bool = False) -> C.CDLL:
     """Load libktir_b200.so (never falls back to anything else)."""
     global _LIB
@@ -237,11 +241,11 @@ def load_library(build_if_missing: bool = False) -> C.CDLL:
     lib.ktir_host_upload.argtypes = [C.POINTER(KtirHostXfer), C.c_int, C.c_int, vp]
     lib.ktir_host_download.argtypes = [C.POINTER(KtirHostXfer), C.c_int, C.POINTER(KtirHostCopy),
                                        C.c_int, C.c_int, vp]
-    lib.ktir_kv_append.argtypes = [vp, vp]      # KtirKvAppendDesc, or its bytes
-    lib.ktir_paged_decode.argtypes = [vp, vp]      # KtirPagedDecodeDesc, or its bytes
+    lib.ktir_kv_append.argtypes = [C.POINTER(KtirKvAppendDesc), vp]
+    lib.ktir_paged_decode.argtypes = [C.POINTER(KtirPagedDecodeDesc), vp]
     lib.ktir_paged_decode_workspace.argtypes = [C.c_int64, C.c_int32, C.c_int32, C.c_int32]
     lib.ktir_paged_decode_workspace.restype = C.c_int64
-    lib.ktir_prompt_attention.argtypes = [vp, vp]      # KtirPromptDesc, or its bytes
+    lib.ktir_prompt_attention.argtypes = [C.POINTER(KtirPromptDesc), vp]
     for name in EXPORTS:
         getattr(lib, name).restype = C.c_int if name != "ktir_last_error" else C.c_char_p
     _LIB = lib
