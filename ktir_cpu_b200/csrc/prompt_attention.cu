@@ -42,6 +42,8 @@
 // CTA still frees its TMEM.
 #include <cuda.h>
 
+#include <type_traits>
+
 #include "serve_common.cuh"
 #include "tc_common.cuh"
 
@@ -106,6 +108,30 @@ __device__ __forceinline__ void tma_load_3d(uint32_t dst, const CUtensorMap* map
       " [%0], [%1, {%2, %3, %4}], [%5];" ::"r"(dst),
       "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(z), "r"(bar)
       : "memory");
+}
+
+// Bounded wait for a barrier's phase: false (and the abort flag raised) when the
+// limit runs out or another role has given up.  Kept from being unrolled: four
+// tests in a row before the first branch cost a wait that is over 120 cycles
+// (8192 tokens, 32 heads over 8: 611 -> 543 us).
+__device__ __forceinline__ bool wait(uint32_t bar, uint32_t parity, volatile int* abort) {
+  if (mbar_try_wait(bar, parity)) return true;
+#pragma unroll 1
+  for (uint32_t i = 0; i < kSpinLimit; ++i) {
+    if (mbar_try_wait(bar, parity)) return true;
+    if (*abort) return false;
+  }
+  *abort = 1;
+  return false;
+}
+
+// One lane of the (converged) warp.  Code under this predicate may use uniform
+// registers, under `lane == 0` it may not: eight tcgen05.mma then take 413
+// cycles to issue instead of 129 (512 to run).
+__device__ __forceinline__ bool elect() {
+  uint32_t one;
+  asm volatile("{\n .reg .pred p;\n elect.sync _|p, 0xffffffff;\n selp.u32 %0, 1, 0, p;\n}\n" : "=r"(one));
+  return one != 0;
 }
 
 __device__ __forceinline__ float max3(float a, float b, float c) {
@@ -283,7 +309,7 @@ __global__ void __launch_bounds__(THREADS, 1)
   // announced tiles, read by whole warps: false at the end (or on an abort)
   auto next_tile = [&](int k, Tile& t) -> bool {
     const int s = k % SCHED;
-    if (!__all_sync(0xffffffffu, mbar_wait(smem_u32(&B.sched_full[s]), (k / SCHED) & 1, abort))) return false;
+    if (!__all_sync(0xffffffffu, wait(smem_u32(&B.sched_full[s]), (k / SCHED) & 1, abort))) return false;
     t = B.tile[s];
     __syncwarp();
     if (lane == 0) mbar_arrive(smem_u32(&B.sched_empty[s]));
@@ -314,7 +340,7 @@ __global__ void __launch_bounds__(THREADS, 1)
       const long long x = (long long)k * gridDim.x + ((k & 1) ? gridDim.x - 1 - blockIdx.x : blockIdx.x);
       const int s = k % SCHED;
       if (k >= SCHED &&
-          !__all_sync(0xffffffffu, mbar_wait(smem_u32(&B.sched_empty[s]), (k / SCHED - 1) & 1, abort)))
+          !__all_sync(0xffffffffu, wait(smem_u32(&B.sched_empty[s]), (k / SCHED - 1) & 1, abort)))
         break;
       // back and forth, a CTA may have a tile in the last round after having none before it
       const bool stop = (long long)k * gridDim.x >= all;
@@ -335,7 +361,8 @@ __global__ void __launch_bounds__(THREADS, 1)
     }
   } else if (warp == 9) {
     // ---------------- TMA ----------------
-    if (lane == 0) {
+    const bool leader = elect();
+    if (leader) {
       tma_prefetch_desc(&tq);
       tma_prefetch_desc(&tk);
       tma_prefetch_desc(&tv);
@@ -346,13 +373,13 @@ __global__ void __launch_bounds__(THREADS, 1)
     Tile t;
     bool ok = true;
     for (int k = 0; ok && next_tile(k, t); ++k) {
-      if (lane == 0) {
+      if (leader) {
         const int blocks = max(t.blocks[0], t.blocks[1]);
         for (int j = 0; ok && j < blocks; ++j) {
           if (j == 0) {
             for (int w = 0; ok && w < 2; ++w) {
               if (!t.blocks[w]) continue;
-              if (q_loads[w] && !mbar_wait(smem_u32(&B.q_empty[w]), (q_loads[w] - 1) & 1, abort)) {
+              if (q_loads[w] && !wait(smem_u32(&B.q_empty[w]), (q_loads[w] - 1) & 1, abort)) {
                 ok = false;
                 break;
               }
@@ -367,7 +394,7 @@ __global__ void __launch_bounds__(THREADS, 1)
           }
           for (int kv = 0; ok && kv < 2; ++kv, ++loads) {
             const int s = loads % STAGES;
-            if (loads >= STAGES && !mbar_wait(smem_u32(&B.empty[s]), (loads / STAGES - 1) & 1, abort)) {
+            if (loads >= STAGES && !wait(smem_u32(&B.empty[s]), (loads / STAGES - 1) & 1, abort)) {
               ok = false;
               break;
             }
@@ -384,17 +411,17 @@ __global__ void __launch_bounds__(THREADS, 1)
           }
         }
       }
-      ok = __shfl_sync(0xffffffffu, ok ? 1 : 0, 0) != 0;
+      ok = __all_sync(0xffffffffu, ok);
     }
-    if (lane == 0 && *abort) {
+    if (leader && *abort) {
       // leave no copy in flight
       int none = 0;
       for (int s = 0; s < STAGES && s < loads; ++s) {
-        if ((was_tail >> s) & 1) mbar_wait(smem_u32(&B.tail[s]), ((tail_phase >> s) & 1) ^ 1, &none);
-        else mbar_wait(smem_u32(&B.full[s]), ((loads - 1 - s) / STAGES) & 1, &none);
+        if ((was_tail >> s) & 1) wait(smem_u32(&B.tail[s]), ((tail_phase >> s) & 1) ^ 1, &none);
+        else wait(smem_u32(&B.full[s]), ((loads - 1 - s) / STAGES) & 1, &none);
       }
       for (int w = 0; w < 2; ++w)
-        if (q_loads[w]) mbar_wait(smem_u32(&B.q_full[w]), (q_loads[w] - 1) & 1, &none);
+        if (q_loads[w]) wait(smem_u32(&B.q_full[w]), (q_loads[w] - 1) & 1, &none);
     }
   } else if (warp == 10) {
     // ---------------- V rows past the last key ----------------
@@ -406,7 +433,7 @@ __global__ void __launch_bounds__(THREADS, 1)
       const int left = t.keys - (blocks - 1) * BK;      // keys of the last block that exist
       if (blocks && left < BK) {
         const int at = loads + 2 * blocks - 1, s = at % STAGES;
-        if (!__all_sync(0xffffffffu, mbar_wait(smem_u32(&B.tail[s]), (phase >> s) & 1, abort))) break;
+        if (!__all_sync(0xffffffffu, wait(smem_u32(&B.tail[s]), (phase >> s) & 1, abort))) break;
         phase ^= 1u << s;
         uint8_t* v = smem_raw + (ring + s * C::TILE - smem_u32(smem_raw));
         // whole 128-byte rows of each panel: the swizzle permutes within a row
@@ -422,76 +449,111 @@ __global__ void __launch_bounds__(THREADS, 1)
     }
   } else if (warp == 8) {
     // ---------------- MMA ----------------
+    // One thread issues every product, so what it does between two of them is
+    // kept short: no indexing of local arrays, no division, descriptors by
+    // adding to constants.
     constexpr uint32_t idesc_s = idesc_f16(BQ, BK, 0, 0) | TYPE;     // Q and K both K-major
     constexpr uint32_t idesc_pv = idesc_f16(BQ, D, 0, 1) | TYPE;     // P K-major, V MN-major
-    int loads = 0;
-    int n_q[2] = {0, 0}, n_p[2] = {0, 0}, n_o[2] = {0, 0};   // Q tiles, P blocks and O tiles so far
+    const uint64_t q_desc = sdesc_sw128(sQ, 16, 1024), k_desc = sdesc_sw128(ring, 16, 1024),
+                   v_desc = sdesc_sw128(ring, C::PANEL, 1024);
+    uint32_t stage = 0, ring_phase = 0;         // next ring load to wait for
+    uint32_t p_phase = 0, q_phase = 0, o_phase = 0, o_used = 0;      // bit w: row tile w
+    auto next_load = [&]() -> bool {            // the next load has arrived
+      const bool ok = wait(smem_u32(&B.full[stage]), ring_phase, abort);
+      if (++stage == STAGES) {
+        stage = 0;
+        ring_phase ^= 1;
+      }
+      return ok;
+    };
+    const bool leader = elect();
     Tile t;
     bool ok = true;
     for (int k = 0; ok && next_tile(k, t); ++k) {
-      if (lane == 0) {
-        const int blocks = max(t.blocks[0], t.blocks[1]);
-        int full_seen = loads - 1;        // ring loads known to have arrived
-        auto arrived = [&](int at) -> bool {
-          for (; full_seen < at; ++full_seen)
-            if (!mbar_wait(smem_u32(&B.full[(full_seen + 1) % STAGES]), ((full_seen + 1) / STAGES) & 1, abort))
-              return false;
-          return true;
-        };
-        auto issue_s = [&](int w, int j) -> bool {
-          const int at = loads + 2 * j;
-          if (!arrived(at)) return false;
-          tc_fence_after();
-          const uint32_t q = sQ + w * C::TILE, kb = ring + (at % STAGES) * C::TILE;
+      if (leader) {
+        const int blocks0 = t.blocks[0], blocks1 = t.blocks[1], blocks = max(blocks0, blocks1);
+        uint32_t k_stage = stage, v_stage = 0;
+        auto issue_s = [&](auto W, int j) {
+          constexpr int w = decltype(W)::value;
+          const uint64_t q = q_desc + (uint64_t)(w * (C::TILE >> 4));
+          const uint64_t kb = k_desc + (uint64_t)(k_stage * (C::TILE >> 4));
 #pragma unroll
           for (int kk = 0; kk < D / 16; ++kk) {
-            const uint32_t off = (kk >> 2) * C::PANEL + (kk & 3) * 32;
-            mma_f16(tmem + w * BK, sdesc_sw128(q + off, 16, 1024), sdesc_sw128(kb + off, 16, 1024), idesc_s,
-                    kk != 0);
+            const uint64_t off = ((kk >> 2) * C::PANEL + (kk & 3) * 32) >> 4;
+            mma_f16(tmem + w * BK, q + off, kb + off, idesc_s, kk != 0);
           }
           mma_commit(smem_u32(&B.s_full[w]));
-          if (j + 1 == t.blocks[w]) mma_commit(smem_u32(&B.q_empty[w]));
-          // the last row tile to use K_j: tile 1, unless only tile 0 goes this far
-          if (w == 1 || j >= t.blocks[1]) mma_commit(smem_u32(&B.empty[at % STAGES]));
+          if (j + 1 == (w ? blocks1 : blocks0)) mma_commit(smem_u32(&B.q_empty[w]));
+        };
+        auto issue_pv = [&](auto W, int j) -> bool {
+          constexpr int w = decltype(W)::value;
+          if (!wait(smem_u32(&B.p_full[w]), (p_phase >> w) & 1, abort)) return false;
+          p_phase ^= 1u << w;
+          if (j == 0) {
+            if ((o_used >> w) & 1) {            // O of the tile before has been read
+              if (!wait(smem_u32(&B.o_free[w]), (o_phase >> w) & 1, abort)) return false;
+              o_phase ^= 1u << w;
+            }
+            o_used |= 1u << w;
+          }
+          tc_fence_after();
+          const uint64_t v = v_desc + (uint64_t)(v_stage * (C::TILE >> 4));
+#pragma unroll
+          for (int kk = 0; kk < BK / 16; ++kk)
+            mma_f16_ts(tmem + O_COL + w * D, tmem + w * BK + kk * 8, v + (uint64_t)((kk * 16 * 128) >> 4), idesc_pv,
+                       kk == 0 ? (uint32_t)(j != 0) : 1u);
+          mma_commit(smem_u32(&B.pv_done[w]));
           return true;
         };
-        for (int w = 0; ok && w < 2; ++w) {
-          if (!t.blocks[w]) continue;
-          ok = mbar_wait(smem_u32(&B.q_full[w]), n_q[w] & 1, abort);
-          ++n_q[w];
-          ok = ok && issue_s(w, 0);
+        using W0 = std::integral_constant<int, 0>;
+        using W1 = std::integral_constant<int, 1>;
+        if (blocks) {
+          ok = next_load();                     // K_0
+          if (ok && blocks0) {
+            ok = wait(smem_u32(&B.q_full[0]), q_phase & 1, abort);
+            q_phase ^= 1;
+            tc_fence_after();
+            if (ok) issue_s(W0(), 0);
+          }
+          if (ok && blocks1) {
+            ok = wait(smem_u32(&B.q_full[1]), q_phase >> 1, abort);
+            q_phase ^= 2;
+            tc_fence_after();
+            if (ok) issue_s(W1(), 0);
+          }
+          if (ok) mma_commit(smem_u32(&B.empty[k_stage]));
         }
         for (int j = 0; ok && j < blocks; ++j) {
-          for (int w = 0; ok && w < 2; ++w) {
-            if (j >= t.blocks[w]) continue;
-            const int at = loads + 2 * j + 1;
-            ok = mbar_wait(smem_u32(&B.p_full[w]), n_p[w] & 1, abort);
-            ++n_p[w];
-            if (ok && j == 0) {
-              if (n_o[w]) ok = mbar_wait(smem_u32(&B.o_free[w]), (n_o[w] - 1) & 1, abort);
-              ++n_o[w];
-            }
-            ok = ok && arrived(at);
+          v_stage = stage;
+          ok = next_load();                     // V_j
+          if (!ok) break;
+          const bool more = j + 1 < blocks;
+          if (j < blocks0) {
+            ok = issue_pv(W0(), j);
+            if (!ok) break;
+          }
+          if (more) {
+            k_stage = stage;
+            ok = next_load();                   // K_{j+1}
             if (!ok) break;
             tc_fence_after();
-            const uint32_t v = ring + (at % STAGES) * C::TILE;
-#pragma unroll
-            for (int kk = 0; kk < BK / 16; ++kk)
-              mma_f16_ts(tmem + O_COL + w * D, tmem + w * BK + kk * 8,
-                         sdesc_sw128(v + kk * 16 * 128, C::PANEL, 1024), idesc_pv, (j | kk) != 0);
-            mma_commit(smem_u32(&B.pv_done[w]));
-            if (w == 1 || j >= t.blocks[1]) mma_commit(smem_u32(&B.empty[at % STAGES]));
-            if (j + 1 < t.blocks[w]) ok = issue_s(w, j + 1);
           }
+          if (j + 1 < blocks0) issue_s(W0(), j + 1);
+          if (j < blocks1) {
+            ok = issue_pv(W1(), j);
+            if (!ok) break;
+          }
+          mma_commit(smem_u32(&B.empty[v_stage]));
+          if (j + 1 < blocks1) issue_s(W1(), j + 1);
+          if (more) mma_commit(smem_u32(&B.empty[k_stage]));
         }
-        loads += 2 * blocks;
       }
-      ok = __shfl_sync(0xffffffffu, ok ? 1 : 0, 0) != 0;
+      ok = __all_sync(0xffffffffu, ok);
     }
-    if (lane == 0 && *abort) {
+    if (leader && *abort) {
       int none = 0;
       mma_commit(smem_u32(&B.drain));
-      mbar_wait(smem_u32(&B.drain), 0, &none);
+      wait(smem_u32(&B.drain), 0, &none);
     }
   } else {
     // ---------------- softmax, one row per thread ----------------
@@ -514,7 +576,7 @@ __global__ void __launch_bounds__(THREADS, 1)
       float m = -INFINITY, l = 0.f;
       bool ok = true;
       for (int j = 0; j < blocks; ++j) {
-        ok = __all_sync(0xffffffffu, mbar_wait(smem_u32(&B.s_full[w]), n_s & 1, abort));
+        ok = __all_sync(0xffffffffu, wait(smem_u32(&B.s_full[w]), n_s & 1, abort));
         if (!ok) break;
         ++n_s;
         tc_fence_after();
@@ -587,7 +649,7 @@ __global__ void __launch_bounds__(THREADS, 1)
       T* out = static_cast<T*>(d.out) + tok * d.out_stride[0] + head * d.out_stride[1];
       if (blocks) {
         // every PV of this row tile is complete
-        if (!__all_sync(0xffffffffu, mbar_wait(smem_u32(&B.pv_done[w]), (n_s - 1) & 1, abort))) break;
+        if (!__all_sync(0xffffffffu, wait(smem_u32(&B.pv_done[w]), (n_s - 1) & 1, abort))) break;
         tc_fence_after();
         const float inv = l == 0.f ? 0.f : 1.f / l;
 #pragma unroll 1
