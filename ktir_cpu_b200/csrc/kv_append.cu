@@ -80,6 +80,8 @@ __global__ void __launch_bounds__(THREADS) k_kv_append(const __grid_constant__ A
   const int rparts = d.rot >> 4;
   const bool turn = j < rparts;
 
+  pdl_launch();
+  pdl_wait();
   const int slot = d.slots[t];
   bool bad = slot >= p.slots_total;
   float c[8], s[8];
@@ -174,11 +176,10 @@ extern "C" int ktir_kv_append(const KtirKvAppendDesc* d, void* stream) {
   p.d = *d;
   const __int128 total = (__int128)d->num_pages * d->page_size;
   p.slots_total = total > 0x7fffffffLL ? 0x80000000LL : (long long)total;
-  const dim3 grid((unsigned)d->tokens);
+  const unsigned grid = (unsigned)d->tokens;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
-  if (d->dtype == KTIR_F16)
-    k_kv_append<__half><<<grid, THREADS, 0, s>>>(p);
-  else
-    k_kv_append<__nv_bfloat16><<<grid, THREADS, 0, s>>>(p);
-  return launched("ktir_kv_append: launch failed");
+  const cudaError_t e = d->dtype == KTIR_F16
+                            ? launch_pdl(k_kv_append<__half>, grid, THREADS, 0, s, p)
+                            : launch_pdl(k_kv_append<__nv_bfloat16>, grid, THREADS, 0, s, p);
+  return launched(e, "ktir_kv_append: launch failed");
 }

@@ -138,6 +138,9 @@ __global__ void __launch_bounds__(THREADS, CTAS_PER_SM)
     return len < 0 || len > most ? 0 : len;
   };
 
+  pdl_launch();
+  pdl_wait();
+
   // this stretch of the list: an exclusive scan over runs of sequences
   const long long per = (d.batch + THREADS - 1) / THREADS;
   const long long r0 = min((long long)d.batch, tid * per), r1 = min((long long)d.batch, r0 + per);
@@ -486,8 +489,8 @@ int launch(const DecodeParams& p, unsigned grid, cudaStream_t stream) {
       return ktir_set_error(KTIR_ERR_CUDA, "ktir_paged_decode: shared-memory attribute refused");
     ready[dev] = true;
   }
-  k_paged_decode<T, D><<<grid, THREADS, Cfg<T, D>::SMEM, stream>>>(p);
-  return launched("ktir_paged_decode: launch failed");
+  return launched(launch_pdl(k_paged_decode<T, D>, grid, THREADS, Cfg<T, D>::SMEM, stream, p),
+                  "ktir_paged_decode: launch failed");
 }
 
 }  // namespace

@@ -17,23 +17,22 @@
 // Roles, meeting only at mbarriers:
 //   warps 0-3, 4-7  the softmax of row tile 0 and 1, one row per thread:
 //                   S from TMEM, mask, running maximum and sum, P = 2^(x - m)
-//                   rounded to the element type back over S's columns, and at
-//                   a tile's end O / l to memory
-//   warp 8 (MMA)    S_w(j) = Q_w K_j^T (128 x 128 x dim) and O_w += P_w(j) V_j,
-//                   P read from TMEM; per row tile and block: PV_w(j), then
-//                   S_w(j+1) over the columns that held P_w(j) (the tensor pipe
-//                   runs one thread's products in order)
+//                   rounded to the element type into TMEM, and at a tile's end
+//                   O / l to memory
+//   warps 8, 10     (MMA) S_w(j) = Q_w K_j^T and O_w += P_w(j) V_j, P read from
+//                   TMEM; S_w(j+1) runs as soon as S_w(j) is in registers, so the
+//                   softmax goes from block to block without waiting for it
 //   warp 9 (TMA)    Q tiles, and K_j, V_j through one ring
-//   warp 10         sets V's rows past the sequence's last key to zero (they
-//                   belong to another sequence; a weight of 0 does not cancel
-//                   an infinity there)
 //   warp 11         finds the next tile: tiles are taken in order of falling
 //                   key counts over all sequences, back and forth over the
-//                   CTAs, so that the last ones to finish are the shortest
-// TMEM: S_0 0..127, S_1 128..255, O_0 and O_1 from 256 on, dim columns each.
+//                   CTAs, so that the last ones to finish are the shortest; and
+//                   sets V's rows past the sequence's last key to zero (they
+//                   belong to another sequence; a weight of 0 does not cancel
+//                   an infinity there)
+// TMEM holds S, P and O of both row tiles apart, which at dim 128 leaves room for
+// blocks of 80 keys (128 at dim 64).
 // The running maximum moves only when a row's maximum exceeds it by more than
-// 2^8; O's rows are then rescaled in TMEM, which S_w(j)'s completion allows:
-// PV_w(j-1) was issued before it.
+// 2^8; O's rows are then rescaled in TMEM, after the product before.
 // Precision: S, O, m and l in f32; P is rounded to the element type for the
 // second product (tcgen05 wants one type for both operands), half an ulp per
 // weight; l adds the unrounded weights.
@@ -53,21 +52,25 @@ using namespace ktir::tc;
 namespace {
 
 constexpr int BQ = 128;              // rows of a row tile
-constexpr int BK = 128;              // keys of a block
 constexpr int THREADS = 384;
 constexpr int SCHED = 4;             // tiles announced ahead
-constexpr int SCHED_READERS = 11;    // 8 softmax warps, MMA, TMA, V's tail
+constexpr int SCHED_READERS = 11;    // 8 softmax warps, two MMA, TMA
 constexpr float RESCALE_THRESHOLD = 8.0f;   // log2 units
+constexpr int SOFTMAX_REGS = 208, OTHER_REGS = 80;
 constexpr uint32_t TMEM_COLS = 512;
-constexpr uint32_t O_COL = 256;
 
+// TMEM has 512 columns for S (BK), P (BK / 2) and O (D) of two row tiles.
 template <int D>
 struct Cfg {
-  static constexpr int PANEL = BK * 128;            // 128 rows of 64 elements, 128-byte swizzle
-  static constexpr int PANELS = D / 64;
-  static constexpr int TILE = PANELS * PANEL;       // a Q tile, a K block or a V block
-  static constexpr int STAGES = D == 128 ? 5 : 10;
-  static constexpr int BYTES = (2 + STAGES) * TILE;
+  static constexpr int BK = D == 128 ? 80 : 128;    // keys of a block
+  static constexpr int PANELS = D / 64;             // of 64 elements, rows of 128 bytes, swizzled
+  static constexpr int Q_PANEL = BQ * 128, Q_TILE = PANELS * Q_PANEL;
+  static constexpr int PANEL = BK * 128, TILE = PANELS * PANEL;      // a K or V block
+  static constexpr int STAGES = D == 128 ? 8 : 10;
+  static constexpr int BYTES = 2 * Q_TILE + STAGES * TILE;
+  // first columns of row tile 0, and from one row tile to the next
+  static constexpr uint32_t S_COL = 0, S_STEP = 128, O_COL = D == 128 ? 256 : 384, O_STEP = D;
+  static constexpr uint32_t P_COL = D == 128 ? 80 : 256, P_STEP = D == 128 ? 128 : 64;
 };
 constexpr int MAX_STAGES = 10;
 
@@ -85,9 +88,9 @@ struct Tile {
 struct Shared {
   uint64_t q_full[2], q_empty[2];
   uint64_t full[MAX_STAGES], empty[MAX_STAGES];
-  uint64_t s_full[2], p_full[2], pv_done[2], o_free[2];
+  uint64_t s_full[2], s_free[2], p_full[2], pv_done[2], o_free[2];
   uint64_t tail[MAX_STAGES];        // a V block with rows past the last key has arrived
-  uint64_t drain;
+  uint64_t drain[2];
   uint64_t sched_full[SCHED], sched_empty[SCHED];
   Tile tile[SCHED];
   uint32_t tmem_base;
@@ -160,6 +163,115 @@ __device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
   return r;
 }
 
+// A block of this thread's TMEM lane, loaded (stored) and waited for in one
+// statement: the registers are the compiler's to move once it ends.
+__device__ __forceinline__ void tmem_ld_block(uint32_t taddr, uint32_t (&r)[128]) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x64.b32 {"
+      "%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
+      "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31, "
+      "%32, %33, %34, %35, %36, %37, %38, %39, %40, %41, %42, %43, %44, %45, %46, %47, "
+      "%48, %49, %50, %51, %52, %53, %54, %55, %56, %57, %58, %59, %60, %61, %62, %63 "
+      "}, [%128];\n"
+      "tcgen05.ld.sync.aligned.32x32b.x64.b32 {"
+      "%64, %65, %66, %67, %68, %69, %70, %71, %72, %73, %74, %75, %76, %77, %78, %79, "
+      "%80, %81, %82, %83, %84, %85, %86, %87, %88, %89, %90, %91, %92, %93, %94, %95, "
+      "%96, %97, %98, %99, %100, %101, %102, %103, %104, %105, %106, %107, %108, %109, %110, %111, "
+      "%112, %113, %114, %115, %116, %117, %118, %119, %120, %121, %122, %123, %124, %125, %126, %127 "
+      "}, [%129];\n"
+      "tcgen05.wait::ld.sync.aligned;"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
+        "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]),
+        "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]),
+        "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31]),
+        "=r"(r[32]), "=r"(r[33]), "=r"(r[34]), "=r"(r[35]), "=r"(r[36]), "=r"(r[37]), "=r"(r[38]), "=r"(r[39]),
+        "=r"(r[40]), "=r"(r[41]), "=r"(r[42]), "=r"(r[43]), "=r"(r[44]), "=r"(r[45]), "=r"(r[46]), "=r"(r[47]),
+        "=r"(r[48]), "=r"(r[49]), "=r"(r[50]), "=r"(r[51]), "=r"(r[52]), "=r"(r[53]), "=r"(r[54]), "=r"(r[55]),
+        "=r"(r[56]), "=r"(r[57]), "=r"(r[58]), "=r"(r[59]), "=r"(r[60]), "=r"(r[61]), "=r"(r[62]), "=r"(r[63]),
+        "=r"(r[64]), "=r"(r[65]), "=r"(r[66]), "=r"(r[67]), "=r"(r[68]), "=r"(r[69]), "=r"(r[70]), "=r"(r[71]),
+        "=r"(r[72]), "=r"(r[73]), "=r"(r[74]), "=r"(r[75]), "=r"(r[76]), "=r"(r[77]), "=r"(r[78]), "=r"(r[79]),
+        "=r"(r[80]), "=r"(r[81]), "=r"(r[82]), "=r"(r[83]), "=r"(r[84]), "=r"(r[85]), "=r"(r[86]), "=r"(r[87]),
+        "=r"(r[88]), "=r"(r[89]), "=r"(r[90]), "=r"(r[91]), "=r"(r[92]), "=r"(r[93]), "=r"(r[94]), "=r"(r[95]),
+        "=r"(r[96]), "=r"(r[97]), "=r"(r[98]), "=r"(r[99]), "=r"(r[100]), "=r"(r[101]), "=r"(r[102]), "=r"(r[103]),
+        "=r"(r[104]), "=r"(r[105]), "=r"(r[106]), "=r"(r[107]), "=r"(r[108]), "=r"(r[109]), "=r"(r[110]), "=r"(r[111]),
+        "=r"(r[112]), "=r"(r[113]), "=r"(r[114]), "=r"(r[115]), "=r"(r[116]), "=r"(r[117]), "=r"(r[118]), "=r"(r[119]),
+        "=r"(r[120]), "=r"(r[121]), "=r"(r[122]), "=r"(r[123]), "=r"(r[124]), "=r"(r[125]), "=r"(r[126]), "=r"(r[127])
+      : "r"(taddr), "r"(taddr + 64)
+      : "memory");
+}
+__device__ __forceinline__ void tmem_ld_block(uint32_t taddr, uint32_t (&r)[80]) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x64.b32 {"
+      "%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
+      "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31, "
+      "%32, %33, %34, %35, %36, %37, %38, %39, %40, %41, %42, %43, %44, %45, %46, %47, "
+      "%48, %49, %50, %51, %52, %53, %54, %55, %56, %57, %58, %59, %60, %61, %62, %63 "
+      "}, [%80];\n"
+      "tcgen05.ld.sync.aligned.32x32b.x16.b32 {"
+      "%64, %65, %66, %67, %68, %69, %70, %71, %72, %73, %74, %75, %76, %77, %78, %79 "
+      "}, [%81];\n"
+      "tcgen05.wait::ld.sync.aligned;"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
+        "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]),
+        "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]),
+        "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31]),
+        "=r"(r[32]), "=r"(r[33]), "=r"(r[34]), "=r"(r[35]), "=r"(r[36]), "=r"(r[37]), "=r"(r[38]), "=r"(r[39]),
+        "=r"(r[40]), "=r"(r[41]), "=r"(r[42]), "=r"(r[43]), "=r"(r[44]), "=r"(r[45]), "=r"(r[46]), "=r"(r[47]),
+        "=r"(r[48]), "=r"(r[49]), "=r"(r[50]), "=r"(r[51]), "=r"(r[52]), "=r"(r[53]), "=r"(r[54]), "=r"(r[55]),
+        "=r"(r[56]), "=r"(r[57]), "=r"(r[58]), "=r"(r[59]), "=r"(r[60]), "=r"(r[61]), "=r"(r[62]), "=r"(r[63]),
+        "=r"(r[64]), "=r"(r[65]), "=r"(r[66]), "=r"(r[67]), "=r"(r[68]), "=r"(r[69]), "=r"(r[70]), "=r"(r[71]),
+        "=r"(r[72]), "=r"(r[73]), "=r"(r[74]), "=r"(r[75]), "=r"(r[76]), "=r"(r[77]), "=r"(r[78]), "=r"(r[79])
+      : "r"(taddr), "r"(taddr + 64)
+      : "memory");
+}
+__device__ __forceinline__ void tmem_st_block(uint32_t taddr, const uint32_t (&r)[64]) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x64.b32 [%64], {"
+      "%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
+      "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31, "
+      "%32, %33, %34, %35, %36, %37, %38, %39, %40, %41, %42, %43, %44, %45, %46, %47, "
+      "%48, %49, %50, %51, %52, %53, %54, %55, %56, %57, %58, %59, %60, %61, %62, %63 "
+      "};\n"
+      "tcgen05.wait::st.sync.aligned;" ::"r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]),
+        "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]),
+        "r"(r[16]), "r"(r[17]), "r"(r[18]), "r"(r[19]), "r"(r[20]), "r"(r[21]), "r"(r[22]), "r"(r[23]),
+        "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]), "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31]),
+        "r"(r[32]), "r"(r[33]), "r"(r[34]), "r"(r[35]), "r"(r[36]), "r"(r[37]), "r"(r[38]), "r"(r[39]),
+        "r"(r[40]), "r"(r[41]), "r"(r[42]), "r"(r[43]), "r"(r[44]), "r"(r[45]), "r"(r[46]), "r"(r[47]),
+        "r"(r[48]), "r"(r[49]), "r"(r[50]), "r"(r[51]), "r"(r[52]), "r"(r[53]), "r"(r[54]), "r"(r[55]),
+        "r"(r[56]), "r"(r[57]), "r"(r[58]), "r"(r[59]), "r"(r[60]), "r"(r[61]), "r"(r[62]), "r"(r[63]),
+        "r"(taddr)
+      : "memory");
+}
+__device__ __forceinline__ void tmem_st_block(uint32_t taddr, const uint32_t (&r)[40]) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x32.b32 [%40], {"
+      "%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
+      "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31 "
+      "};\n"
+      "tcgen05.st.sync.aligned.32x32b.x8.b32 [%41], {"
+      "%32, %33, %34, %35, %36, %37, %38, %39 "
+      "};\n"
+      "tcgen05.wait::st.sync.aligned;" ::"r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]),
+        "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]),
+        "r"(r[16]), "r"(r[17]), "r"(r[18]), "r"(r[19]), "r"(r[20]), "r"(r[21]), "r"(r[22]), "r"(r[23]),
+        "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]), "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31]),
+        "r"(r[32]), "r"(r[33]), "r"(r[34]), "r"(r[35]), "r"(r[36]), "r"(r[37]), "r"(r[38]), "r"(r[39]),
+        "r"(taddr), "r"(taddr + 32)
+      : "memory");
+}
+
+// registers per thread after the split of a launch's 168 x 384 between the
+// softmax warps (8) and the other four: 208 x 256 + 80 x 128 = 63,488 of 64,512
+template <int N>
+__device__ __forceinline__ void more_registers() {
+  asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N));
+}
+template <int N>
+__device__ __forceinline__ void fewer_registers() {
+  asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N));
+}
+
 // -- the order of tiles -----------------------------------------------------------
 // Tile i of a sequence (n tokens, m keys) holds tokens [i T, (i + 1) T), T = two row
 // tiles; its weight is the number of key blocks that its last token sees.  Tiles
@@ -180,6 +292,7 @@ __device__ __forceinline__ Seq sequence(const KtirPromptDesc& d, long long b, in
 }
 
 // tiles of weight at least `w`: the last ones of the sequence
+template <int BK>
 __device__ __forceinline__ int heavier(const Seq& s, int w, int T, int causal) {
   if (w <= 0) return s.tiles;
   const int need = (w - 1) * BK;             // more than this many keys seen
@@ -195,22 +308,24 @@ __device__ __forceinline__ int warp_sum(int v) {
   return v;
 }
 
+template <int BK>
 __device__ int tiles_of_weight(const KtirPromptDesc& d, int w, int T, int lane) {
   int c = 0;
   for (long long b = lane; b < d.batch; b += 32) {
     bool bad;
-    c += heavier(sequence(d, b, T, bad), w, T, d.causal);
+    c += heavier<BK>(sequence(d, b, T, bad), w, T, d.causal);
   }
   return warp_sum(c);
 }
 
 // tile number `x` (0 = heaviest), by one warp
+template <int BK>
 __device__ void find_tile(const KtirPromptDesc& d, int x, int head, int T, int heaviest, int lane, Tile& t) {
   int lo = 0, hi = heaviest + 1;             // count(lo) > x >= count(hi)
   int above = 0;
   while (hi - lo > 1) {
     const int mid = (lo + hi) >> 1;
-    const int c = tiles_of_weight(d, mid, T, lane);
+    const int c = tiles_of_weight<BK>(d, mid, T, lane);
     if (c > x) {
       lo = mid;
     } else {
@@ -226,8 +341,8 @@ __device__ void find_tile(const KtirPromptDesc& d, int x, int head, int T, int h
     bool bad;
     if (b < d.batch) {
       s = sequence(d, b, T, bad);
-      const int c = heavier(s, lo, T, d.causal);
-      count = c - heavier(s, lo + 1, T, d.causal);
+      const int c = heavier<BK>(s, lo, T, d.causal);
+      count = c - heavier<BK>(s, lo + 1, T, d.causal);
       first = s.tiles - c;
     }
     int incl = count;
@@ -266,13 +381,13 @@ __global__ void __launch_bounds__(THREADS, 1)
                        const __grid_constant__ CUtensorMap tv, const __grid_constant__ PromptParams p) {
   using C = Cfg<D>;
   constexpr uint32_t TYPE = sizeof(T) == 2 && Elem<T>::BF16 ? (1u << 7) | (1u << 10) : 0u;
-  constexpr int STAGES = C::STAGES;
+  constexpr int STAGES = C::STAGES, BK = C::BK;
   extern __shared__ uint8_t smem_raw[];
   __shared__ Shared B;
   const KtirPromptDesc& d = p.d;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const uint32_t base = (smem_u32(smem_raw) + 1023u) & ~1023u;
-  const uint32_t sQ = base, ring = base + 2 * C::TILE;
+  const uint32_t sQ = base, ring = base + 2 * C::Q_TILE;
   volatile int* abort = &B.abort_flag;
 
   if (tid == 0) {
@@ -281,16 +396,17 @@ __global__ void __launch_bounds__(THREADS, 1)
       mbar_init(smem_u32(&B.q_full[w]), 1);
       mbar_init(smem_u32(&B.q_empty[w]), 1);
       mbar_init(smem_u32(&B.s_full[w]), 1);
+      mbar_init(smem_u32(&B.s_free[w]), 4);
       mbar_init(smem_u32(&B.p_full[w]), 4);
       mbar_init(smem_u32(&B.pv_done[w]), 1);
       mbar_init(smem_u32(&B.o_free[w]), 4);
     }
     for (int s = 0; s < STAGES; ++s) {
       mbar_init(smem_u32(&B.full[s]), 1);
-      mbar_init(smem_u32(&B.empty[s]), 1);
+      mbar_init(smem_u32(&B.empty[s]), 2);
       mbar_init(smem_u32(&B.tail[s]), 1);
     }
-    mbar_init(smem_u32(&B.drain), 1);
+    for (int w = 0; w < 2; ++w) mbar_init(smem_u32(&B.drain[w]), 1);
     for (int s = 0; s < SCHED; ++s) {
       mbar_init(smem_u32(&B.sched_full[s]), 1);
       mbar_init(smem_u32(&B.sched_empty[s]), SCHED_READERS);
@@ -305,6 +421,8 @@ __global__ void __launch_bounds__(THREADS, 1)
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = B.tmem_base;
+  pdl_launch();
+  pdl_wait();
 
   // announced tiles, read by whole warps: false at the end (or on an abort)
   auto next_tile = [&](int k, Tile& t) -> bool {
@@ -316,89 +434,126 @@ __global__ void __launch_bounds__(THREADS, 1)
     return !t.stop;
   };
 
-  if (warp == 11) {
-    // ---------------- tile finder ----------------
-    const int span = 2 * p.tile_tokens;
-    int heaviest = 0, total = 0;
-    bool any_bad = false;
-    for (long long b = lane; b < d.batch; b += 32) {
-      bool bad;
-      const Seq s = sequence(d, b, span, bad);
-      any_bad |= bad;
-      if (s.n) heaviest = max(heaviest, (s.m + BK - 1) / BK);
-      total += s.tiles;
-    }
-    if (blockIdx.x == 0) {
-      if (lane == 0) any_bad |= d.offsets[0] != 0 || d.offsets[d.batch] != d.tokens;
-      if (any_bad) atomicOr(d.status, KTIR_STATUS_BAD_INDEX);
-    }
-    total = warp_sum(total);
-#pragma unroll
-    for (int w = 16; w; w >>= 1) heaviest = max(heaviest, __shfl_xor_sync(0xffffffffu, heaviest, w));
-    const long long all = (long long)total * d.kv_heads;
-    for (int k = 0;; ++k) {
-      const long long x = (long long)k * gridDim.x + ((k & 1) ? gridDim.x - 1 - blockIdx.x : blockIdx.x);
-      const int s = k % SCHED;
-      if (k >= SCHED &&
-          !__all_sync(0xffffffffu, wait(smem_u32(&B.sched_empty[s]), (k / SCHED - 1) & 1, abort)))
-        break;
-      // back and forth, a CTA may have a tile in the last round after having none before it
-      const bool stop = (long long)k * gridDim.x >= all;
-      if (stop) {
-        if (lane == 0) B.tile[s].stop = 1;
-      } else if (x < all) {
-        find_tile(d, (int)(x / d.kv_heads), (int)(x % d.kv_heads), span, heaviest, lane, B.tile[s]);
-      } else if (lane == 0) {
-        Tile& t = B.tile[s];
-        t.stop = 0;
-        t.tokens = t.blocks[0] = t.blocks[1] = t.keys = 0;
-        t.token = t.key0 = t.head = 0;
-        t.seen = 0;
+  if (warp >= 8) {
+    fewer_registers<OTHER_REGS>();
+    if (warp == 11) {
+      // ---------------- tile finder ----------------
+      const int span = 2 * p.tile_tokens;
+      int heaviest = 0, total = 0;
+      bool any_bad = false;
+      for (long long b = lane; b < d.batch; b += 32) {
+        bool bad;
+        const Seq s = sequence(d, b, span, bad);
+        any_bad |= bad;
+        if (s.n) heaviest = max(heaviest, (s.m + BK - 1) / BK);
+        total += s.tiles;
       }
-      __syncwarp();
-      if (lane == 0) mbar_arrive(smem_u32(&B.sched_full[s]));
-      if (stop) break;
-    }
-  } else if (warp == 9) {
-    // ---------------- TMA ----------------
-    const bool leader = elect();
-    if (leader) {
-      tma_prefetch_desc(&tq);
-      tma_prefetch_desc(&tk);
-      tma_prefetch_desc(&tv);
-    }
-    const uint32_t q_bytes = (uint32_t)(p.group * p.tile_tokens) * 128u * C::PANELS;
-    int loads = 0, q_loads[2] = {0, 0};
-    uint32_t was_tail = 0, tail_phase = 0;      // per ring stage: last load, next phase's parity
-    Tile t;
-    bool ok = true;
-    for (int k = 0; ok && next_tile(k, t); ++k) {
-      if (leader) {
-        const int blocks = max(t.blocks[0], t.blocks[1]);
-        for (int j = 0; ok && j < blocks; ++j) {
-          if (j == 0) {
-            for (int w = 0; ok && w < 2; ++w) {
-              if (!t.blocks[w]) continue;
-              if (q_loads[w] && !wait(smem_u32(&B.q_empty[w]), (q_loads[w] - 1) & 1, abort)) {
-                ok = false;
-                break;
-              }
-              const uint32_t bar = smem_u32(&B.q_full[w]);
-              mbar_arrive_expect_tx(bar, q_bytes);
-#pragma unroll
-              for (int c = 0; c < C::PANELS; ++c)
-                tma_load_3d(sQ + w * C::TILE + c * C::PANEL, &tq, bar, 64 * c, t.head * p.q_head_step,
-                            t.token + w * p.tile_tokens);
-              ++q_loads[w];
-            }
+      if (blockIdx.x == 0) {
+        if (lane == 0) any_bad |= d.offsets[0] != 0 || d.offsets[d.batch] != d.tokens;
+        if (any_bad) atomicOr(d.status, KTIR_STATUS_BAD_INDEX);
+      }
+      total = warp_sum(total);
+  #pragma unroll
+      for (int w = 16; w; w >>= 1) heaviest = max(heaviest, __shfl_xor_sync(0xffffffffu, heaviest, w));
+      const long long all = (long long)total * d.kv_heads;
+      int next = 0, fix = 0, loads = 0;         // tile to announce, tile to look after, ring loads before it
+      bool stop = false;
+      uint32_t phase = 0;                       // of the ring stages' tail barriers
+      for (uint32_t idle = 0; !stop || fix < next - 1;) {
+        bool moved = false;
+        const int s = next % SCHED;
+        if (!stop && next < fix + SCHED &&
+            (next < SCHED || __all_sync(0xffffffffu, mbar_test_wait(smem_u32(&B.sched_empty[s]),
+                                                                    (next / SCHED - 1) & 1)))) {
+          const long long x =
+              (long long)next * gridDim.x + ((next & 1) ? gridDim.x - 1 - blockIdx.x : blockIdx.x);
+          // back and forth, a CTA may have a tile in the last round after having none before it
+          stop = (long long)next * gridDim.x >= all;
+          if (stop) {
+            if (lane == 0) B.tile[s].stop = 1;
+          } else if (x < all) {
+            find_tile<BK>(d, (int)(x / d.kv_heads), (int)(x % d.kv_heads), span, heaviest, lane, B.tile[s]);
+          } else if (lane == 0) {
+            Tile& t = B.tile[s];
+            t.stop = 0;
+            t.tokens = t.blocks[0] = t.blocks[1] = t.keys = 0;
+            t.token = t.key0 = t.head = 0;
+            t.seen = 0;
           }
-          for (int kv = 0; ok && kv < 2; ++kv, ++loads) {
-            const int s = loads % STAGES;
-            if (loads >= STAGES && !wait(smem_u32(&B.empty[s]), (loads / STAGES - 1) & 1, abort)) {
+          __syncwarp();
+          if (lane == 0) mbar_arrive(smem_u32(&B.sched_full[s]));
+          ++next;
+          moved = true;
+        }
+        if (fix < next - (stop ? 1 : 0)) {
+          // V rows past the last key of tile `fix`
+          const Tile& t = B.tile[fix % SCHED];
+          const int blocks = max(t.blocks[0], t.blocks[1]), left = t.keys - (blocks - 1) * BK;
+          const int r = (loads + 2 * blocks - 1) % STAGES;
+          const bool tail = blocks && left < BK;
+          if (!tail || __all_sync(0xffffffffu, mbar_test_wait(smem_u32(&B.tail[r]), (phase >> r) & 1))) {
+            if (tail) {
+              phase ^= 1u << r;
+              uint8_t* v = smem_raw + (ring + r * C::TILE - smem_u32(smem_raw));
+              // whole 128-byte rows of each panel: the swizzle permutes within a row
+              for (int i = left * 8 + lane; i < BK * 8; i += 32)
+#pragma unroll
+                for (int c = 0; c < C::PANELS; ++c)
+                  *reinterpret_cast<uint4*>(v + c * C::PANEL + i * 16) = make_uint4(0, 0, 0, 0);
+              fence_proxy_async();
+              __syncwarp();
+              if (lane == 0) mbar_arrive(smem_u32(&B.full[r]));
+            }
+            loads += 2 * blocks;
+            ++fix;
+            moved = true;
+          }
+        }
+        if (moved) {
+          idle = 0;
+        } else {
+          if (__any_sync(0xffffffffu, *abort != 0)) break;
+          if (++idle > kSpinLimit) {
+            *abort = 1;
+            break;
+          }
+          __nanosleep(40);
+        }
+      }
+    } else if (warp == 9) {
+      // ---------------- TMA ----------------
+      const bool leader = elect();
+      if (leader) {
+        tma_prefetch_desc(&tq);
+        tma_prefetch_desc(&tk);
+        tma_prefetch_desc(&tv);
+      }
+      const uint32_t q_bytes = (uint32_t)(p.group * p.tile_tokens) * 128u * C::PANELS;
+      int loads = 0, q_loads[2] = {0, 0};
+      uint32_t was_tail = 0, tail_phase = 0;      // per ring stage: last load, next phase's parity
+      Tile t;
+      bool ok = true;
+      for (int k = 0; ok && next_tile(k, t); ++k) {
+          if (leader) {
+          const int blocks = max(t.blocks[0], t.blocks[1]);
+          for (int w = 0; ok && w < 2; ++w) {
+            if (!t.blocks[w]) continue;
+            if (q_loads[w] && !wait(smem_u32(&B.q_empty[w]), (q_loads[w] - 1) & 1, abort)) {
               ok = false;
               break;
             }
-            // V rows past the last key: warp 10 passes the block on when it has cleared them
+            const uint32_t bar = smem_u32(&B.q_full[w]);
+            mbar_arrive_expect_tx(bar, q_bytes);
+#pragma unroll
+            for (int c = 0; c < C::PANELS; ++c)
+              tma_load_3d(sQ + w * C::Q_TILE + c * C::Q_PANEL, &tq, bar, 64 * c, t.head * p.q_head_step,
+                          t.token + w * p.tile_tokens);
+            ++q_loads[w];
+          }
+          auto load = [&](bool kv, int j) -> bool {
+            const int s = loads % STAGES;
+            if (loads >= STAGES && !wait(smem_u32(&B.empty[s]), (loads / STAGES - 1) & 1, abort)) return false;
+            // V rows past the last key: warp 11 passes the block on when it has cleared them
             const bool tail = kv && (j + 1) * BK > t.keys;
             const uint32_t bar = smem_u32(tail ? &B.tail[s] : &B.full[s]);
             was_tail = (was_tail & ~(1u << s)) | (tail ? 1u << s : 0u);
@@ -408,164 +563,140 @@ __global__ void __launch_bounds__(THREADS, 1)
             for (int c = 0; c < C::PANELS; ++c)
               tma_load_3d(ring + s * C::TILE + c * C::PANEL, kv ? &tv : &tk, bar, 64 * c,
                           t.head * (kv ? p.v_head_step : p.k_head_step), t.key0 + j * BK);
+            ++loads;
+            return true;
+          };
+          // in the order of their use: K_0, K_1, then V_j and K_{j+2}
+          for (int j = 0; ok && j < 2 && j < blocks; ++j) ok = load(false, j);
+          for (int j = 0; ok && j < blocks; ++j) {
+            ok = load(true, j);
+            if (ok && j + 2 < blocks) ok = load(false, j + 2);
           }
         }
+        ok = __all_sync(0xffffffffu, ok);
       }
-      ok = __all_sync(0xffffffffu, ok);
-    }
-    if (leader && *abort) {
-      // leave no copy in flight
-      int none = 0;
-      for (int s = 0; s < STAGES && s < loads; ++s) {
-        if ((was_tail >> s) & 1) wait(smem_u32(&B.tail[s]), ((tail_phase >> s) & 1) ^ 1, &none);
-        else wait(smem_u32(&B.full[s]), ((loads - 1 - s) / STAGES) & 1, &none);
+      if (leader && *abort) {
+        // leave no copy in flight
+        int none = 0;
+        for (int s = 0; s < STAGES && s < loads; ++s) {
+          if ((was_tail >> s) & 1) wait(smem_u32(&B.tail[s]), ((tail_phase >> s) & 1) ^ 1, &none);
+          else wait(smem_u32(&B.full[s]), ((loads - 1 - s) / STAGES) & 1, &none);
+        }
+        for (int w = 0; w < 2; ++w)
+          if (q_loads[w]) wait(smem_u32(&B.q_full[w]), (q_loads[w] - 1) & 1, &none);
       }
-      for (int w = 0; w < 2; ++w)
-        if (q_loads[w]) wait(smem_u32(&B.q_full[w]), (q_loads[w] - 1) & 1, &none);
-    }
-  } else if (warp == 10) {
-    // ---------------- V rows past the last key ----------------
-    int loads = 0;
-    uint32_t phase = 0;                                 // per ring stage
-    Tile t;
-    for (int k = 0; next_tile(k, t); ++k) {
-      const int blocks = max(t.blocks[0], t.blocks[1]);
-      const int left = t.keys - (blocks - 1) * BK;      // keys of the last block that exist
-      if (blocks && left < BK) {
-        const int at = loads + 2 * blocks - 1, s = at % STAGES;
-        if (!__all_sync(0xffffffffu, wait(smem_u32(&B.tail[s]), (phase >> s) & 1, abort))) break;
-        phase ^= 1u << s;
-        uint8_t* v = smem_raw + (ring + s * C::TILE - smem_u32(smem_raw));
-        // whole 128-byte rows of each panel: the swizzle permutes within a row
-        for (int i = left * 8 + lane; i < BK * 8; i += 32)
-#pragma unroll
-          for (int c = 0; c < C::PANELS; ++c)
-            *reinterpret_cast<uint4*>(v + c * C::PANEL + i * 16) = make_uint4(0, 0, 0, 0);
-        fence_proxy_async();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(smem_u32(&B.full[s]));
-      }
-      loads += 2 * blocks;
-    }
-  } else if (warp == 8) {
-    // ---------------- MMA ----------------
-    // One thread issues every product, so what it does between two of them is
-    // kept short: no indexing of local arrays, no division, descriptors by
-    // adding to constants.
-    constexpr uint32_t idesc_s = idesc_f16(BQ, BK, 0, 0) | TYPE;     // Q and K both K-major
-    constexpr uint32_t idesc_pv = idesc_f16(BQ, D, 0, 1) | TYPE;     // P K-major, V MN-major
-    const uint64_t q_desc = sdesc_sw128(sQ, 16, 1024), k_desc = sdesc_sw128(ring, 16, 1024),
-                   v_desc = sdesc_sw128(ring, C::PANEL, 1024);
-    uint32_t stage = 0, ring_phase = 0;         // next ring load to wait for
-    uint32_t p_phase = 0, q_phase = 0, o_phase = 0, o_used = 0;      // bit w: row tile w
-    auto next_load = [&]() -> bool {            // the next load has arrived
-      const bool ok = wait(smem_u32(&B.full[stage]), ring_phase, abort);
-      if (++stage == STAGES) {
-        stage = 0;
-        ring_phase ^= 1;
-      }
-      return ok;
-    };
-    const bool leader = elect();
-    Tile t;
-    bool ok = true;
-    for (int k = 0; ok && next_tile(k, t); ++k) {
-      if (leader) {
-        const int blocks0 = t.blocks[0], blocks1 = t.blocks[1], blocks = max(blocks0, blocks1);
-        uint32_t k_stage = stage, v_stage = 0;
-        auto issue_s = [&](auto W, int j) {
-          constexpr int w = decltype(W)::value;
-          const uint64_t q = q_desc + (uint64_t)(w * (C::TILE >> 4));
-          const uint64_t kb = k_desc + (uint64_t)(k_stage * (C::TILE >> 4));
-#pragma unroll
-          for (int kk = 0; kk < D / 16; ++kk) {
-            const uint64_t off = ((kk >> 2) * C::PANEL + (kk & 3) * 32) >> 4;
-            mma_f16(tmem + w * BK, q + off, kb + off, idesc_s, kk != 0);
-          }
-          mma_commit(smem_u32(&B.s_full[w]));
-          if (j + 1 == (w ? blocks1 : blocks0)) mma_commit(smem_u32(&B.q_empty[w]));
+    } else {
+      // ---------------- MMA, one warp per row tile ----------------
+      // One thread issues a row tile's products, and its waits, one after the
+      // other, are on the way of every block: so there is one for each row tile,
+      // and what it does between two products is kept short.
+      auto mma = [&](auto W) {
+        constexpr int w = decltype(W)::value;
+        constexpr uint32_t idesc_s = idesc_f16(BQ, BK, 0, 0) | TYPE;     // Q and K both K-major
+        constexpr uint32_t idesc_pv = idesc_f16(BQ, D, 0, 1) | TYPE;     // P K-major, V MN-major
+        const uint64_t q_desc = sdesc_sw128(sQ + w * C::Q_TILE, 16, 1024), k_desc = sdesc_sw128(ring, 16, 1024),
+                       v_desc = sdesc_sw128(ring, C::PANEL, 1024);
+        const uint32_t S = tmem + C::S_COL + w * C::S_STEP, P = tmem + C::P_COL + w * C::P_STEP,
+                       O = tmem + C::O_COL + w * C::O_STEP;
+        uint32_t stage = 0, ring_phase = 0;         // next ring load to wait for
+        uint32_t p_phase = 0, q_phase = 0;
+        uint32_t o_phase = 1, s_phase = 1;          // a first wait for these is over at once
+        auto next_load = [&]() -> bool {
+          return wait(smem_u32(&B.full[stage]), ring_phase, abort);
         };
-        auto issue_pv = [&](auto W, int j) -> bool {
-          constexpr int w = decltype(W)::value;
-          if (!wait(smem_u32(&B.p_full[w]), (p_phase >> w) & 1, abort)) return false;
-          p_phase ^= 1u << w;
-          if (j == 0) {
-            if ((o_used >> w) & 1) {            // O of the tile before has been read
-              if (!wait(smem_u32(&B.o_free[w]), (o_phase >> w) & 1, abort)) return false;
-              o_phase ^= 1u << w;
+        auto advance = [&]() {
+          if (++stage == STAGES) {
+            stage = 0;
+            ring_phase ^= 1;
+          }
+        };
+        const bool leader = elect();
+        Tile t;
+        bool ok = true;
+        for (int k = 0; ok && next_tile(k, t); ++k) {
+          if (leader) {
+            const int mine = t.blocks[w], blocks = max(mine, t.blocks[w ^ 1]);
+            // S(j) from the K block just arrived, which both row tiles give back
+            auto issue_s = [&](int j) -> bool {
+              if (!next_load()) return false;
+              const uint32_t bar = smem_u32(&B.empty[stage]);
+              if (j < mine) {
+                if (j == 0) {
+                  if (!wait(smem_u32(&B.q_full[w]), q_phase, abort)) return false;
+                  q_phase ^= 1;
+                }
+                // the block before is in registers
+                if (!wait(smem_u32(&B.s_free[w]), s_phase, abort)) return false;
+                s_phase ^= 1;
+                tc_fence_after();
+                const uint64_t kb = k_desc + (uint64_t)(stage * (C::TILE >> 4));
+#pragma unroll
+                for (int kk = 0; kk < D / 16; ++kk)
+                  mma_f16(S, q_desc + (((kk >> 2) * C::Q_PANEL + (kk & 3) * 32) >> 4),
+                          kb + (((kk >> 2) * C::PANEL + (kk & 3) * 32) >> 4), idesc_s, kk != 0);
+                mma_commit(smem_u32(&B.s_full[w]));
+                mma_commit(bar);
+                if (j + 1 == mine) mma_commit(smem_u32(&B.q_empty[w]));
+              } else {
+                mbar_arrive(bar);
+              }
+              advance();
+              return true;
+            };
+            auto issue_pv = [&](int j) -> bool {
+              if (!next_load()) return false;
+              const uint32_t bar = smem_u32(&B.empty[stage]);
+              if (j < mine) {
+                if (j == 0) {                       // O of the tile before has been read
+                  if (!wait(smem_u32(&B.o_free[w]), o_phase, abort)) return false;
+                  o_phase ^= 1;
+                }
+                if (!wait(smem_u32(&B.p_full[w]), p_phase, abort)) return false;
+                p_phase ^= 1;
+                tc_fence_after();
+                const uint64_t v = v_desc + (uint64_t)(stage * (C::TILE >> 4));
+#pragma unroll
+                for (int kk = 0; kk < BK / 16; ++kk)
+                  mma_f16_ts(O, P + kk * 8, v + (uint64_t)((kk * 16 * 128) >> 4), idesc_pv,
+                             kk == 0 ? (uint32_t)(j != 0) : 1u);
+                mma_commit(smem_u32(&B.pv_done[w]));
+                mma_commit(bar);
+              } else {
+                mbar_arrive(bar);
+              }
+              advance();
+              return true;
+            };
+            for (int j = 0; ok && j < 2 && j < blocks; ++j) ok = issue_s(j);
+            for (int j = 0; ok && j < blocks; ++j) {
+              ok = issue_pv(j);
+              if (ok && j + 2 < blocks) ok = issue_s(j + 2);
             }
-            o_used |= 1u << w;
           }
-          tc_fence_after();
-          const uint64_t v = v_desc + (uint64_t)(v_stage * (C::TILE >> 4));
-#pragma unroll
-          for (int kk = 0; kk < BK / 16; ++kk)
-            mma_f16_ts(tmem + O_COL + w * D, tmem + w * BK + kk * 8, v + (uint64_t)((kk * 16 * 128) >> 4), idesc_pv,
-                       kk == 0 ? (uint32_t)(j != 0) : 1u);
-          mma_commit(smem_u32(&B.pv_done[w]));
-          return true;
-        };
-        using W0 = std::integral_constant<int, 0>;
-        using W1 = std::integral_constant<int, 1>;
-        if (blocks) {
-          ok = next_load();                     // K_0
-          if (ok && blocks0) {
-            ok = wait(smem_u32(&B.q_full[0]), q_phase & 1, abort);
-            q_phase ^= 1;
-            tc_fence_after();
-            if (ok) issue_s(W0(), 0);
-          }
-          if (ok && blocks1) {
-            ok = wait(smem_u32(&B.q_full[1]), q_phase >> 1, abort);
-            q_phase ^= 2;
-            tc_fence_after();
-            if (ok) issue_s(W1(), 0);
-          }
-          if (ok) mma_commit(smem_u32(&B.empty[k_stage]));
+          ok = __all_sync(0xffffffffu, ok);
         }
-        for (int j = 0; ok && j < blocks; ++j) {
-          v_stage = stage;
-          ok = next_load();                     // V_j
-          if (!ok) break;
-          const bool more = j + 1 < blocks;
-          if (j < blocks0) {
-            ok = issue_pv(W0(), j);
-            if (!ok) break;
-          }
-          if (more) {
-            k_stage = stage;
-            ok = next_load();                   // K_{j+1}
-            if (!ok) break;
-            tc_fence_after();
-          }
-          if (j + 1 < blocks0) issue_s(W0(), j + 1);
-          if (j < blocks1) {
-            ok = issue_pv(W1(), j);
-            if (!ok) break;
-          }
-          mma_commit(smem_u32(&B.empty[v_stage]));
-          if (j + 1 < blocks1) issue_s(W1(), j + 1);
-          if (more) mma_commit(smem_u32(&B.empty[k_stage]));
+        if (leader && *abort) {
+          int none = 0;
+          mma_commit(smem_u32(&B.drain[w]));
+          wait(smem_u32(&B.drain[w]), 0, &none);
         }
-      }
-      ok = __all_sync(0xffffffffu, ok);
-    }
-    if (leader && *abort) {
-      int none = 0;
-      mma_commit(smem_u32(&B.drain));
-      wait(smem_u32(&B.drain), 0, &none);
+      };
+      if (warp == 8) mma(std::integral_constant<int, 0>());
+      else mma(std::integral_constant<int, 1>());
     }
   } else {
     // ---------------- softmax, one row per thread ----------------
+    more_registers<SOFTMAX_REGS>();
     const int w = warp >> 2;
     const int row = tid & 127;
-    const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
-    const uint32_t S = tmem + lanes + w * BK, O = tmem + lanes + O_COL + w * D;
+    const uint32_t at_lane = tmem + ((uint32_t)((warp & 3) * 32) << 16);
+    const uint32_t S = at_lane + C::S_COL + w * C::S_STEP, P = at_lane + C::P_COL + w * C::P_STEP,
+                   O = at_lane + C::O_COL + w * C::O_STEP;
     const int token = row / p.group;                 // of the row tile
     const int head_in = row - token * p.group;
     const bool real = token < p.tile_tokens;
     const float c = d.scale * LOG2E;
-    int n_s = 0;
+    int n_s = 0;                                     // blocks so far: S, P and PV each
     Tile t;
     for (int k = 0; next_tile(k, t); ++k) {
       const int at = w * p.tile_tokens + token;       // of the tile's tokens
@@ -578,36 +709,37 @@ __global__ void __launch_bounds__(THREADS, 1)
       for (int j = 0; j < blocks; ++j) {
         ok = __all_sync(0xffffffffu, wait(smem_u32(&B.s_full[w]), n_s & 1, abort));
         if (!ok) break;
-        ++n_s;
         tc_fence_after();
         float s[BK];
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          uint32_t r[64];
-          tmem_ld64_wait(S + 64 * h, r);
-#pragma unroll
-          for (int i = 0; i < 64; ++i) s[64 * h + i] = __uint_as_float(r[i]);
-        }
+        tmem_ld_block(S, reinterpret_cast<uint32_t (&)[BK]>(s));
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(smem_u32(&B.s_free[w]));
         if ((j + 1) * BK > least) {
           const int left = limit - j * BK;
 #pragma unroll
           for (int i = 0; i < BK; ++i)
             if (i >= left) s[i] = -INFINITY;
         }
-        float m8[8];
+        float m4[4];
 #pragma unroll
-        for (int i = 0; i < 8; ++i) m8[i] = fmaxf(s[i], s[8 + i]);
+        for (int x = 0; x < 4; ++x) m4[x] = fmaxf(s[x], s[4 + x]);
 #pragma unroll
-        for (int i = 16; i < BK; i += 16)
+        for (int i = 8; i < BK; i += 8)
 #pragma unroll
-          for (int x = 0; x < 8; ++x) m8[x] = max3(m8[x], s[i + x], s[i + 8 + x]);
-        const float top = fmaxf(max3(m8[0], m8[1], m8[2]), fmaxf(max3(m8[3], m8[4], m8[5]), fmaxf(m8[6], m8[7]))) * c;
+          for (int x = 0; x < 4; ++x) m4[x] = max3(m4[x], s[i + x], s[i + 4 + x]);
+        const float top = fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3])) * c;
         const bool move = top > m + RESCALE_THRESHOLD;     // also from -inf
+        bool done = j == 0;                                // PV of the block before
         if (__any_sync(0xffffffffu, move)) {
           const float f = move ? ex2(m - top) : 1.f;
           if (move) m = top;
           l *= f;
           if (j) {
+            ok = __all_sync(0xffffffffu, wait(smem_u32(&B.pv_done[w]), (n_s - 1) & 1, abort));
+            if (!ok) break;
+            done = true;
+            tc_fence_after();
 #pragma unroll 1
             for (int i = 0; i < D; i += 32) {
               uint32_t r[32];
@@ -621,27 +753,29 @@ __global__ void __launch_bounds__(THREADS, 1)
         const float sub = m == -INFINITY ? 0.f : -m;
         const uint64_t c2 = pack2(c, c), sub2 = pack2(sub, sub);
         uint64_t l4[4] = {0, 0, 0, 0};
+        uint32_t r[BK / 2];
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          uint32_t r[32];
-#pragma unroll
-          for (int i = 0; i < 32; ++i) {
-            const int e = 64 * h + 2 * i;
-            float a, b;
-            unpack2(fma2(pack2(s[e], s[e + 1]), c2, sub2), a, b);
-            a = ex2(a);
-            b = ex2(b);
-            l4[i & 3] = add2(l4[i & 3], pack2(a, b));
-            r[i] = Elem<T>::from2(a, b);
-          }
-          tmem_st32_wait(S + 32 * h, r);
+        for (int i = 0; i < BK / 2; ++i) {
+          float a, b;
+          unpack2(fma2(pack2(s[2 * i], s[2 * i + 1]), c2, sub2), a, b);
+          a = ex2(a);
+          b = ex2(b);
+          l4[i & 3] = add2(l4[i & 3], pack2(a, b));
+          r[i] = Elem<T>::from2(a, b);
         }
-        float a, b;
-        unpack2(add2(add2(l4[0], l4[1]), add2(l4[2], l4[3])), a, b);
-        l += a + b;
+        if (!done) {                                       // it has read P
+          ok = __all_sync(0xffffffffu, wait(smem_u32(&B.pv_done[w]), (n_s - 1) & 1, abort));
+          if (!ok) break;
+          tc_fence_after();
+        }
+        tmem_st_block(P, r);
         tc_fence_before();
         __syncwarp();
         if (lane == 0) mbar_arrive(smem_u32(&B.p_full[w]));
+        float a, b;
+        unpack2(add2(add2(l4[0], l4[1]), add2(l4[2], l4[3])), a, b);
+        l += a + b;
+        ++n_s;
       }
       if (!ok) break;
       const long long tok = (long long)t.token + at;
@@ -739,10 +873,15 @@ int launch(const CUtensorMap& tq, const CUtensorMap& tk, const CUtensorMap& tv, 
     if (cudaFuncSetAttribute(k_prompt_attention<T, D>, cudaFuncAttributeMaxDynamicSharedMemorySize, BYTES) !=
         cudaSuccess)
       return ktir_set_error(KTIR_ERR_CUDA, "ktir_prompt_attention: shared-memory attribute refused");
+    // the split of registers inside the kernel draws on what it is launched with
+    cudaFuncAttributes attr;
+    if (cudaFuncGetAttributes(&attr, k_prompt_attention<T, D>) != cudaSuccess ||
+        attr.numRegs * THREADS < SOFTMAX_REGS * 256 + OTHER_REGS * 128)
+      return ktir_set_error(KTIR_ERR_CUDA, "ktir_prompt_attention: built with too few registers for its split");
     ready[dev] = true;
   }
-  k_prompt_attention<T, D><<<grid, THREADS, BYTES, stream>>>(tq, tk, tv, p);
-  return launched("ktir_prompt_attention: launch failed");
+  return launched(launch_pdl(k_prompt_attention<T, D>, grid, THREADS, BYTES, stream, tq, tk, tv, p),
+                  "ktir_prompt_attention: launch failed");
 }
 
 }  // namespace
@@ -779,13 +918,14 @@ extern "C" int ktir_prompt_attention(const KtirPromptDesc* d, void* stream) {
   // without keys nothing is loaded, but the maps must be valid
   const int64_t none[2] = {d->dim, d->dim};
   const int64_t keys = d->kv_tokens > 0 ? d->kv_tokens : 1;
+  const int block = d->dim == 128 ? Cfg<128>::BK : Cfg<64>::BK;
   CUtensorMap tq, tk, tv;
   if (!make_map(&tq, d->q, bf16, d->dim, d->heads, d->tokens, d->q_stride, p.group, p.tile_tokens,
                 &p.q_head_step) ||
       !make_map(&tk, d->kv_tokens > 0 ? d->k : d->q, bf16, d->dim, d->kv_tokens > 0 ? d->kv_heads : 1, keys,
-                d->kv_tokens > 0 ? d->k_stride : none, 1, BK, &p.k_head_step) ||
+                d->kv_tokens > 0 ? d->k_stride : none, 1, block, &p.k_head_step) ||
       !make_map(&tv, d->kv_tokens > 0 ? d->v : d->q, bf16, d->dim, d->kv_tokens > 0 ? d->kv_heads : 1, keys,
-                d->kv_tokens > 0 ? d->v_stride : none, 1, BK, &p.v_head_step))
+                d->kv_tokens > 0 ? d->v_stride : none, 1, block, &p.v_head_step))
     return ktir_set_error(KTIR_ERR_UNSUPPORTED, "ktir_prompt_attention: strides that a tensor map does not take");
   const int sms = sm_count();
   if (sms < 1) return ktir_set_error(KTIR_ERR_CUDA, "ktir_prompt_attention: no usable current device");

@@ -47,6 +47,28 @@ __device__ __forceinline__ float ex2(float x) {
   return y;
 }
 
+// Programmatic dependent launch: the kernels are launched while the one before
+// them on the stream still runs, and touch no memory before it has completed
+// (pdl_wait); pdl_launch lets the next one come as early.
+__device__ __forceinline__ void pdl_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+__device__ __forceinline__ void pdl_launch() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+
+template <typename... Params, typename... Args>
+inline cudaError_t launch_pdl(void (*kernel)(Params...), unsigned grid, unsigned threads, size_t smem,
+                              cudaStream_t stream, const Args&... args) {
+  cudaLaunchConfig_t c = {};
+  c.gridDim = dim3(grid);
+  c.blockDim = dim3(threads);
+  c.dynamicSmemBytes = smem;
+  c.stream = stream;
+  cudaLaunchAttribute a[1];
+  a[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  a[0].val.programmaticStreamSerializationAllowed = 1;
+  c.attrs = a;
+  c.numAttrs = 1;
+  return cudaLaunchKernelEx(&c, kernel, args...);
+}
+
 // -- host-side checks ---------------------------------------------------------
 inline bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
 
@@ -74,8 +96,10 @@ inline int sm_count() {   // of the current device, 0 if there is none
   return count[dev];
 }
 
-inline int launched(const char* what) {
-  return cudaGetLastError() == cudaSuccess ? KTIR_OK : ktir_set_error(KTIR_ERR_CUDA, what);
+inline int launched(cudaError_t e, const char* what) {
+  if (e == cudaSuccess) return KTIR_OK;
+  cudaGetLastError();      // the error is this call's, not the next one's
+  return ktir_set_error(KTIR_ERR_CUDA, what);
 }
 
 }  // namespace serve
