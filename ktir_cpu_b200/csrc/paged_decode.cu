@@ -39,6 +39,7 @@ constexpr int ROWS = 16;                   // query heads per head tile
 constexpr int CTAS_PER_SM = 2;
 constexpr int MAX_CTAS = 512;              // of a launch that splits sequences
 constexpr int MIN_TILES = 2;               // per stretch: both in flight at once
+constexpr int LOOK = 3;                    // tiles between a look into the page table and the copy
 constexpr float RESCALE_THRESHOLD = 8.0f;  // log2 units
 constexpr int PART_STRIDE = ROWS * (128 + 2);   // floats of a part: o, then (m, l) per row
 constexpr int64_t PARTS_BYTES = (int64_t)MAX_CTAS * 2 * PART_STRIDE * 4;
@@ -217,30 +218,52 @@ __global__ void __launch_bounds__(THREADS, CTAS_PER_SM)
   const uint32_t ring = (uint32_t)__cvta_generic_to_shared(smem) + warp * (C::STAGES * C::STAGE);
   float* join = reinterpret_cast<float*>(smem + C::RING);
 
-  // -- copies: lane l < 16 looks up key l of the warp's 16 one tile ahead ------
-  int page = -1, place = 0;
-  auto look = [&]() {                         // page and place for cursor `get`
+  // -- copies: lane l < 16 looks up key l of the warp's 16, LOOK tiles ahead (a look
+  // into the page table takes about as long as a tile) --------------------------
+  int page[LOOK], place[LOOK];
+  auto look = [&](int i) {                    // page and place for cursor `get`
     const int key = get.t * TILE + warp * KPW + (lane & 15);
-    page = -1;
+    page[i] = -1;
     if (key < get.len) {
       const int pi = p.page_shift >= 0 ? key >> p.page_shift : key / (int)d.page_size;
-      place = key - pi * (int)d.page_size;
-      page = d.pages[get.b * d.page_row + pi];
-      if (page < 0 || page >= d.num_pages) {
-        atomicOr(d.status, KTIR_STATUS_BAD_INDEX);
-        page = -1;
-      }
+      place[i] = key - pi * (int)d.page_size;
+      page[i] = d.pages[get.b * d.page_row + pi];
+      if (page[i] < 0) page[i] = -2;          // a bad page; -1 is no key
     }
   };
-  int got = 0;                                // tiles issued
+  int looked = 1, got = 0;                    // tiles looked up, tiles issued
+  look(0);
+#pragma unroll
+  for (int i = 1; i < LOOK; ++i) {
+    page[i] = -1;
+    if (looked < n) {
+      step(get);
+      look(i);
+      ++looked;
+    }
+  }
   auto issue = [&]() {
     if (got < n) {
       const uint32_t st = ring + (got % C::STAGES) * C::STAGE;
-      const long long ko = page < 0 ? -1 : page * d.kc_stride[0] + place * d.kc_stride[1] + kvh * d.kc_stride[2];
-      const long long vo = page < 0 ? -1 : page * d.vc_stride[0] + place * d.vc_stride[1] + kvh * d.vc_stride[2];
-      if (++got < n) {                        // the next tile's pages are on their way meanwhile
+      const int pg = page[0];
+      long long ko = -1, vo = -1;
+      if (pg >= 0 && pg < d.num_pages) {
+        ko = pg * d.kc_stride[0] + place[0] * d.kc_stride[1] + kvh * d.kc_stride[2];
+        vo = pg * d.vc_stride[0] + place[0] * d.vc_stride[1] + kvh * d.vc_stride[2];
+      } else if (pg != -1) {
+        atomicOr(d.status, KTIR_STATUS_BAD_INDEX);
+      }
+      ++got;
+#pragma unroll
+      for (int i = 0; i + 1 < LOOK; ++i) {
+        page[i] = page[i + 1];
+        place[i] = place[i + 1];
+      }
+      page[LOOK - 1] = -1;
+      if (looked < n) {
         step(get);
-        look();
+        look(LOOK - 1);
+        ++looked;
       }
       const int c = lane % C::CHUNKS;
       constexpr int PER = 32 / C::CHUNKS;     // rows per instruction
@@ -255,7 +278,6 @@ __global__ void __launch_bounds__(THREADS, CTAS_PER_SM)
     }
     cp_commit();
   };
-  look();
 #pragma unroll
   for (int s = 0; s < C::STAGES - 1; ++s) issue();
 
@@ -383,17 +405,20 @@ __global__ void __launch_bounds__(THREADS, CTAS_PER_SM)
       for (int k = 0; k < D / 8; ++k)
 #pragma unroll
         for (int r = 0; r < 2; ++r)
-          *reinterpret_cast<float2*>(to + (row + 8 * r) * D + k * 8 + col) = make_float2(o[k][2 * r], o[k][2 * r + 1]);
+          if (row + 8 * r < nrows)
+            *reinterpret_cast<float2*>(to + (row + 8 * r) * D + k * 8 + col) =
+                make_float2(o[k][2 * r], o[k][2 * r + 1]);
     };
     auto add = [&](const float* from) {
 #pragma unroll
       for (int k = 0; k < D / 8; ++k)
 #pragma unroll
-        for (int r = 0; r < 2; ++r) {
-          const float2 x = *reinterpret_cast<const float2*>(from + (row + 8 * r) * D + k * 8 + col);
-          o[k][2 * r] += x.x;
-          o[k][2 * r + 1] += x.y;
-        }
+        for (int r = 0; r < 2; ++r)
+          if (row + 8 * r < nrows) {
+            const float2 x = *reinterpret_cast<const float2*>(from + (row + 8 * r) * D + k * 8 + col);
+            o[k][2 * r] += x.x;
+            o[k][2 * r + 1] += x.y;
+          }
     };
     if (warp >= 2) put(join + (warp - 2) * ROWS * D);
     __syncthreads();
@@ -446,21 +471,42 @@ __global__ void __launch_bounds__(THREADS, CTAS_PER_SM)
           const int r = e / (D / 4), c = (e - r * (D / 4)) * 4;
           float mm = -INFINITY, ll = 0.f;
           float4 oo = make_float4(0.f, 0.f, 0.f, 0.f);
-          for (long long g = g0; g <= g1; ++g) {
-            // the first part ends its stretch, the others begin theirs
-            const bool begins = base >= total * g / ng;
-            const float* part = p.parts + ((g * p.ht + ht) * 2 + (begins ? 1 : 0)) * PART_STRIDE;
-            const float2 ml = __ldcg(reinterpret_cast<const float2*>(part + ROWS * D) + r);
-            const float4 x = __ldcg(reinterpret_cast<const float4*>(part + r * D + c));
-            const float mn = fmaxf(mm, ml.x);
+          // eight parts on their way at once
+          for (long long g = g0; g <= g1; g += 8) {
+            float2 ml[8];
+            float4 x[8];
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+              ml[i] = make_float2(-INFINITY, 0.f);
+              x[i] = make_float4(0.f, 0.f, 0.f, 0.f);
+              if (g + i <= g1) {
+                // the first part ends its stretch, the others begin theirs
+                const bool begins = g + i == g0;
+                const float* part = p.parts + (((g + i) * p.ht + ht) * 2 + (begins ? 1 : 0)) * PART_STRIDE;
+                ml[i] = __ldcg(reinterpret_cast<const float2*>(part + ROWS * D) + r);
+                x[i] = __ldcg(reinterpret_cast<const float4*>(part + r * D + c));
+              }
+            }
+            float mn = mm;
+#pragma unroll
+            for (int i = 0; i < 8; ++i) mn = fmaxf(mn, ml[i].x);
             const float sub = mn == -INFINITY ? 0.f : mn;
-            const float f = ex2(mm - sub), w = ex2(ml.x - sub);
+            const float f = ex2(mm - sub);
             mm = mn;
-            ll = ll * f + ml.y * w;
-            oo.x = oo.x * f + x.x * w;
-            oo.y = oo.y * f + x.y * w;
-            oo.z = oo.z * f + x.z * w;
-            oo.w = oo.w * f + x.w * w;
+            ll *= f;
+            oo.x *= f;
+            oo.y *= f;
+            oo.z *= f;
+            oo.w *= f;
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+              const float w = ex2(ml[i].x - sub);
+              ll += ml[i].y * w;
+              oo.x += x[i].x * w;
+              oo.y += x[i].y * w;
+              oo.z += x[i].z * w;
+              oo.w += x[i].w * w;
+            }
           }
           const float inv = ll == 0.f ? 0.f : 1.f / ll;
           uint2 v;
