@@ -286,24 +286,28 @@ __global__ void __launch_bounds__(THREADS, CTAS_PER_SM)
   const float sl = d.scale * LOG2E;
   const int row = lane >> 2, col = (lane & 3) * 2;
 
+  auto begin = [&](long long b) {             // a sequence, or this stretch of it: its queries, nothing summed
+    const T* q = static_cast<const T*>(d.q) + b * d.q_stride[0];
+#pragma unroll
+    for (int k = 0; k < D / 16; ++k)
+#pragma unroll
+      for (int x = 0; x < 4; ++x) {
+        const int r = row + (x & 1) * 8;
+        qa[k][x] = r < nrows ? *reinterpret_cast<const uint32_t*>(q + (head0 + r) * d.q_stride[1] + k * 16 +
+                                                                   (x >> 1) * 8 + col)
+                             : 0u;
+      }
+  };
+  auto clear = [&]() {
+#pragma unroll
+    for (int k = 0; k < D / 8; ++k) o[k][0] = o[k][1] = o[k][2] = o[k][3] = 0.f;
+    m[0] = m[1] = -INFINITY;
+    l[0] = l[1] = 0.f;
+  };
+  begin(use.b);
+  clear();
+
   for (int i = 0; i < n; ++i) {
-    if (i == 0 || use.t == 0) {
-      // a sequence begins (or this stretch of it): its queries, and nothing summed yet
-      const T* q = static_cast<const T*>(d.q) + use.b * d.q_stride[0];
-#pragma unroll
-      for (int k = 0; k < D / 16; ++k)
-#pragma unroll
-        for (int x = 0; x < 4; ++x) {
-          const int r = row + (x & 1) * 8;
-          qa[k][x] = r < nrows ? *reinterpret_cast<const uint32_t*>(q + (head0 + r) * d.q_stride[1] + k * 16 +
-                                                                     (x >> 1) * 8 + col)
-                               : 0u;
-        }
-#pragma unroll
-      for (int k = 0; k < D / 8; ++k) o[k][0] = o[k][1] = o[k][2] = o[k][3] = 0.f;
-      m[0] = m[1] = -INFINITY;
-      l[0] = l[1] = 0.f;
-    }
     cp_wait<C::STAGES - 2>();
     __syncwarp();                             // every lane's copies of tile i, and its reads of tile i - 1
     issue();
@@ -373,6 +377,13 @@ __global__ void __launch_bounds__(THREADS, CTAS_PER_SM)
       continue;
     }
     // -- the sequence, or this stretch of it, ends: join the warps ---------------
+    const long long b = use.b, end = base + use.nt;
+    const bool whole = base >= t_begin && end <= t_end;
+    const bool more = i + 1 < n;
+    if (more) {                               // the next one's queries are on their way meanwhile
+      open(use, b + 1);
+      begin(use.b);
+    }
 #pragma unroll
     for (int r = 0; r < 2; ++r) {
       l[r] += __shfl_xor_sync(0xffffffffu, l[r], 1);
@@ -382,84 +393,60 @@ __global__ void __launch_bounds__(THREADS, CTAS_PER_SM)
       s_ml[warp][row] = make_float2(m[0], l[0]);
       s_ml[warp][row + 8] = make_float2(m[1], l[1]);
     }
-    __syncthreads();
-    float mt[2], lt[2];
+    T* out = static_cast<T*>(d.out) + b * d.out_stride[0];
+    float* part = p.parts + ((long long)blockIdx.x * 2 + (base >= t_begin ? 1 : 0)) * PART_STRIDE;
+    // eight rows at a time: [warp][row][D] in shared memory, eight floats of a row
+    // moved by its number (a column of rows would lie in one bank), then each
+    // thread four outputs
 #pragma unroll
-    for (int r = 0; r < 2; ++r) {
-      mt[r] = -INFINITY;
+    for (int h = 0; h < 2; ++h) {
+      if (8 * h < nrows) {
+        if (8 * h + row < nrows)
 #pragma unroll
-      for (int w = 0; w < WARPS; ++w) mt[r] = fmaxf(mt[r], s_ml[w][row + 8 * r].x);
-      const float sub = mt[r] == -INFINITY ? 0.f : mt[r];
-      lt[r] = 0.f;
+          for (int k = 0; k < D / 8; ++k)
+            *reinterpret_cast<float2*>(join + (warp * 8 + row) * D + ((k * 8) ^ ((row & 3) * 8)) + col) =
+                make_float2(o[k][2 * h], o[k][2 * h + 1]);
+        __syncthreads();
+        for (int e = tid; e < min(8, nrows - 8 * h) * (D / 4); e += THREADS) {
+          const int r = e / (D / 4), c = (e - r * (D / 4)) * 4;
+          float mt = -INFINITY, lt = 0.f;
 #pragma unroll
-      for (int w = 0; w < WARPS; ++w) lt[r] += s_ml[w][row + 8 * r].y * ex2(s_ml[w][row + 8 * r].x - sub);
-      const float f = ex2(m[r] - sub);
+          for (int w = 0; w < WARPS; ++w) mt = fmaxf(mt, s_ml[w][8 * h + r].x);
+          const float sub = mt == -INFINITY ? 0.f : mt;
+          float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
-      for (int k = 0; k < D / 8; ++k) {
-        o[k][2 * r] *= f;
-        o[k][2 * r + 1] *= f;
-      }
-    }
-    auto put = [&](float* to) {
-#pragma unroll
-      for (int k = 0; k < D / 8; ++k)
-#pragma unroll
-        for (int r = 0; r < 2; ++r)
-          if (row + 8 * r < nrows)
-            *reinterpret_cast<float2*>(to + (row + 8 * r) * D + k * 8 + col) =
-                make_float2(o[k][2 * r], o[k][2 * r + 1]);
-    };
-    auto add = [&](const float* from) {
-#pragma unroll
-      for (int k = 0; k < D / 8; ++k)
-#pragma unroll
-        for (int r = 0; r < 2; ++r)
-          if (row + 8 * r < nrows) {
-            const float2 x = *reinterpret_cast<const float2*>(from + (row + 8 * r) * D + k * 8 + col);
-            o[k][2 * r] += x.x;
-            o[k][2 * r + 1] += x.y;
+          for (int w = 0; w < WARPS; ++w) {
+            const float2 ml = s_ml[w][8 * h + r];
+            const float f = ex2(ml.x - sub);
+            const float4 y = *reinterpret_cast<const float4*>(join + (w * 8 + r) * D + (c ^ ((r & 3) * 8)));
+            lt += ml.y * f;
+            x.x += y.x * f;
+            x.y += y.y * f;
+            x.z += y.z * f;
+            x.w += y.w * f;
           }
-    };
-    if (warp >= 2) put(join + (warp - 2) * ROWS * D);
-    __syncthreads();
-    if (warp < 2) add(join + warp * ROWS * D);
-    if (warp == 1) put(join + ROWS * D);
-    __syncthreads();
-    const long long end = base + use.nt;
-    const bool whole = base >= t_begin && end <= t_end;
-    if (warp == 0) {
-      add(join + ROWS * D);
-      if (whole) {
-        T* out = static_cast<T*>(d.out) + use.b * d.out_stride[0];
-#pragma unroll
-        for (int r = 0; r < 2; ++r) {
-          if (row + 8 * r < nrows) {
-            const float inv = lt[r] == 0.f ? 0.f : 1.f / lt[r];   // every score -inf: nothing to weigh
-#pragma unroll
-            for (int k = 0; k < D / 8; ++k)
-              *reinterpret_cast<uint32_t*>(out + (head0 + row + 8 * r) * d.out_stride[1] + k * 8 + col) =
-                  Elem<T>::from2(o[k][2 * r] * inv, o[k][2 * r + 1] * inv);
-            if (d.lse && (lane & 3) == 0)
-              d.lse[use.b * d.heads + head0 + row + 8 * r] = (mt[r] + log2f(lt[r])) * LN2;
+          if (whole) {
+            const float inv = lt == 0.f ? 0.f : 1.f / lt;     // every score -inf: nothing to weigh
+            uint2 v;
+            v.x = Elem<T>::from2(x.x * inv, x.y * inv);
+            v.y = Elem<T>::from2(x.z * inv, x.w * inv);
+            *reinterpret_cast<uint2*>(out + (head0 + 8 * h + r) * d.out_stride[1] + c) = v;
+            if (d.lse && c == 0) d.lse[b * d.heads + head0 + 8 * h + r] = (mt + log2f(lt)) * LN2;
+          } else {
+            *reinterpret_cast<float4*>(part + (8 * h + r) * D + c) = x;
+            if (c == 0) reinterpret_cast<float2*>(part + ROWS * D)[8 * h + r] = make_float2(mt, lt);
           }
         }
-      } else {
-        float* part = p.parts + ((long long)blockIdx.x * 2 + (base >= t_begin ? 1 : 0)) * PART_STRIDE;
-        put(part);
-        if ((lane & 3) == 0) {
-          float2* ml = reinterpret_cast<float2*>(part + ROWS * D);
-          ml[row] = make_float2(mt[0], lt[0]);
-          ml[row + 8] = make_float2(mt[1], lt[1]);
-        }
-        __threadfence();
+        if (!whole) __threadfence();
+        __syncthreads();
       }
     }
+    clear();
     if (!whole) {
       // stretches that share the sequence: those of its first to its last tile
       const long long g0 = ((base + 1) * ng - 1) / total, g1 = (end * ng - 1) / total;
-      __syncthreads();
       if (tid == 0) {
-        int* counter = p.counters + use.b * p.ht + ht;
+        int* counter = p.counters + b * p.ht + ht;
         const int before = atomicAdd(counter, 1);
         s_last = before == (int)(g1 - g0);
         if (s_last) *counter = 0;
@@ -512,14 +499,13 @@ __global__ void __launch_bounds__(THREADS, CTAS_PER_SM)
           uint2 v;
           v.x = Elem<T>::from2(oo.x * inv, oo.y * inv);
           v.y = Elem<T>::from2(oo.z * inv, oo.w * inv);
-          *reinterpret_cast<uint2*>(static_cast<T*>(d.out) + use.b * d.out_stride[0] +
+          *reinterpret_cast<uint2*>(static_cast<T*>(d.out) + b * d.out_stride[0] +
                                     (head0 + r) * d.out_stride[1] + c) = v;
-          if (d.lse && c == 0) d.lse[use.b * d.heads + head0 + r] = (mm + log2f(ll)) * LN2;
+          if (d.lse && c == 0) d.lse[b * d.heads + head0 + r] = (mm + log2f(ll)) * LN2;
         }
       }
     }
     base = end;
-    if (i + 1 < n) open(use, use.b + 1);
   }
 }
 
