@@ -6,9 +6,10 @@
 // Bound by memory: every cached key and value is read once and meets the g =
 // heads / kv_heads queries that share it, 2 g operations per byte.  So the
 // cache streams through shared memory in 16-byte asynchronous copies, and the
-// two products run on mma.sync (m16n8k16, up to 16 query heads as its rows; a
-// larger g takes several head tiles), which tcgen05's 64 or 128 rows would
-// leave mostly empty.
+// two products run on mma.sync (m16n8k16) with 16 keys, or 16 elements of the
+// values, as its rows and 8 query heads as its columns: x^T = K q^T, then o^T +=
+// V^T p^T (tcgen05's 64 or 128 rows would be mostly empty).  A head tile has 8
+// heads, or 16 where g is above 8; a larger g takes several.
 //
 // Split over the cache: the 64-key tiles of all sequences form one list, cut
 // into equal stretches, one per group of CTAs; the CTAs of a group take the
@@ -35,7 +36,7 @@ constexpr int WARPS = 4;
 constexpr int THREADS = WARPS * 32;
 constexpr int KPW = 16;                    // keys per warp and tile
 constexpr int TILE = WARPS * KPW;          // keys per tile
-constexpr int ROWS = 16;                   // query heads per head tile
+constexpr int ROWS = 16;                   // query heads per head tile at most
 constexpr int CTAS_PER_SM = 2;
 constexpr int MAX_CTAS = 512;              // of a launch that splits sequences
 constexpr int MIN_TILES = 2;               // per stretch: both in flight at once
@@ -51,6 +52,7 @@ struct DecodeParams {
   int ht;             // kv_heads * htiles
   int groups;         // CTA groups of the launch
   int page_shift;     // log2(page_size), or -1
+  int same;           // K and V have the same strides
   float* parts;
   int* counters;      // [batch][ht], zero between calls
 };
@@ -93,6 +95,12 @@ __device__ __forceinline__ void cp16(uint32_t dst, const void* src, int bytes) {
   asm volatile("cp.async.cg.shared.global.L2::128B [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes)
                : "memory");
 }
+// an 8 x 8 tile of 16-bit values transposed across the warp
+__device__ __forceinline__ uint32_t transpose8(uint32_t v) {
+  uint32_t r;
+  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(v));
+  return r;
+}
 __device__ __forceinline__ void cp_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 template <int N>
 __device__ __forceinline__ void cp_wait() {
@@ -105,7 +113,7 @@ struct Cursor {
   int t, nt, len;
 };
 
-template <typename T, int D>
+template <int D>
 struct Cfg {
   static constexpr int CHUNKS = D / 8;                 // 16-byte pieces of a row
   static constexpr int ROW_BYTES = D * 2;
@@ -113,14 +121,14 @@ struct Cfg {
   static constexpr int STAGE = 2 * HALF_STAGE;
   static constexpr int STAGES = D == 128 ? 3 : 6;      // 24 KiB in flight per warp
   static constexpr int RING = WARPS * STAGES * STAGE;
-  static constexpr int JOIN = 2 * ROWS * D * 4;        // two warps' outputs
+  static constexpr int JOIN = WARPS * 8 * D * 4;       // eight heads' outputs of each warp
   static constexpr int SMEM = RING + JOIN;
 };
 
-template <typename T, int D>
+template <typename T, int D, int NT>       // NT: tiles of 8 heads
 __global__ void __launch_bounds__(THREADS, CTAS_PER_SM)
     k_paged_decode(const __grid_constant__ DecodeParams p) {
-  using C = Cfg<T, D>;
+  using C = Cfg<D>;
   const KtirPagedDecodeDesc& d = p.d;
   extern __shared__ __align__(128) uint8_t smem[];
   __shared__ long long s_scan[WARPS];
@@ -129,8 +137,8 @@ __global__ void __launch_bounds__(THREADS, CTAS_PER_SM)
   __shared__ int s_last;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int grp = blockIdx.x / p.ht, ht = blockIdx.x - grp * p.ht;
-  const int kvh = ht / p.htiles, head0 = kvh * p.group + (ht - kvh * p.htiles) * ROWS;
-  const int nrows = min(ROWS, (kvh + 1) * p.group - head0);
+  const int kvh = ht / p.htiles, head0 = kvh * p.group + (ht - kvh * p.htiles) * (8 * NT);
+  const int nrows = min(8 * NT, (kvh + 1) * p.group - head0);
   const long long most = d.max_pages * d.page_size;
 
   // tiles of a sequence; a length outside its range counts as 0
@@ -270,7 +278,8 @@ __global__ void __launch_bounds__(THREADS, CTAS_PER_SM)
 #pragma unroll
       for (int i = 0; i < KPW / PER; ++i) {
         const int r = i * PER + lane / C::CHUNKS;
-        const long long k = __shfl_sync(0xffffffffu, ko, r), v = __shfl_sync(0xffffffffu, vo, r);
+        const long long k = __shfl_sync(0xffffffffu, ko, r);
+        const long long v = p.same ? k : __shfl_sync(0xffffffffu, vo, r);
         const uint32_t dst = st + r * C::ROW_BYTES + ((c ^ (r & 7)) << 4);
         cp16(dst, static_cast<const T*>(d.k_cache) + (k < 0 ? 0 : k + c * 8), k < 0 ? 0 : 16);
         cp16(dst + C::HALF_STAGE, static_cast<const T*>(d.v_cache) + (v < 0 ? 0 : v + c * 8), v < 0 ? 0 : 16);
@@ -281,28 +290,33 @@ __global__ void __launch_bounds__(THREADS, CTAS_PER_SM)
 #pragma unroll
   for (int s = 0; s < C::STAGES - 1; ++s) issue();
 
-  uint32_t qa[D / 16][4];
-  float o[D / 8][4], m[2], l[2];
+  // q^T as the first product's second operand; o^T, and per head m and l (l over
+  // this thread's keys): heads 2 (lane % 4) and the next of every tile of 8
+  uint32_t qb[D / 16][NT][2];
+  float o[D / 16][NT][4], m[NT][2], l[NT][2];
   const float sl = d.scale * LOG2E;
-  const int row = lane >> 2, col = (lane & 3) * 2;
+  const int at = lane >> 2, col = (lane & 3) * 2;
 
-  auto begin = [&](long long b) {             // a sequence, or this stretch of it: its queries, nothing summed
+  auto begin = [&](long long b) {             // a sequence, or this stretch of it
     const T* q = static_cast<const T*>(d.q) + b * d.q_stride[0];
 #pragma unroll
-    for (int k = 0; k < D / 16; ++k)
+    for (int h = 0; h < NT; ++h)
 #pragma unroll
-      for (int x = 0; x < 4; ++x) {
-        const int r = row + (x & 1) * 8;
-        qa[k][x] = r < nrows ? *reinterpret_cast<const uint32_t*>(q + (head0 + r) * d.q_stride[1] + k * 16 +
-                                                                   (x >> 1) * 8 + col)
-                             : 0u;
-      }
+      for (int k = 0; k < D / 16; ++k)
+#pragma unroll
+        for (int x = 0; x < 2; ++x)
+          qb[k][h][x] = 8 * h + at < nrows ? *reinterpret_cast<const uint32_t*>(
+                                                 q + (head0 + 8 * h + at) * d.q_stride[1] + k * 16 + x * 8 + col)
+                                           : 0u;
   };
   auto clear = [&]() {
 #pragma unroll
-    for (int k = 0; k < D / 8; ++k) o[k][0] = o[k][1] = o[k][2] = o[k][3] = 0.f;
-    m[0] = m[1] = -INFINITY;
-    l[0] = l[1] = 0.f;
+    for (int h = 0; h < NT; ++h) {
+#pragma unroll
+      for (int k = 0; k < D / 16; ++k) o[k][h][0] = o[k][h][1] = o[k][h][2] = o[k][h][3] = 0.f;
+      m[h][0] = m[h][1] = -INFINITY;
+      l[h][0] = l[h][1] = 0.f;
+    }
   };
   begin(use.b);
   clear();
@@ -313,63 +327,63 @@ __global__ void __launch_bounds__(THREADS, CTAS_PER_SM)
     issue();
     const uint32_t kt = ring + (i % C::STAGES) * C::STAGE, vt = kt + C::HALF_STAGE;
 
-    // x = q k^T for 16 keys: s[0] keys 0-7, s[1] keys 8-15
-    float s[2][4] = {};
+    // x^T = K q^T, in two chains
+    float s[NT][4] = {}, s2[NT][4] = {};
 #pragma unroll
     for (int k = 0; k < D / 16; ++k) {
-      uint32_t b[4];
-      const int r = (lane & 7) + ((lane >> 4) << 3), c = 2 * k + ((lane >> 3) & 1);
-      ldsm4(b, kt + r * C::ROW_BYTES + ((c ^ (r & 7)) << 4));
-      mma16816<T>(s[0], qa[k], b[0], b[1]);
-      mma16816<T>(s[1], qa[k], b[2], b[3]);
+      uint32_t a[4];
+      const int r = (lane & 7) + (((lane >> 3) & 1) << 3), c = 2 * k + (lane >> 4);
+      ldsm4(a, kt + r * C::ROW_BYTES + ((c ^ (r & 7)) << 4));
+#pragma unroll
+      for (int h = 0; h < NT; ++h) mma16816<T>(k & 1 ? s2[h] : s[h], a, qb[k][h][0], qb[k][h][1]);
     }
     const int left = use.len - use.t * TILE - warp * KPW;      // keys of the 16 that exist
+    uint32_t pb[NT][2];
 #pragma unroll
-    for (int h = 0; h < 2; ++h)
+    for (int h = 0; h < NT; ++h) {
+      float top[2];
 #pragma unroll
-      for (int x = 0; x < 4; ++x) {
-        s[h][x] = 8 * h + col + (x & 1) < left ? s[h][x] * sl : -INFINITY;
+      for (int x = 0; x < 4; ++x)
+        s[h][x] = at + 8 * (x >> 1) < left ? (s[h][x] + s2[h][x]) * sl : -INFINITY;
+#pragma unroll
+      for (int x = 0; x < 2; ++x) {
+        top[x] = fmaxf(s[h][x], s[h][x + 2]);
+        top[x] = fmaxf(top[x], __shfl_xor_sync(0xffffffffu, top[x], 4));
+        top[x] = fmaxf(top[x], __shfl_xor_sync(0xffffffffu, top[x], 8));
+        top[x] = fmaxf(top[x], __shfl_xor_sync(0xffffffffu, top[x], 16));
       }
-    float top[2];
+      if (__any_sync(0xffffffffu,
+                     top[0] > m[h][0] + RESCALE_THRESHOLD || top[1] > m[h][1] + RESCALE_THRESHOLD)) {
 #pragma unroll
-    for (int r = 0; r < 2; ++r) {
-      top[r] = fmaxf(fmaxf(s[0][2 * r], s[0][2 * r + 1]), fmaxf(s[1][2 * r], s[1][2 * r + 1]));
-      top[r] = fmaxf(top[r], __shfl_xor_sync(0xffffffffu, top[r], 1));
-      top[r] = fmaxf(top[r], __shfl_xor_sync(0xffffffffu, top[r], 2));
-    }
-    if (__any_sync(0xffffffffu, top[0] > m[0] + RESCALE_THRESHOLD || top[1] > m[1] + RESCALE_THRESHOLD)) {
+        for (int x = 0; x < 2; ++x) {
+          const float mn = fmaxf(m[h][x], top[x]);
+          const float f = mn == -INFINITY ? 1.f : ex2(m[h][x] - mn);
+          m[h][x] = mn;
+          l[h][x] *= f;
 #pragma unroll
-      for (int r = 0; r < 2; ++r) {
-        const float mn = fmaxf(m[r], top[r]);
-        const float f = mn == -INFINITY ? 1.f : ex2(m[r] - mn);
-        m[r] = mn;
-        l[r] *= f;
-#pragma unroll
-        for (int k = 0; k < D / 8; ++k) {
-          o[k][2 * r] *= f;
-          o[k][2 * r + 1] *= f;
+          for (int k = 0; k < D / 16; ++k) {
+            o[k][h][x] *= f;
+            o[k][h][x + 2] *= f;
+          }
         }
       }
-    }
-    uint32_t pa[4];
+      const float sub0 = m[h][0] == -INFINITY ? 0.f : m[h][0], sub1 = m[h][1] == -INFINITY ? 0.f : m[h][1];
 #pragma unroll
-    for (int r = 0; r < 2; ++r) {
-      const float sub = m[r] == -INFINITY ? 0.f : m[r];
-#pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        const float a = ex2(s[h][2 * r] - sub), b = ex2(s[h][2 * r + 1] - sub);
-        l[r] += a + b;
-        pa[2 * h + r] = Elem<T>::from2(a, b);
+      for (int x = 0; x < 2; ++x) {           // keys `at` and `at` + 8
+        const float a = ex2(s[h][2 * x] - sub0), b = ex2(s[h][2 * x + 1] - sub1);
+        l[h][0] += a;
+        l[h][1] += b;
+        pb[h][x] = transpose8(Elem<T>::from2(a, b));
       }
     }
-    // o += p v
+    // o^T += V^T p^T
 #pragma unroll
     for (int k = 0; k < D / 16; ++k) {
-      uint32_t b[4];
-      const int r = (lane & 7) + (((lane >> 3) & 1) << 3), c = 2 * k + (lane >> 4);
-      ldsm4t(b, vt + r * C::ROW_BYTES + ((c ^ (r & 7)) << 4));
-      mma16816<T>(o[2 * k], pa, b[0], b[1]);
-      mma16816<T>(o[2 * k + 1], pa, b[2], b[3]);
+      uint32_t a[4];
+      const int r = (lane & 7) + ((lane >> 4) << 3), c = 2 * k + ((lane >> 3) & 1);
+      ldsm4t(a, vt + r * C::ROW_BYTES + ((c ^ (r & 7)) << 4));
+#pragma unroll
+      for (int h = 0; h < NT; ++h) mma16816<T>(o[k][h], a, pb[h][0], pb[h][1]);
     }
 
     if (use.t + 1 < use.nt && i + 1 < n) {
@@ -385,27 +399,27 @@ __global__ void __launch_bounds__(THREADS, CTAS_PER_SM)
       begin(use.b);
     }
 #pragma unroll
-    for (int r = 0; r < 2; ++r) {
-      l[r] += __shfl_xor_sync(0xffffffffu, l[r], 1);
-      l[r] += __shfl_xor_sync(0xffffffffu, l[r], 2);
-    }
-    if ((lane & 3) == 0) {
-      s_ml[warp][row] = make_float2(m[0], l[0]);
-      s_ml[warp][row + 8] = make_float2(m[1], l[1]);
-    }
+    for (int h = 0; h < NT; ++h)
+#pragma unroll
+      for (int x = 0; x < 2; ++x) {
+#pragma unroll
+        for (int w = 4; w < 32; w <<= 1) l[h][x] += __shfl_xor_sync(0xffffffffu, l[h][x], w);
+        if (lane < 4) s_ml[warp][8 * h + col + x] = make_float2(m[h][x], l[h][x]);
+      }
     T* out = static_cast<T*>(d.out) + b * d.out_stride[0];
     float* part = p.parts + ((long long)blockIdx.x * 2 + (base >= t_begin ? 1 : 0)) * PART_STRIDE;
-    // eight rows at a time: [warp][row][D] in shared memory, eight floats of a row
-    // moved by its number (a column of rows would lie in one bank), then each
-    // thread four outputs
+    // eight heads at a time: [warp][head][D] in shared memory, eight floats of a
+    // head moved by its number (the heads would lie in one bank), then each thread
+    // four outputs
 #pragma unroll
-    for (int h = 0; h < 2; ++h) {
+    for (int h = 0; h < NT; ++h) {
       if (8 * h < nrows) {
-        if (8 * h + row < nrows)
+        float* to = join + (warp * 8 + col) * D;
+        const int move = (lane & 3) * 8;       // of heads `col` and `col` + 1
 #pragma unroll
-          for (int k = 0; k < D / 8; ++k)
-            *reinterpret_cast<float2*>(join + (warp * 8 + row) * D + ((k * 8) ^ ((row & 3) * 8)) + col) =
-                make_float2(o[k][2 * h], o[k][2 * h + 1]);
+        for (int k = 0; k < D / 16; ++k)
+#pragma unroll
+          for (int x = 0; x < 4; ++x) to[(x & 1) * D + ((16 * k + 8 * (x >> 1)) ^ move) + at] = o[k][h][x];
         __syncthreads();
         for (int e = tid; e < min(8, nrows - 8 * h) * (D / 4); e += THREADS) {
           const int r = e / (D / 4), c = (e - r * (D / 4)) * 4;
@@ -418,7 +432,7 @@ __global__ void __launch_bounds__(THREADS, CTAS_PER_SM)
           for (int w = 0; w < WARPS; ++w) {
             const float2 ml = s_ml[w][8 * h + r];
             const float f = ex2(ml.x - sub);
-            const float4 y = *reinterpret_cast<const float4*>(join + (w * 8 + r) * D + (c ^ ((r & 3) * 8)));
+            const float4 y = *reinterpret_cast<const float4*>(join + (w * 8 + r) * D + (c ^ ((r >> 1) * 8)));
             lt += ml.y * f;
             x.x += y.x * f;
             x.y += y.y * f;
@@ -458,12 +472,12 @@ __global__ void __launch_bounds__(THREADS, CTAS_PER_SM)
           const int r = e / (D / 4), c = (e - r * (D / 4)) * 4;
           float mm = -INFINITY, ll = 0.f;
           float4 oo = make_float4(0.f, 0.f, 0.f, 0.f);
-          // eight parts on their way at once
-          for (long long g = g0; g <= g1; g += 8) {
-            float2 ml[8];
-            float4 x[8];
+          // sixteen parts on their way at once
+          for (long long g = g0; g <= g1; g += 16) {
+            float2 ml[16];
+            float4 x[16];
 #pragma unroll
-            for (int i = 0; i < 8; ++i) {
+            for (int i = 0; i < 16; ++i) {
               ml[i] = make_float2(-INFINITY, 0.f);
               x[i] = make_float4(0.f, 0.f, 0.f, 0.f);
               if (g + i <= g1) {
@@ -476,7 +490,7 @@ __global__ void __launch_bounds__(THREADS, CTAS_PER_SM)
             }
             float mn = mm;
 #pragma unroll
-            for (int i = 0; i < 8; ++i) mn = fmaxf(mn, ml[i].x);
+            for (int i = 0; i < 16; ++i) mn = fmaxf(mn, ml[i].x);
             const float sub = mn == -INFINITY ? 0.f : mn;
             const float f = ex2(mm - sub);
             mm = mn;
@@ -486,7 +500,7 @@ __global__ void __launch_bounds__(THREADS, CTAS_PER_SM)
             oo.z *= f;
             oo.w *= f;
 #pragma unroll
-            for (int i = 0; i < 8; ++i) {
+            for (int i = 0; i < 16; ++i) {
               const float w = ex2(ml[i].x - sub);
               ll += ml[i].y * w;
               oo.x += x[i].x * w;
@@ -509,28 +523,31 @@ __global__ void __launch_bounds__(THREADS, CTAS_PER_SM)
   }
 }
 
-template <typename T, int D>
+template <typename T, int D, int NT>
 int launch(const DecodeParams& p, unsigned grid, cudaStream_t stream) {
   // the attribute is per device
   static bool ready[MAX_DEVICES] = {};
   const int dev = current_device();
   if (dev < 0) return ktir_set_error(KTIR_ERR_CUDA, "ktir_paged_decode: no usable current device");
   if (!ready[dev]) {
-    if (cudaFuncSetAttribute(k_paged_decode<T, D>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                             Cfg<T, D>::SMEM) != cudaSuccess)
+    if (cudaFuncSetAttribute(k_paged_decode<T, D, NT>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                             Cfg<D>::SMEM) != cudaSuccess)
       return ktir_set_error(KTIR_ERR_CUDA, "ktir_paged_decode: shared-memory attribute refused");
     ready[dev] = true;
   }
-  return launched(launch_pdl(k_paged_decode<T, D>, grid, THREADS, Cfg<T, D>::SMEM, stream, p),
+  return launched(launch_pdl(k_paged_decode<T, D, NT>, grid, THREADS, Cfg<D>::SMEM, stream, p),
                   "ktir_paged_decode: launch failed");
 }
+
+// head tiles of a kv head: 8 query heads each, 16 where there are more than 8
+int head_tiles(int group) { return group <= 8 ? 1 : (group + 15) / 16; }
 
 }  // namespace
 
 extern "C" int64_t ktir_paged_decode_workspace(int64_t batch, int32_t heads, int32_t kv_heads,
                                                int32_t dim) {
   if (batch < 1 || heads < 1 || kv_heads < 1 || dim < 1) return 0;
-  const int64_t htiles = (heads / kv_heads + ROWS - 1) / ROWS;
+  const int64_t htiles = head_tiles(heads / kv_heads);
   // the parts first, at a size of their own: the counters keep their places
   // (and their zeros) between calls of different batches
   return PARTS_BYTES + batch * kv_heads * htiles * 4;
@@ -567,7 +584,9 @@ extern "C" int ktir_paged_decode(const KtirPagedDecodeDesc* d, void* stream) {
   DecodeParams p;
   p.d = *d;
   p.group = d->heads / d->kv_heads;
-  p.htiles = (p.group + ROWS - 1) / ROWS;
+  p.htiles = head_tiles(p.group);
+  p.same = 1;
+  for (int i = 0; i < 3; ++i) p.same &= d->kc_stride[i] == d->vc_stride[i];
   p.ht = d->kv_heads * p.htiles;
   p.parts = static_cast<float*>(d->workspace);
   p.counters = reinterpret_cast<int*>(static_cast<char*>(d->workspace) + PARTS_BYTES);
@@ -585,6 +604,10 @@ extern "C" int ktir_paged_decode(const KtirPagedDecodeDesc* d, void* stream) {
   const unsigned grid = (unsigned)(groups * p.ht);
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   const bool f16 = d->dtype == KTIR_F16;
-  if (d->dim == 64) return f16 ? launch<__half, 64>(p, grid, s) : launch<__nv_bfloat16, 64>(p, grid, s);
-  return f16 ? launch<__half, 128>(p, grid, s) : launch<__nv_bfloat16, 128>(p, grid, s);
+  if (p.group <= 8) {
+    if (d->dim == 64) return f16 ? launch<__half, 64, 1>(p, grid, s) : launch<__nv_bfloat16, 64, 1>(p, grid, s);
+    return f16 ? launch<__half, 128, 1>(p, grid, s) : launch<__nv_bfloat16, 128, 1>(p, grid, s);
+  }
+  if (d->dim == 64) return f16 ? launch<__half, 64, 2>(p, grid, s) : launch<__nv_bfloat16, 64, 2>(p, grid, s);
+  return f16 ? launch<__half, 128, 2>(p, grid, s) : launch<__nv_bfloat16, 128, 2>(p, grid, s);
 }
