@@ -37,7 +37,6 @@ constexpr int THREADS = WARPS * 32;
 constexpr int KPW = 16;                    // keys per warp and tile
 constexpr int TILE = WARPS * KPW;          // keys per tile
 constexpr int ROWS = 16;                   // query heads per head tile at most
-constexpr int CTAS_PER_SM = 2;
 constexpr int MAX_CTAS = 512;              // of a launch that splits sequences
 constexpr int MIN_TILES = 2;               // per stretch: both in flight at once
 constexpr int LOOK = 3;                    // tiles between a look into the page table and the copy
@@ -119,14 +118,19 @@ struct Cfg {
   static constexpr int ROW_BYTES = D * 2;
   static constexpr int HALF_STAGE = KPW * ROW_BYTES;   // K, then V
   static constexpr int STAGE = 2 * HALF_STAGE;
-  static constexpr int STAGES = D == 128 ? 3 : 6;      // 24 KiB in flight per warp
+  // what hides a tile's latency: copies in flight at dim 128 (24 KiB per warp), more
+  // warps at dim 64, whose tiles are half as long (45 sequences of 20 heads: 26 us
+  // against 32 with two CTAs of six stages; at dim 128 three CTAs leave two stages,
+  // 34 us against 32 for 32 sequences)
+  static constexpr int CTAS_PER_SM = D == 128 ? 2 : 3;
+  static constexpr int STAGES = 3;
   static constexpr int RING = WARPS * STAGES * STAGE;
   static constexpr int JOIN = WARPS * 8 * D * 4;       // eight heads' outputs of each warp
   static constexpr int SMEM = RING + JOIN;
 };
 
 template <typename T, int D, int NT>       // NT: tiles of 8 heads
-__global__ void __launch_bounds__(THREADS, CTAS_PER_SM)
+__global__ void __launch_bounds__(THREADS, Cfg<D>::CTAS_PER_SM)
     k_paged_decode(const __grid_constant__ DecodeParams p) {
   using C = Cfg<D>;
   const KtirPagedDecodeDesc& d = p.d;
@@ -594,7 +598,7 @@ extern "C" int ktir_paged_decode(const KtirPagedDecodeDesc* d, void* stream) {
   if ((d->page_size & (d->page_size - 1)) == 0)
     for (p.page_shift = 0; (1LL << p.page_shift) < d->page_size; ++p.page_shift) {}
   // one resident wave of CTAs, no more groups than the cache could have stretches
-  int slots = sms * CTAS_PER_SM;
+  int slots = sms * (d->dim == 128 ? Cfg<128>::CTAS_PER_SM : Cfg<64>::CTAS_PER_SM);
   if (slots > MAX_CTAS) slots = MAX_CTAS;
   long long groups = slots / p.ht;
   const __int128 tiles = (__int128)d->batch * ((d->max_pages * d->page_size + TILE - 1) / TILE);
