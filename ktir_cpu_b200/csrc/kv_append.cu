@@ -4,22 +4,27 @@
 // cosine and sine of the position times the pair's frequency, read from an f32
 // table and applied in f32; one rounding to the element type at the end.
 //
-// Bound by memory: each of q, k, v is read once and written once.  dim / 16
-// threads share a head vector, each with two 16-byte vectors that hold whole
-// pairs: vectors j and j + rot/16 of the rotated part when pairs are (i, i +
-// rot/2), vectors 2j and 2j+1 when they are (2i, 2i+1).  A thread keeps its
-// cosines and sines in registers and walks over the token's heads.
+// Bound by memory: each of q, k, v is read once and written once.  One block per
+// token; dim / 16 threads share a head vector, each with two 16-byte vectors
+// that hold whole pairs: vectors j and j + rot/16 of the rotated part when pairs
+// are (i, i + rot/2), vectors 2j and 2j+1 when they are (2i, 2i+1).  A thread
+// keeps its cosines and sines in registers and walks over the token's heads,
+// three vectors on their way at once, the first ones asked for before the
+// position, the slot and the table's row are there.  Blocks of 64 threads, 32 of
+// them per SM, keep the most copies in flight: 24576 tokens of 32 + 8 + 8 heads
+// of 128 take 93 us = 6.6 TB/s (128 threads: 106 us, one vector at a time: 98).
 #include "serve_common.cuh"
 
 using namespace ktir::serve;
 
 namespace {
 
-constexpr int THREADS = 128;
+constexpr int UNROLL = 3;      // head vectors of a thread on their way at once
 
 struct AppendParams {
   KtirKvAppendDesc d;
   long long slots_total;
+  int vector_table;      // rows of the table start on 16-byte boundaries
 };
 
 template <typename T>
@@ -68,81 +73,89 @@ __device__ __forceinline__ uint4 rotate_pairs(const uint4& a, const float (&c)[8
   return r;
 }
 
-template <typename T>
+template <typename T, int THREADS>
 __global__ void __launch_bounds__(THREADS) k_kv_append(const __grid_constant__ AppendParams p) {
   const KtirKvAppendDesc& d = p.d;
   const long long t = blockIdx.x;
   const int parts = d.dim >> 4;                 // threads per head vector
-  const int j = threadIdx.x % parts;
   const int lanes = THREADS / parts;            // head vectors in flight per block
-  int hl = threadIdx.x / parts;
+  const int hl = threadIdx.x / parts, j = threadIdx.x - hl * parts;
   if (hl >= lanes) return;
   const int rparts = d.rot >> 4;
   const bool turn = j < rparts;
+  // this thread's two vectors of a head vector, rotated or copied
+  const int first = d.interleaved ? 16 * j : turn ? 8 * j : d.rot + 16 * (j - rparts);
+  const int second = !d.interleaved && turn ? first + (d.rot >> 1) : first + 8;
+  const int hq = d.q ? d.heads : 0, hk = hq + d.kv_heads, n = hk + d.kv_heads;
 
   pdl_launch();
   pdl_wait();
   const int slot = d.slots[t];
-  bool bad = slot >= p.slots_total;
+  const int pos = rparts ? d.positions[t] : 0;
+  const bool bad = slot >= p.slots_total || (rparts && (pos < 0 || pos >= d.table_rows));
   float c[8], s[8];
-  if (rparts) {
-    const int pos = d.positions[t];
-    if (pos < 0 || pos >= d.table_rows) {
-      bad = true;
-    } else if (turn) {
-      const float* row = d.table + (long long)pos * d.table_stride + 8 * j;
+  const bool kept = slot >= 0 && !bad;
+  const long long page = kept ? slot / d.page_size : 0;
+  const long long place = kept ? slot - page * d.page_size : 0;
+  for (int h0 = hl; h0 < n; h0 += UNROLL * lanes) {
+    uint4 a[UNROLL], b[UNROLL];
 #pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        c[i] = row[i];
-        s[i] = row[(d.rot >> 1) + i];
+    for (int u = 0; u < UNROLL; ++u) {
+      const int h = h0 + u * lanes;
+      if (h < n) {
+        const T* src = h < hq   ? static_cast<const T*>(d.q) + t * d.q_stride[0] + h * d.q_stride[1]
+                       : h < hk ? static_cast<const T*>(d.k) + t * d.k_stride[0] + (h - hq) * d.k_stride[1]
+                                : static_cast<const T*>(d.v) + t * d.v_stride[0] + (h - hk) * d.v_stride[1];
+        a[u] = *reinterpret_cast<const uint4*>(src + first);
+        b[u] = *reinterpret_cast<const uint4*>(src + second);
       }
     }
-  }
-  if (bad) {
-    if (threadIdx.x == 0) atomicOr(d.status, KTIR_STATUS_BAD_INDEX);
-    return;
-  }
-  // this thread's two vectors of a head vector, rotated (r) or copied
-  const int first = d.interleaved ? 16 * j : turn ? 8 * j : d.rot + 16 * (j - rparts);
-  const int second = !d.interleaved && turn ? first + (d.rot >> 1) : first + 8;
-  const T* q = static_cast<const T*>(d.q);
-  const int hq = q ? d.heads : 0;
-  const int n = hq + (slot >= 0 ? 2 * d.kv_heads : 0);
-  const long long page = slot >= 0 ? slot / d.page_size : 0;
-  const long long place = slot >= 0 ? slot - page * d.page_size : 0;
-  for (int h = hl; h < n; h += lanes) {
-    const T* src;
-    T* dst;
-    bool r = turn;
-    if (h < hq) {
-      src = q + t * d.q_stride[0] + h * d.q_stride[1];
-      dst = static_cast<T*>(d.q_out) + t * d.qo_stride[0] + h * d.qo_stride[1];
-    } else if (h < hq + d.kv_heads) {
-      const int g = h - hq;
-      src = static_cast<const T*>(d.k) + t * d.k_stride[0] + g * d.k_stride[1];
-      dst = static_cast<T*>(d.k_cache) + page * d.kc_stride[0] + place * d.kc_stride[1] +
-            g * d.kc_stride[2];
-    } else {
-      const int g = h - hq - d.kv_heads;
-      src = static_cast<const T*>(d.v) + t * d.v_stride[0] + g * d.v_stride[1];
-      dst = static_cast<T*>(d.v_cache) + page * d.vc_stride[0] + place * d.vc_stride[1] +
-            g * d.vc_stride[2];
-      r = false;
-    }
-    const uint4 a = *reinterpret_cast<const uint4*>(src + first);
-    const uint4 b = *reinterpret_cast<const uint4*>(src + second);
-    uint4 x = a, y = b;
-    if (r) {
-      if (d.interleaved) {
-        x = rotate_pairs<T>(a, c, s, 0);
-        y = rotate_pairs<T>(b, c, s, 4);
-      } else {
-        x = rotate_first<T>(a, b, c, s);
-        y = rotate_second<T>(a, b, c, s);
+    if (h0 == hl) {                             // the vectors are on their way meanwhile
+      if (bad) {
+        if (threadIdx.x == 0) atomicOr(d.status, KTIR_STATUS_BAD_INDEX);
+        return;
+      }
+      if (turn) {
+        const float* row = d.table + (long long)pos * d.table_stride + 8 * j;
+        if (p.vector_table) {
+#pragma unroll
+          for (int i = 0; i < 8; i += 4) {
+            *reinterpret_cast<float4*>(c + i) = __ldg(reinterpret_cast<const float4*>(row + i));
+            *reinterpret_cast<float4*>(s + i) = __ldg(reinterpret_cast<const float4*>(row + (d.rot >> 1) + i));
+          }
+        } else {
+#pragma unroll
+          for (int i = 0; i < 8; ++i) {
+            c[i] = row[i];
+            s[i] = row[(d.rot >> 1) + i];
+          }
+        }
       }
     }
-    *reinterpret_cast<uint4*>(dst + first) = x;
-    *reinterpret_cast<uint4*>(dst + second) = y;
+#pragma unroll
+    for (int u = 0; u < UNROLL; ++u) {
+      const int h = h0 + u * lanes;
+      if (h >= n || (h >= hq && !kept)) continue;
+      uint4 x = a[u], y = b[u];
+      if (turn && h < hk) {
+        if (d.interleaved) {
+          x = rotate_pairs<T>(a[u], c, s, 0);
+          y = rotate_pairs<T>(b[u], c, s, 4);
+        } else {
+          x = rotate_first<T>(a[u], b[u], c, s);
+          y = rotate_second<T>(a[u], b[u], c, s);
+        }
+      }
+      T* dst;
+      if (h < hq)
+        dst = static_cast<T*>(d.q_out) + t * d.qo_stride[0] + h * d.qo_stride[1];
+      else if (h < hk)
+        dst = static_cast<T*>(d.k_cache) + page * d.kc_stride[0] + place * d.kc_stride[1] + (h - hq) * d.kc_stride[2];
+      else
+        dst = static_cast<T*>(d.v_cache) + page * d.vc_stride[0] + place * d.vc_stride[1] + (h - hk) * d.vc_stride[2];
+      *reinterpret_cast<uint4*>(dst + first) = x;
+      *reinterpret_cast<uint4*>(dst + second) = y;
+    }
   }
 }
 
@@ -176,10 +189,17 @@ extern "C" int ktir_kv_append(const KtirKvAppendDesc* d, void* stream) {
   p.d = *d;
   const __int128 total = (__int128)d->num_pages * d->page_size;
   p.slots_total = total > 0x7fffffffLL ? 0x80000000LL : (long long)total;
+  p.vector_table = aligned16(d->table) && !(d->table_stride & 3);
   const unsigned grid = (unsigned)d->tokens;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
-  const cudaError_t e = d->dtype == KTIR_F16
-                            ? launch_pdl(k_kv_append<__half>, grid, THREADS, 0, s, p)
-                            : launch_pdl(k_kv_append<__nv_bfloat16>, grid, THREADS, 0, s, p);
+  // with no more tokens than SMs a larger block is quicker (one token 2.4 us against
+  // 3.2), with more a smaller one (200 tokens 2.65 us against 3.2)
+  const bool f16 = d->dtype == KTIR_F16;
+  const cudaError_t e =
+      d->tokens <= sm_count()
+          ? (f16 ? launch_pdl(k_kv_append<__half, 128>, grid, 128, 0, s, p)
+                 : launch_pdl(k_kv_append<__nv_bfloat16, 128>, grid, 128, 0, s, p))
+          : (f16 ? launch_pdl(k_kv_append<__half, 64>, grid, 64, 0, s, p)
+                 : launch_pdl(k_kv_append<__nv_bfloat16, 64>, grid, 64, 0, s, p));
   return launched(e, "ktir_kv_append: launch failed");
 }
