@@ -488,7 +488,9 @@ int ktir_paged_decode(const KtirPagedDecodeDesc* desc, void* stream);
  * end: query i of n sees keys j <= i + m - n of m (m > n when the first part
  * of the prompt was read earlier); a query that sees no key gives zeros (lse
  * -inf).  lse as above, [tokens][heads].  dim 64 or 128; heads / kv_heads at
- * most 128. */
+ * most 128.  With a workspace (ktir_prompt_attention_workspace() bytes, zero
+ * before its first use, its own for calls that may overlap) few queries over
+ * many keys share the keys among the SMs. */
 typedef struct {
   const void* q;                 /* [tokens][heads][dim] */
   const void* k; const void* v;  /* [kv_tokens][kv_heads][dim] */
@@ -497,12 +499,15 @@ typedef struct {
   const int32_t* offsets;        /* [batch + 1] */
   const int32_t* kv_offsets;     /* [batch + 1] */
   int32_t* status;
+  void* workspace;               /* or null */
+  int64_t workspace_bytes;
   int64_t batch, tokens, kv_tokens;
   int64_t q_stride[2], k_stride[2], v_stride[2], out_stride[2];   /* token, head */
   int32_t heads, kv_heads, dim, dtype;
   float scale;
   int32_t causal;
 } KtirPromptDesc;
+int64_t ktir_prompt_attention_workspace(void);
 int ktir_prompt_attention(const KtirPromptDesc* desc, void* stream);
 
 #ifdef __cplusplus

@@ -10,9 +10,17 @@
 // while the other is in the tensor pipe.
 //
 // A row is a (token, head) pair: the g = heads / kv_heads queries that share a
-// kv head lie side by side, 128 / g tokens per tile, so that every row of a
+// kv head lie side by side, 128 / g tokens per row tile, so that every row of a
 // tile uses the same K and V whatever g is, and a short prompt fills more of a
 // tile.
+//
+// Which row tiles a CTA takes depends on how many there are (see plan()):
+//   pairs    two that follow each other in a sequence, sharing its K and V blocks
+//   singles  two of any sequences and heads, each with blocks of its own, where
+//            most sequences have but one row tile per head
+//   parts    no more row tiles than SMs: one per CTA, or, where its keys are many,
+//            a stretch of them; the stretches' (m, l, O) are left in the workspace
+//            and the last CTA of a row tile joins them in their order
 //
 // Roles, meeting only at mbarriers:
 //   warps 0-3, 4-7  the softmax of row tile 0 and 1, one row per thread:
@@ -25,10 +33,10 @@
 //   warp 9 (TMA)    Q tiles, and K_j, V_j through one ring
 //   warp 11         finds the next tile: tiles are taken in order of falling
 //                   key counts over all sequences, back and forth over the
-//                   CTAs, so that the last ones to finish are the shortest; and
-//                   sets V's rows past the sequence's last key to zero (they
-//                   belong to another sequence; a weight of 0 does not cancel
-//                   an infinity there)
+//                   CTAs, so that the last ones to finish are the shortest
+// V rows past a sequence's last key belong to another sequence, and a weight of 0
+// does not cancel an infinity there: a softmax warp sets them to zero in shared
+// memory before the last block's product.
 // TMEM holds S, P and O of both row tiles apart, which at dim 128 leaves room for
 // blocks of 80 keys (128 at dim 64).
 // The running maximum moves only when a row's maximum exceeds it by more than
@@ -54,6 +62,11 @@ namespace {
 constexpr int BQ = 128;              // rows of a row tile
 constexpr int THREADS = 384;
 constexpr int SCHED = 4;             // tiles announced ahead
+constexpr int WEIGHTS = 512;         // weights whose tile counts a CTA keeps there
+constexpr int CACHED = 256;          // sequences whose lengths a CTA keeps in shared memory
+constexpr int MAX_PARTS = 160;       // CTAs of a launch that splits keys
+constexpr int PART_FLOATS = 128 * BQ + 2 * BQ;      // O [dim][row], then (m, l) per row
+constexpr int64_t PARTS_BYTES = (int64_t)MAX_PARTS * PART_FLOATS * 4;
 constexpr int SCHED_READERS = 11;    // 8 softmax warps, two MMA, TMA
 constexpr float RESCALE_THRESHOLD = 8.0f;   // log2 units
 constexpr int SOFTMAX_REGS = 208, OTHER_REGS = 80;
@@ -66,23 +79,46 @@ struct Cfg {
   static constexpr int PANELS = D / 64;             // of 64 elements, rows of 128 bytes, swizzled
   static constexpr int Q_PANEL = BQ * 128, Q_TILE = PANELS * Q_PANEL;
   static constexpr int PANEL = BK * 128, TILE = PANELS * PANEL;      // a K or V block
-  static constexpr int STAGES = D == 128 ? 8 : 10;
-  static constexpr int BYTES = 2 * Q_TILE + STAGES * TILE;
+  static constexpr int STAGES = D == 128 ? 6 : 9;
+  // a softmax warp's 32 rows of 64 output elements on their way to memory, rows
+  // 16 bytes apart from a multiple of 128 (no two of eight lanes in one bank)
+  static constexpr int OUT_ROW = 144, OUT_WARP = 32 * OUT_ROW;
+  static constexpr int OUT = 2 * Q_TILE + STAGES * TILE;
+  static constexpr int BYTES = OUT + 8 * OUT_WARP;
   // first columns of row tile 0, and from one row tile to the next
   static constexpr uint32_t S_COL = 0, S_STEP = 128, O_COL = D == 128 ? 256 : 384, O_STEP = D;
   static constexpr uint32_t P_COL = D == 128 ? 80 : 256, P_STEP = D == 128 ? 128 : 64;
 };
-constexpr int MAX_STAGES = 10;
+constexpr int MAX_STAGES = 9;
 
-struct Tile {
-  int stop;
-  int token;      // first token of the tile (of row tile 0)
-  int tokens;     // of the sequence from there on
+struct RowTile {
+  int token;      // its first token
+  int tokens;     // of the sequence from there on, at most a row tile's
   int seen;       // keys that the first token sees (causal)
   int keys;       // of the sequence
   int key0;       // its first key
   int head;       // kv head
-  int blocks[2];  // key blocks of each row tile
+  int blocks;     // key blocks
+};
+
+struct Tile {
+  int stop;
+  int shared;     // both row tiles use the same K and V blocks
+  int splits;     // CTAs that share row tile 0, each with a stretch of its keys,
+  int split;      // which of them this is
+  int unit;       // and the row tile's number
+  RowTile r[2];
+};
+
+struct PromptParams {
+  KtirPromptDesc d;
+  int group;            // query heads per kv head
+  int tile_tokens;      // tokens of a row tile
+  int k_head_step, v_head_step, q_head_step;   // 0 where all heads share one vector
+  uint32_t token_magic;  // for divisions by tile_tokens, and by twice that
+  uint32_t pair_magic;
+  float* parts;          // or null: no splitting
+  int* counters;         // zero between calls
 };
 
 struct Shared {
@@ -92,17 +128,15 @@ struct Shared {
   uint64_t tail[MAX_STAGES];        // a V block with rows past the last key has arrived
   uint64_t drain[2];
   uint64_t sched_full[SCHED], sched_empty[SCHED];
+  uint64_t part_in, part_out;
   Tile tile[SCHED];
+  int2 lengths[CACHED];             // tokens and keys of the first sequences
+  int last;
+  int weights[WEIGHTS];             // tiles of at least this weight
   uint32_t tmem_base;
   int abort_flag;
 };
 
-struct PromptParams {
-  KtirPromptDesc d;
-  int group;            // query heads per kv head
-  int tile_tokens;      // tokens of a row tile
-  int k_head_step, v_head_step, q_head_step;   // 0 where all heads share one vector
-};
 
 __device__ __forceinline__ void tma_load_3d(uint32_t dst, const CUtensorMap* map, uint32_t bar, int x, int y,
                                             int z) {
@@ -273,106 +307,166 @@ __device__ __forceinline__ void fewer_registers() {
 }
 
 // -- the order of tiles -----------------------------------------------------------
-// Tile i of a sequence (n tokens, m keys) holds tokens [i T, (i + 1) T), T = two row
-// tiles; its weight is the number of key blocks that its last token sees.  Tiles
-// are numbered by falling weight over all sequences; within a weight by
-// sequence, and each tile once per kv head.
+// A tile holds T tokens of a sequence (n tokens, m keys): tile i tokens [i T, (i + 1)
+// T).  Its weight is the number of key blocks that its last token sees.  Tiles are
+// numbered by falling weight over all sequences, within a weight by sequence, and
+// each once per kv head.
 struct Seq {
-  int n, m, tiles;
+  int n, m;
 };
 
-__device__ __forceinline__ Seq sequence(const KtirPromptDesc& d, long long b, int T, bool& bad) {
+__device__ __forceinline__ Seq sequence(const KtirPromptDesc& d, long long b, bool& bad) {
   const int q0 = d.offsets[b], q1 = d.offsets[b + 1], k0 = d.kv_offsets[b], k1 = d.kv_offsets[b + 1];
   bad = q0 < 0 || q1 < q0 || q1 > d.tokens || k0 < 0 || k1 < k0 || k1 > d.kv_tokens;
   Seq s;
   s.n = bad ? 0 : q1 - q0;
   s.m = bad ? 0 : k1 - k0;
-  s.tiles = (s.n + T - 1) / T;
   return s;
 }
 
-// tiles of weight at least `w`: the last ones of the sequence
-template <int BK>
-__device__ __forceinline__ int heavier(const Seq& s, int w, int T, int causal) {
-  if (w <= 0) return s.tiles;
-  const int need = (w - 1) * BK;             // more than this many keys seen
-  if (s.m <= need) return 0;
-  if (!causal) return s.tiles;
-  const int x = need - (s.m - s.n);          // (i + 1) T > x
-  return x <= 0 ? s.tiles : s.tiles - x / T;
-}
+__device__ __forceinline__ int warp_sum(int v) { return __reduce_add_sync(0xffffffffu, v); }
 
-__device__ __forceinline__ int warp_sum(int v) {
-#pragma unroll
-  for (int w = 16; w; w >>= 1) v += __shfl_xor_sync(0xffffffffu, v, w);
-  return v;
-}
-
+// The tiles of one size, walked from heaviest to lightest by one warp.
 template <int BK>
-__device__ int tiles_of_weight(const KtirPromptDesc& d, int w, int T, int lane) {
-  int c = 0;
-  for (long long b = lane; b < d.batch; b += 32) {
-    bool bad;
-    c += heavier<BK>(sequence(d, b, T, bad), w, T, d.causal);
+struct Order {
+  const PromptParams& p;
+  const int2* cached;
+  int lane, T;
+  uint32_t magic;
+  int weight;            // of the tile last found, at first the heaviest of all
+  int above;             // tiles heavier than that
+  int* table;            // tiles of at least each weight, or null
+
+  __device__ __forceinline__ int divide(int x) const {      // x / T, x >= 0
+    int q = (int)__umulhi((uint32_t)x, magic);
+    q -= q * T > x;
+    q += (q + 1) * T <= x;
+    return q;
   }
-  return warp_sum(c);
-}
-
-// tile number `x` (0 = heaviest), by one warp
-template <int BK>
-__device__ void find_tile(const KtirPromptDesc& d, int x, int head, int T, int heaviest, int lane, Tile& t) {
-  int lo = 0, hi = heaviest + 1;             // count(lo) > x >= count(hi)
-  int above = 0;
-  while (hi - lo > 1) {
-    const int mid = (lo + hi) >> 1;
-    const int c = tiles_of_weight<BK>(d, mid, T, lane);
-    if (c > x) {
-      lo = mid;
-    } else {
-      hi = mid;
-      above = c;
+  __device__ __forceinline__ Seq seq(long long b) const {
+    if (b < CACHED) {
+      const int2 v = cached[b];
+      return Seq{v.x, v.y};
     }
-  }
-  int r = x - above;
-  for (long long b0 = 0; b0 < d.batch; b0 += 32) {
-    const long long b = b0 + lane;
-    Seq s = {0, 0, 0};
-    int first = 0, count = 0;
     bool bad;
-    if (b < d.batch) {
-      s = sequence(d, b, T, bad);
-      const int c = heavier<BK>(s, lo, T, d.causal);
-      count = c - heavier<BK>(s, lo + 1, T, d.causal);
-      first = s.tiles - c;
-    }
-    int incl = count;
-#pragma unroll
-    for (int w = 1; w < 32; w <<= 1) {
-      const int o = __shfl_up_sync(0xffffffffu, incl, w);
-      if (lane >= w) incl += o;
-    }
-    const int all = __shfl_sync(0xffffffffu, incl, 31);
-    if (r >= all) {
-      r -= all;
-      continue;
-    }
-    if (r >= incl - count && r < incl) {
-      const int i = first + r - (incl - count), at = i * T, half = T / 2;
-      t.stop = 0;
-      t.token = d.offsets[b] + at;
-      t.tokens = s.n - at;
-      t.seen = at + s.m - s.n + 1;
-      t.keys = s.m;
-      t.key0 = d.kv_offsets[b];
-      t.head = head;
-      for (int w = 0; w < 2; ++w) {
-        const int here = min(half, t.tokens - w * half);       // tokens of the row tile
-        const int end = d.causal ? min(s.m, at + w * half + here + s.m - s.n) : s.m;
-        t.blocks[w] = here > 0 && end > 0 ? (end + BK - 1) / BK : 0;
+    return sequence(p.d, b, bad);
+  }
+  // tiles of weight at least `w`: the last ones of the sequence
+  __device__ __forceinline__ int heavier(const Seq& s, int w) const {
+    const int tiles = divide(s.n + T - 1);
+    if (w <= 0) return tiles;
+    const int need = (w - 1) * BK;             // more than this many keys seen
+    if (s.m <= need) return 0;
+    if (!p.d.causal) return tiles;
+    const int x = need - (s.m - s.n);          // (i + 1) T > x
+    return x <= 0 ? tiles : tiles - divide(x);
+  }
+  __device__ int count(int w) const {
+    int c = 0;
+    for (long long b = lane; b < p.d.batch; b += 32) c += heavier(seq(b), w);
+    return warp_sum(c);
+  }
+  // the table: every tile counted at its weight, then summed from the heaviest down
+  __device__ void tabulate(int* place, int heaviest) {
+    if (heaviest >= WEIGHTS) return;
+    table = place;
+    for (int w = lane; w <= heaviest; w += 32) table[w] = 0;
+    __syncwarp();
+    for (long long b = lane; b < p.d.batch; b += 32) {
+      const Seq s = seq(b);
+      if (!s.n) continue;
+      const int seen = p.d.causal ? min(s.m, min(s.n, T) + s.m - s.n) : s.m;        // by the first tile
+      for (int w = seen > 0 ? (seen + BK - 1) / BK : 0, have = divide(s.n + T - 1); have > 0; ++w) {
+        const int more = heavier(s, w + 1);                            // the others have weight w
+        if (have > more) atomicAdd(table + w, have - more);
+        have = more;
       }
     }
-    break;
+    __syncwarp();
+    int sum = 0;
+    for (int w0 = heaviest - (heaviest & 31); w0 >= 0; w0 -= 32) {
+      int v = w0 + lane <= heaviest ? table[w0 + lane] : 0;
+#pragma unroll
+      for (int k = 1; k < 32; k <<= 1) {
+        const int o = __shfl_down_sync(0xffffffffu, v, k);
+        if (lane + k < 32) v += o;
+      }
+      v += sum;
+      sum = __shfl_sync(0xffffffffu, v, 0);
+      if (w0 + lane <= heaviest) table[w0 + lane] = v;
+    }
+    __syncwarp();
   }
+  // tile number `x`, not below the last one found: its sequence and place there
+  __device__ void find(int x, long long& b_out, int& i_out) {
+    if (table) {
+      while (weight > 0 && table[weight] <= x) above = table[weight--];
+    } else {
+      int hi = weight + 1, hi_count = above;   // count(hi) <= x
+      int step = 1, lo = max(0, hi - 1), c = count(lo);
+      while (c <= x && lo > 0) {
+        hi = lo;
+        hi_count = c;
+        step <<= 1;
+        lo = max(0, hi - step);
+        c = count(lo);
+      }
+      while (hi - lo > 1) {                    // count(lo) > x >= count(hi)
+        const int mid = (lo + hi) >> 1;
+        c = count(mid);
+        if (c > x) {
+          lo = mid;
+        } else {
+          hi = mid;
+          hi_count = c;
+        }
+      }
+      weight = lo;
+      above = hi_count;
+    }
+    const int lo = weight;
+    int r = x - above;
+    b_out = -1;
+    i_out = 0;
+    for (long long b0 = 0; b0 < p.d.batch; b0 += 32) {
+      const long long b = b0 + lane;
+      int first = 0, mine = 0;
+      if (b < p.d.batch) {
+        const Seq s = seq(b);
+        const int all = heavier(s, lo);
+        mine = all - heavier(s, lo + 1);
+        first = divide(s.n + T - 1) - all;
+      }
+      int incl = mine;
+#pragma unroll
+      for (int w = 1; w < 32; w <<= 1) {
+        const int o = __shfl_up_sync(0xffffffffu, incl, w);
+        if (lane >= w) incl += o;
+      }
+      const unsigned hit = __ballot_sync(0xffffffffu, r >= incl - mine && r < incl);
+      if (hit) {
+        const int from = __ffs(hit) - 1;
+        b_out = b0 + from;
+        i_out = __shfl_sync(0xffffffffu, first + r - (incl - mine), from);
+        return;
+      }
+      r -= __shfl_sync(0xffffffffu, incl, 31);
+    }
+  }
+};
+
+// the row tile at token `at` of sequence b
+template <int BK>
+__device__ __forceinline__ void row_tile(const PromptParams& p, long long b, const Seq& s, int at, int head, RowTile& r) {
+  const int here = max(0, min(p.tile_tokens, s.n - at));     // its tokens
+  const int end = p.d.causal ? min(s.m, at + here + s.m - s.n) : s.m;
+  r.token = p.d.offsets[b] + at;
+  r.tokens = here;
+  r.seen = at + s.m - s.n + 1;
+  r.keys = s.m;
+  r.key0 = p.d.kv_offsets[b];
+  r.head = head;
+  r.blocks = here > 0 && end > 0 ? (end + BK - 1) / BK : 0;
 }
 
 template <typename T, int D>
@@ -407,6 +501,8 @@ __global__ void __launch_bounds__(THREADS, 1)
       mbar_init(smem_u32(&B.tail[s]), 1);
     }
     for (int w = 0; w < 2; ++w) mbar_init(smem_u32(&B.drain[w]), 1);
+    mbar_init(smem_u32(&B.part_in), 4);
+    mbar_init(smem_u32(&B.part_out), 1);
     for (int s = 0; s < SCHED; ++s) {
       mbar_init(smem_u32(&B.sched_full[s]), 1);
       mbar_init(smem_u32(&B.sched_empty[s]), SCHED_READERS);
@@ -424,101 +520,110 @@ __global__ void __launch_bounds__(THREADS, 1)
   pdl_launch();
   pdl_wait();
 
-  // announced tiles, read by whole warps: false at the end (or on an abort)
-  auto next_tile = [&](int k, Tile& t) -> bool {
+  // announced tiles, waited for by whole warps (false at the end, or on an abort) and
+  // left in their place until the warp has done with them
+  auto next_tile = [&](int k) -> bool {
     const int s = k % SCHED;
-    if (!__all_sync(0xffffffffu, wait(smem_u32(&B.sched_full[s]), (k / SCHED) & 1, abort))) return false;
-    t = B.tile[s];
+    return __all_sync(0xffffffffu, wait(smem_u32(&B.sched_full[s]), (k / SCHED) & 1, abort)) && !B.tile[s].stop;
+  };
+  auto done_tile = [&](int k) {
     __syncwarp();
-    if (lane == 0) mbar_arrive(smem_u32(&B.sched_empty[s]));
-    return !t.stop;
+    if (lane == 0) mbar_arrive(smem_u32(&B.sched_empty[k % SCHED]));
   };
 
   if (warp >= 8) {
     fewer_registers<OTHER_REGS>();
     if (warp == 11) {
       // ---------------- tile finder ----------------
-      const int span = 2 * p.tile_tokens;
-      int heaviest = 0, total = 0;
+      // plan(): the same in every CTA
+      const int half = p.tile_tokens;
+      int heaviest = 0, singles = 0, pairs = 0;
       bool any_bad = false;
       for (long long b = lane; b < d.batch; b += 32) {
         bool bad;
-        const Seq s = sequence(d, b, span, bad);
+        const Seq s = sequence(d, b, bad);
+        if (b < CACHED) B.lengths[b] = make_int2(s.n, s.m);
         any_bad |= bad;
         if (s.n) heaviest = max(heaviest, (s.m + BK - 1) / BK);
-        total += s.tiles;
+        singles += (s.n + half - 1) / half;
+        pairs += (s.n + 2 * half - 1) / (2 * half);
       }
       if (blockIdx.x == 0) {
         if (lane == 0) any_bad |= d.offsets[0] != 0 || d.offsets[d.batch] != d.tokens;
         if (any_bad) atomicOr(d.status, KTIR_STATUS_BAD_INDEX);
       }
-      total = warp_sum(total);
-  #pragma unroll
-      for (int w = 16; w; w >>= 1) heaviest = max(heaviest, __shfl_xor_sync(0xffffffffu, heaviest, w));
-      const long long all = (long long)total * d.kv_heads;
-      int next = 0, fix = 0, loads = 0;         // tile to announce, tile to look after, ring loads before it
-      bool stop = false;
-      uint32_t phase = 0;                       // of the ring stages' tail barriers
-      for (uint32_t idle = 0; !stop || fix < next - 1;) {
-        bool moved = false;
+      __syncwarp();
+      heaviest = (int)__reduce_max_sync(0xffffffffu, (unsigned)heaviest);
+      const long long rows = (long long)warp_sum(singles) * d.kv_heads, twos = (long long)warp_sum(pairs) * d.kv_heads;
+      const int G = (int)gridDim.x;
+      // no more row tiles than CTAs: one each, and what is left over shares their keys.
+      // A stretch costs its blocks, joining S of them about as much as S blocks.
+      const bool parts = rows <= G;
+      int splits = 1;
+      if (parts && rows > 0 && p.parts) {
+        while (splits * splits < heaviest) ++splits;
+        splits = max(1, min(splits, (int)(min(G, MAX_PARTS) / rows)));
+      }
+      // Singles where a CTA has few row tiles, each then next to one of another weight
+      // (7 pieces of prompts, 195 row tiles: 43 us against 55 in pairs), or where pairs
+      // would leave more than a third of them empty (200 prompts of 32 tokens: 46 us
+      // against 67).  Else pairs: their shared blocks save L2 traffic (8192 tokens: 477
+      // us against 573).
+      const bool singly = parts || rows <= 2 * G || 2 * twos - rows > (2 * twos) / 3;
+      const long long all = parts ? rows * splits : singly ? (rows + 1) / 2 : twos;
+      Order<BK> order = {p, B.lengths, lane, singly ? half : 2 * half, singly ? p.token_magic : p.pair_magic, heaviest, 0, nullptr};
+
+      for (int next = 0;; ++next) {
         const int s = next % SCHED;
-        if (!stop && next < fix + SCHED &&
-            (next < SCHED || __all_sync(0xffffffffu, mbar_test_wait(smem_u32(&B.sched_empty[s]),
-                                                                    (next / SCHED - 1) & 1)))) {
-          const long long x =
-              (long long)next * gridDim.x + ((next & 1) ? gridDim.x - 1 - blockIdx.x : blockIdx.x);
-          // back and forth, a CTA may have a tile in the last round after having none before it
-          stop = (long long)next * gridDim.x >= all;
-          if (stop) {
-            if (lane == 0) B.tile[s].stop = 1;
-          } else if (x < all) {
-            find_tile<BK>(d, (int)(x / d.kv_heads), (int)(x % d.kv_heads), span, heaviest, lane, B.tile[s]);
-          } else if (lane == 0) {
-            Tile& t = B.tile[s];
-            t.stop = 0;
-            t.tokens = t.blocks[0] = t.blocks[1] = t.keys = 0;
-            t.token = t.key0 = t.head = 0;
-            t.seen = 0;
-          }
-          __syncwarp();
-          if (lane == 0) mbar_arrive(smem_u32(&B.sched_full[s]));
-          ++next;
-          moved = true;
+        if (next >= SCHED &&
+            !__all_sync(0xffffffffu, wait(smem_u32(&B.sched_empty[s]), (next / SCHED - 1) & 1, abort)))
+          break;
+        // rounds of G (two of them at once for singles), back and forth: a heavy one here
+        // is followed by a light one
+        const long long x = (long long)next * G + ((next & 1) ? G - 1 - blockIdx.x : blockIdx.x);
+        const long long first = parts ? x : singly ? 2LL * next * G + blockIdx.x : x;
+        Tile& t = B.tile[s];
+        // a CTA may have a tile in the last round after having none before it
+        const bool stop = (long long)next * G >= all;
+        if (lane == 0) {
+          t.stop = stop;
+          t.shared = !singly;
+          t.splits = 1;                       // an empty tile has no part in another's
+          t.split = t.unit = 0;
+          for (int w = 0; w < 2; ++w) t.r[w].tokens = t.r[w].blocks = t.r[w].keys = 0;
         }
-        if (fix < next - (stop ? 1 : 0)) {
-          // V rows past the last key of tile `fix`
-          const Tile& t = B.tile[fix % SCHED];
-          const int blocks = max(t.blocks[0], t.blocks[1]), left = t.keys - (blocks - 1) * BK;
-          const int r = (loads + 2 * blocks - 1) % STAGES;
-          const bool tail = blocks && left < BK;
-          if (!tail || __all_sync(0xffffffffu, mbar_test_wait(smem_u32(&B.tail[r]), (phase >> r) & 1))) {
-            if (tail) {
-              phase ^= 1u << r;
-              uint8_t* v = smem_raw + (ring + r * C::TILE - smem_u32(smem_raw));
-              // whole 128-byte rows of each panel: the swizzle permutes within a row
-              for (int i = left * 8 + lane; i < BK * 8; i += 32)
-#pragma unroll
-                for (int c = 0; c < C::PANELS; ++c)
-                  *reinterpret_cast<uint4*>(v + c * C::PANEL + i * 16) = make_uint4(0, 0, 0, 0);
-              fence_proxy_async();
-              __syncwarp();
-              if (lane == 0) mbar_arrive(smem_u32(&B.full[r]));
+        __syncwarp();
+        if (!stop) {
+          for (int w = 0; w < 2; ++w) {
+            const long long y = parts ? x / splits : singly && w ? first + 2 * (G - 1 - blockIdx.x) + 1 : first;
+            if ((parts && (w || x >= all)) || y >= (singly ? rows : twos)) break;
+            long long b;
+            int i;
+            order.find((int)(y / d.kv_heads), b, i);
+            if (lane == 0 && b >= 0) {
+              const int head = (int)(y % d.kv_heads);
+              const Seq q = order.seq(b);
+              row_tile<BK>(p, b, q, i * order.T, head, t.r[w]);
+              if (!singly) row_tile<BK>(p, b, q, i * order.T + half, head, t.r[1]);
+              if (splits > 1) {               // this CTA's stretch of the keys
+                RowTile& r = t.r[0];
+                t.splits = splits;
+                t.split = (int)(x % splits);
+                t.unit = (int)y;
+                const int per = (r.blocks + splits - 1) / splits, from = min(r.blocks, t.split * per);
+                r.blocks = min(per, r.blocks - from);
+                r.key0 += from * BK;
+                r.keys -= from * BK;
+                r.seen -= from * BK;
+              }
             }
-            loads += 2 * blocks;
-            ++fix;
-            moved = true;
+            if (!singly) break;
           }
         }
-        if (moved) {
-          idle = 0;
-        } else {
-          if (__any_sync(0xffffffffu, *abort != 0)) break;
-          if (++idle > kSpinLimit) {
-            *abort = 1;
-            break;
-          }
-          __nanosleep(40);
-        }
+        __syncwarp();
+        if (lane == 0) mbar_arrive(smem_u32(&B.sched_full[s]));
+        if (stop) break;
+        if (next == 0 && all > 2 * G) order.tabulate(B.weights, heaviest);    // worth it for a few more
       }
     } else if (warp == 9) {
       // ---------------- TMA ----------------
@@ -531,13 +636,13 @@ __global__ void __launch_bounds__(THREADS, 1)
       const uint32_t q_bytes = (uint32_t)(p.group * p.tile_tokens) * 128u * C::PANELS;
       int loads = 0, q_loads[2] = {0, 0};
       uint32_t was_tail = 0, tail_phase = 0;      // per ring stage: last load, next phase's parity
-      Tile t;
       bool ok = true;
-      for (int k = 0; ok && next_tile(k, t); ++k) {
-          if (leader) {
-          const int blocks = max(t.blocks[0], t.blocks[1]);
+      for (int k = 0; ok && next_tile(k); ++k) {
+        const Tile& t = B.tile[k % SCHED];
+        if (leader) {
           for (int w = 0; ok && w < 2; ++w) {
-            if (!t.blocks[w]) continue;
+            const RowTile& r = t.r[w];
+            if (!r.blocks) continue;
             if (q_loads[w] && !wait(smem_u32(&B.q_empty[w]), (q_loads[w] - 1) & 1, abort)) {
               ok = false;
               break;
@@ -546,27 +651,37 @@ __global__ void __launch_bounds__(THREADS, 1)
             mbar_arrive_expect_tx(bar, q_bytes);
 #pragma unroll
             for (int c = 0; c < C::PANELS; ++c)
-              tma_load_3d(sQ + w * C::Q_TILE + c * C::Q_PANEL, &tq, bar, 64 * c, t.head * p.q_head_step,
-                          t.token + w * p.tile_tokens);
+              tma_load_3d(sQ + w * C::Q_TILE + c * C::Q_PANEL, &tq, bar, 64 * c, r.head * p.q_head_step, r.token);
             ++q_loads[w];
           }
+          // block j for both row tiles, or for each that has one
           auto load = [&](bool kv, int j) -> bool {
-            const int s = loads % STAGES;
-            if (loads >= STAGES && !wait(smem_u32(&B.empty[s]), (loads / STAGES - 1) & 1, abort)) return false;
-            // V rows past the last key: warp 11 passes the block on when it has cleared them
-            const bool tail = kv && (j + 1) * BK > t.keys;
-            const uint32_t bar = smem_u32(tail ? &B.tail[s] : &B.full[s]);
-            was_tail = (was_tail & ~(1u << s)) | (tail ? 1u << s : 0u);
-            if (tail) tail_phase ^= 1u << s;
-            mbar_arrive_expect_tx(bar, C::TILE);
+            for (int w = 0; w < 2; ++w) {
+              const RowTile& r = t.r[t.shared && !t.r[0].blocks ? 1 : w];
+              const int has = t.shared ? max(t.r[0].blocks, t.r[1].blocks) : r.blocks;
+              if (j >= has) {
+                if (t.shared) break;
+                continue;
+              }
+              const int s = loads % STAGES;
+              if (loads >= STAGES && !wait(smem_u32(&B.empty[s]), (loads / STAGES - 1) & 1, abort)) return false;
+              // V rows past the last key: a softmax warp passes the block on when it has cleared them
+              const bool tail = kv && (j + 1) * BK > r.keys;
+              const uint32_t bar = smem_u32(tail ? &B.tail[s] : &B.full[s]);
+              was_tail = (was_tail & ~(1u << s)) | (tail ? 1u << s : 0u);
+              if (tail) tail_phase ^= 1u << s;
+              mbar_arrive_expect_tx(bar, C::TILE);
 #pragma unroll
-            for (int c = 0; c < C::PANELS; ++c)
-              tma_load_3d(ring + s * C::TILE + c * C::PANEL, kv ? &tv : &tk, bar, 64 * c,
-                          t.head * (kv ? p.v_head_step : p.k_head_step), t.key0 + j * BK);
-            ++loads;
+              for (int c = 0; c < C::PANELS; ++c)
+                tma_load_3d(ring + s * C::TILE + c * C::PANEL, kv ? &tv : &tk, bar, 64 * c,
+                            r.head * (kv ? p.v_head_step : p.k_head_step), r.key0 + j * BK);
+              ++loads;
+              if (t.shared) break;
+            }
             return true;
           };
           // in the order of their use: K_0, K_1, then V_j and K_{j+2}
+          const int blocks = max(t.r[0].blocks, t.r[1].blocks);
           for (int j = 0; ok && j < 2 && j < blocks; ++j) ok = load(false, j);
           for (int j = 0; ok && j < blocks; ++j) {
             ok = load(true, j);
@@ -574,6 +689,7 @@ __global__ void __launch_bounds__(THREADS, 1)
           }
         }
         ok = __all_sync(0xffffffffu, ok);
+        done_tile(k);
       }
       if (leader && *abort) {
         // leave no copy in flight
@@ -611,60 +727,77 @@ __global__ void __launch_bounds__(THREADS, 1)
           }
         };
         const bool leader = elect();
-        Tile t;
         bool ok = true;
-        for (int k = 0; ok && next_tile(k, t); ++k) {
+        for (int k = 0; ok && next_tile(k); ++k) {
+          const Tile& t = B.tile[k % SCHED];
           if (leader) {
-            const int mine = t.blocks[w], blocks = max(mine, t.blocks[w ^ 1]);
-            // S(j) from the K block just arrived, which both row tiles give back
-            auto issue_s = [&](int j) -> bool {
+            const bool shared = t.shared;
+            const int mine = t.r[w].blocks, other = t.r[w ^ 1].blocks, blocks = max(mine, other);
+            // Both row tiles see every load arrive and give its place in the ring back
+            // (else one could take a phase of a barrier for another): a shared block after
+            // its product, the other's at once.
+            auto pass = [&]() -> bool {
               if (!next_load()) return false;
-              const uint32_t bar = smem_u32(&B.empty[stage]);
-              if (j < mine) {
-                if (j == 0) {
-                  if (!wait(smem_u32(&B.q_full[w]), q_phase, abort)) return false;
-                  q_phase ^= 1;
-                }
-                // the block before is in registers
-                if (!wait(smem_u32(&B.s_free[w]), s_phase, abort)) return false;
-                s_phase ^= 1;
-                tc_fence_after();
-                const uint64_t kb = k_desc + (uint64_t)(stage * (C::TILE >> 4));
-#pragma unroll
-                for (int kk = 0; kk < D / 16; ++kk)
-                  mma_f16(S, q_desc + (((kk >> 2) * C::Q_PANEL + (kk & 3) * 32) >> 4),
-                          kb + (((kk >> 2) * C::PANEL + (kk & 3) * 32) >> 4), idesc_s, kk != 0);
-                mma_commit(smem_u32(&B.s_full[w]));
-                mma_commit(bar);
-                if (j + 1 == mine) mma_commit(smem_u32(&B.q_empty[w]));
-              } else {
-                mbar_arrive(bar);
-              }
+              mbar_arrive(smem_u32(&B.empty[stage]));
               advance();
               return true;
             };
-            auto issue_pv = [&](int j) -> bool {
-              if (!next_load()) return false;
-              const uint32_t bar = smem_u32(&B.empty[stage]);
-              if (j < mine) {
-                if (j == 0) {                       // O of the tile before has been read
-                  if (!wait(smem_u32(&B.o_free[w]), o_phase, abort)) return false;
-                  o_phase ^= 1;
-                }
-                if (!wait(smem_u32(&B.p_full[w]), p_phase, abort)) return false;
-                p_phase ^= 1;
-                tc_fence_after();
-                const uint64_t v = v_desc + (uint64_t)(stage * (C::TILE >> 4));
+            auto issue_s = [&](int j) -> bool {
+              if (!shared && w == 1 && j < other && !pass()) return false;
+              if (shared || j < mine) {
+                if (!next_load()) return false;
+                const uint32_t bar = smem_u32(&B.empty[stage]);
+                if (j < mine) {
+                  if (j == 0) {
+                    if (!wait(smem_u32(&B.q_full[w]), q_phase, abort)) return false;
+                    q_phase ^= 1;
+                  }
+                  // the block before is in registers
+                  if (!wait(smem_u32(&B.s_free[w]), s_phase, abort)) return false;
+                  s_phase ^= 1;
+                  tc_fence_after();
+                  const uint64_t kb = k_desc + (uint64_t)(stage * (C::TILE >> 4));
 #pragma unroll
-                for (int kk = 0; kk < BK / 16; ++kk)
-                  mma_f16_ts(O, P + kk * 8, v + (uint64_t)((kk * 16 * 128) >> 4), idesc_pv,
-                             kk == 0 ? (uint32_t)(j != 0) : 1u);
-                mma_commit(smem_u32(&B.pv_done[w]));
-                mma_commit(bar);
-              } else {
-                mbar_arrive(bar);
+                  for (int kk = 0; kk < D / 16; ++kk)
+                    mma_f16(S, q_desc + (((kk >> 2) * C::Q_PANEL + (kk & 3) * 32) >> 4),
+                            kb + (((kk >> 2) * C::PANEL + (kk & 3) * 32) >> 4), idesc_s, kk != 0);
+                  mma_commit(smem_u32(&B.s_full[w]));
+                  mma_commit(bar);
+                  if (j + 1 == mine) mma_commit(smem_u32(&B.q_empty[w]));
+                } else {
+                  mbar_arrive(bar);
+                }
+                advance();
               }
-              advance();
+              if (!shared && w == 0 && j < other && !pass()) return false;
+              return true;
+            };
+            auto issue_pv = [&](int j) -> bool {
+              if (!shared && w == 1 && j < other && !pass()) return false;
+              if (shared || j < mine) {
+                if (!next_load()) return false;
+                const uint32_t bar = smem_u32(&B.empty[stage]);
+                if (j < mine) {
+                  if (j == 0) {                       // O of the tile before has been read
+                    if (!wait(smem_u32(&B.o_free[w]), o_phase, abort)) return false;
+                    o_phase ^= 1;
+                  }
+                  if (!wait(smem_u32(&B.p_full[w]), p_phase, abort)) return false;
+                  p_phase ^= 1;
+                  tc_fence_after();
+                  const uint64_t v = v_desc + (uint64_t)(stage * (C::TILE >> 4));
+#pragma unroll
+                  for (int kk = 0; kk < BK / 16; ++kk)
+                    mma_f16_ts(O, P + kk * 8, v + (uint64_t)((kk * 16 * 128) >> 4), idesc_pv,
+                               kk == 0 ? (uint32_t)(j != 0) : 1u);
+                  mma_commit(smem_u32(&B.pv_done[w]));
+                  mma_commit(bar);
+                } else {
+                  mbar_arrive(bar);
+                }
+                advance();
+              }
+              if (!shared && w == 0 && j < other && !pass()) return false;
               return true;
             };
             for (int j = 0; ok && j < 2 && j < blocks; ++j) ok = issue_s(j);
@@ -674,6 +807,7 @@ __global__ void __launch_bounds__(THREADS, 1)
             }
           }
           ok = __all_sync(0xffffffffu, ok);
+          done_tile(k);
         }
         if (leader && *abort) {
           int none = 0;
@@ -696,14 +830,57 @@ __global__ void __launch_bounds__(THREADS, 1)
     const int head_in = row - token * p.group;
     const bool real = token < p.tile_tokens;
     const float c = d.scale * LOG2E;
+    uint8_t* staged = smem_raw + (base - smem_u32(smem_raw)) + C::OUT + warp * C::OUT_WARP;
     int n_s = 0;                                     // blocks so far: S, P and PV each
-    Tile t;
-    for (int k = 0; next_tile(k, t); ++k) {
-      const int at = w * p.tile_tokens + token;       // of the tile's tokens
-      const bool store = real && at < t.tokens;
-      const int blocks = t.blocks[w];
-      const int limit = d.causal ? t.seen + at : t.keys;                           // keys this row sees
-      const int least = d.causal ? t.seen + w * p.tile_tokens : t.keys;            // and the tile's first row
+    int loads = 0;                                   // ring loads of the tiles before
+    uint32_t tails = 0;                              // per place of the ring: the next tail's phase
+    for (int k = 0; next_tile(k); ++k) {
+      const Tile& t = B.tile[k % SCHED];
+      const RowTile& r_t = t.r[w];
+      const int splits = t.splits;
+      // of a split row tile both groups of softmax warps join, half of the outputs each
+      const RowTile& o_t = t.r[splits > 1 ? 0 : w];
+      const bool store = real && token < o_t.tokens;
+      const int blocks = r_t.blocks;
+      const int limit = d.causal ? r_t.seen + token : r_t.keys;      // keys this row sees
+      const int least = d.causal ? r_t.seen : r_t.keys;              // and the tile's first row
+      // V blocks with rows past the last key: their places in the ring, and the phases
+      // of those places' barriers, counted by every warp over all of them
+      int tail_stage = 0;
+      uint32_t tail_phase = 0;
+      bool tail = false;
+      {
+        const int b0 = t.r[0].blocks, b1 = t.r[1].blocks, most = max(b0, b1);
+        int at[2];                 // of the row tiles' last V blocks, or -1
+        if (t.shared) {
+          at[0] = most && most * BK > r_t.keys ? 2 * most - 1 : -1;
+          at[1] = -1;
+          tail = at[0] >= 0 && w == (b0 == most ? 0 : 1);
+        } else {
+#pragma unroll
+          for (int v = 0; v < 2; ++v) {
+            const int j = (v ? b1 : b0) - 1;
+            at[v] = j >= 0 && (j + 1) * BK > t.r[v].keys
+                        ? min(b0, 2) + min(b1, 2) + min(b0, j) + min(b1, j) + min(max(b0 - 2, 0), j) +
+                              min(max(b1 - 2, 0), j) + (v && j < b0 ? 1 : 0)
+                        : -1;
+          }
+          tail = at[w] >= 0;
+        }
+        const bool swap = at[1] >= 0 && at[1] < at[0];
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {          // in the order of the loads
+          const int v = swap ? u ^ 1 : u;
+          if (at[v] >= 0) {
+            const int st = (loads + at[v]) % STAGES;
+            if (t.shared || v == w) {
+              tail_stage = st;
+              tail_phase = (tails >> st) & 1;
+            }
+            tails ^= 1u << st;
+          }
+        }
+      }
       float m = -INFINITY, l = 0.f;
       bool ok = true;
       for (int j = 0; j < blocks; ++j) {
@@ -776,39 +953,151 @@ __global__ void __launch_bounds__(THREADS, 1)
         unpack2(add2(add2(l4[0], l4[1]), add2(l4[2], l4[3])), a, b);
         l += a + b;
         ++n_s;
+        // the last block's V, cleared by one warp (of the first row tile that uses it)
+        if (tail && j + 1 == blocks && (warp & 3) == 3) {
+          ok = __all_sync(0xffffffffu, wait(smem_u32(&B.tail[tail_stage]), tail_phase, abort));
+          if (!ok) break;
+          uint8_t* v = smem_raw + (ring + tail_stage * C::TILE - smem_u32(smem_raw));
+          // whole 128-byte rows of each panel: the swizzle permutes within a row
+          for (int i = (r_t.keys - j * BK) * 8 + lane; i < BK * 8; i += 32)
+#pragma unroll
+            for (int c = 0; c < C::PANELS; ++c)
+              *reinterpret_cast<uint4*>(v + c * C::PANEL + i * 16) = make_uint4(0, 0, 0, 0);
+          fence_proxy_async();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(smem_u32(&B.full[tail_stage]));
+        }
       }
+      loads += t.shared ? 2 * max(t.r[0].blocks, t.r[1].blocks) : 2 * (t.r[0].blocks + t.r[1].blocks);
       if (!ok) break;
-      const long long tok = (long long)t.token + at;
-      const int head = t.head * p.group + head_in;
+      const long long tok = (long long)o_t.token + token;
+      const int head = o_t.head * p.group + head_in;
+      const int unit = t.unit, split = t.split;
+      done_tile(k);
       T* out = static_cast<T*>(d.out) + tok * d.out_stride[0] + head * d.out_stride[1];
+      // 64 outputs of the warp's 32 rows: every lane's own row to shared memory, then
+      // eight lanes a row from there (a row at a time from one lane, a store would
+      // touch 32 rows: 4,600 cycles a tile against 1,300)
+      const uint32_t keep = __ballot_sync(0xffffffffu, store);
+      auto store_rows = [&](int i, const uint32_t (&v)[32]) {
+        uint8_t* mine = staged + lane * C::OUT_ROW;
+#pragma unroll
+        for (int x = 0; x < 8; ++x)
+          *reinterpret_cast<uint4*>(mine + 16 * x) = make_uint4(v[4 * x], v[4 * x + 1], v[4 * x + 2], v[4 * x + 3]);
+        __syncwarp();
+#pragma unroll
+        for (int x = 0; x < 8; ++x) {
+          const int from = 4 * x + (lane >> 3);
+          T* to = reinterpret_cast<T*>(__shfl_sync(0xffffffffu, reinterpret_cast<unsigned long long>(out), from));
+          if ((keep >> from) & 1)
+            *reinterpret_cast<uint4*>(to + i + 8 * (lane & 7)) =
+                *reinterpret_cast<const uint4*>(staged + from * C::OUT_ROW + 16 * (lane & 7));
+        }
+        __syncwarp();
+      };
       if (blocks) {
         // every PV of this row tile is complete
         if (!__all_sync(0xffffffffu, wait(smem_u32(&B.pv_done[w]), (n_s - 1) & 1, abort))) break;
         tc_fence_after();
-        const float inv = l == 0.f ? 0.f : 1.f / l;
+      }
+      if (splits > 1) {
+        // this stretch's O [dim][row], m and l; the last CTA of the row tile joins them
+        if (w == 0) {
+          float* part = p.parts + (long long)(unit * splits + split) * PART_FLOATS;
+          if (blocks) {
 #pragma unroll 1
-        for (int i = 0; i < D; i += 32) {
-          uint32_t r[32];
-          tmem_ld32_wait(O + i, r);
-          if (store) {
+            for (int i = 0; i < D; i += 32) {
+              uint32_t r[32];
+              tmem_ld32_wait(O + i, r);
 #pragma unroll
-            for (int x = 0; x < 32; x += 8) {
-              uint32_t v[4];
-#pragma unroll
-              for (int y = 0; y < 4; ++y)
-                v[y] = l == 0.f ? 0u
-                                : Elem<T>::from2(__uint_as_float(r[x + 2 * y]) * inv,
-                                                 __uint_as_float(r[x + 2 * y + 1]) * inv);
-              *reinterpret_cast<uint4*>(out + i + x) = make_uint4(v[0], v[1], v[2], v[3]);
+              for (int x = 0; x < 32; ++x) part[(i + x) * BQ + row] = __uint_as_float(r[x]);
             }
           }
+          reinterpret_cast<float2*>(part + 128 * BQ)[row] = make_float2(m, l);
+          __threadfence();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(smem_u32(&B.part_in));
+          if (!__all_sync(0xffffffffu, wait(smem_u32(&B.part_in), 0, abort))) break;
+          if (tid == 0) {
+            B.last = atomicAdd(p.counters + unit, 1) == splits - 1;
+            if (B.last) p.counters[unit] = 0;
+            __threadfence();
+            mbar_arrive(smem_u32(&B.part_out));
+          }
         }
-        tc_fence_before();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(smem_u32(&B.o_free[w]));
-      } else if (store) {
+        if (!__all_sync(0xffffffffu, wait(smem_u32(&B.part_out), 0, abort))) break;
+        if (!B.last) continue;
+        const float* all = p.parts + (long long)unit * splits * PART_FLOATS;
+        auto ml_of = [&](int q) -> float2 {
+          return __ldcg(reinterpret_cast<const float2*>(all + (long long)q * PART_FLOATS + 128 * BQ) + row);
+        };
+        float top = -INFINITY, sum = 0.f;
+        for (int q = 0; q < splits; ++q) top = fmaxf(top, ml_of(q).x);
+        const float sub = top == -INFINITY ? 0.f : top;
+        for (int q = 0; q < splits; ++q) {
+          const float2 ml = ml_of(q);
+          sum += ml.y * ex2(ml.x - sub);
+        }
+        const float inv = sum == 0.f ? 0.f : 1.f / sum;
+        constexpr int EACH = D / 2;                    // outputs per group
+        uint32_t v[32];
 #pragma unroll
-        for (int i = 0; i < D; i += 8) *reinterpret_cast<uint4*>(out + i) = make_uint4(0, 0, 0, 0);
+        for (int i = 0; i < EACH; i += 32) {
+          float o[32];
+#pragma unroll
+          for (int x = 0; x < 32; ++x) o[x] = 0.f;
+#pragma unroll 1
+          for (int q = 0; q < splits; q += 4) {        // four parts on their way at once
+            float f[4], y[4][32];
+#pragma unroll
+            for (int u = 0; u < 4; ++u) {
+              const float mq = q + u < splits ? ml_of(q + u).x : -INFINITY;
+              f[u] = ex2(mq - sub) * inv;
+              const float* from = all + (long long)(q + u) * PART_FLOATS + (w * EACH + i) * BQ + row;
+#pragma unroll
+              for (int x = 0; x < 32; ++x)
+                y[u][x] = mq == -INFINITY ? 0.f : __ldcg(from + x * BQ);     // nothing seen, perhaps nothing written
+            }
+#pragma unroll
+            for (int u = 0; u < 4; ++u)
+#pragma unroll
+              for (int x = 0; x < 32; ++x) o[x] += f[u] * y[u][x];
+          }
+#pragma unroll
+          for (int x = 0; x < 16; ++x) v[(i & 32) / 2 + x] = Elem<T>::from2(o[2 * x], o[2 * x + 1]);
+        }
+        if constexpr (EACH == 64) {
+          store_rows(w * 64, v);
+        } else if (store) {
+#pragma unroll
+          for (int x = 0; x < 16; x += 4)
+            *reinterpret_cast<uint4*>(out + w * 32 + 2 * x) = make_uint4(v[x], v[x + 1], v[x + 2], v[x + 3]);
+        }
+        if (store && d.lse && w == 0) d.lse[tok * d.heads + head] = sum == 0.f ? -INFINITY : (top + log2f(sum)) * LN2;
+        continue;
+      }
+      if (blocks) {
+        const float inv = l == 0.f ? 0.f : 1.f / l;
+#pragma unroll 1
+        for (int i = 0; i < D; i += 64) {
+          uint32_t r[64], v[32];
+          tmem_ld64_wait(O + i, r);
+#pragma unroll
+          for (int x = 0; x < 32; ++x)
+            v[x] = l == 0.f ? 0u
+                            : Elem<T>::from2(__uint_as_float(r[2 * x]) * inv, __uint_as_float(r[2 * x + 1]) * inv);
+          if (i + 64 == D) {
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(smem_u32(&B.o_free[w]));
+          }
+          store_rows(i, v);
+        }
+      } else if (keep) {
+        uint32_t v[32];
+#pragma unroll
+        for (int x = 0; x < 32; ++x) v[x] = 0u;
+        for (int i = 0; i < D; i += 64) store_rows(i, v);
       }
       if (store && d.lse) d.lse[tok * d.heads + head] = l == 0.f ? -INFINITY : (m + log2f(l)) * LN2;
     }
@@ -886,6 +1175,8 @@ int launch(const CUtensorMap& tq, const CUtensorMap& tk, const CUtensorMap& tv, 
 
 }  // namespace
 
+extern "C" int64_t ktir_prompt_attention_workspace(void) { return PARTS_BYTES + MAX_PARTS * 4; }
+
 extern "C" int ktir_prompt_attention(const KtirPromptDesc* d, void* stream) {
   if (!d) return ktir_set_error(KTIR_ERR_ARG, "ktir_prompt_attention: null argument");
   if (d->tokens == 0) return KTIR_OK;
@@ -907,7 +1198,7 @@ extern "C" int ktir_prompt_attention(const KtirPromptDesc* d, void* stream) {
   const int64_t qe[2] = {d->tokens, d->heads}, ke[2] = {d->kv_tokens, d->kv_heads};
   if (!vector_strides(d->q_stride, qe, 2) || !vector_strides(d->out_stride, qe, 2) ||
       !vector_strides(d->k_stride, ke, 2) || !vector_strides(d->v_stride, ke, 2) || !aligned16(d->q) ||
-      !aligned16(d->k) || !aligned16(d->v) || !aligned16(d->out))
+      !aligned16(d->k) || !aligned16(d->v) || !aligned16(d->out) || !aligned16(d->workspace))
     return ktir_set_error(KTIR_ERR_UNSUPPORTED,
                           "ktir_prompt_attention: head vectors must start on 16-byte boundaries");
   const bool bf16 = d->dtype == KTIR_BF16;
@@ -929,10 +1220,15 @@ extern "C" int ktir_prompt_attention(const KtirPromptDesc* d, void* stream) {
     return ktir_set_error(KTIR_ERR_UNSUPPORTED, "ktir_prompt_attention: strides that a tensor map does not take");
   const int sms = sm_count();
   if (sms < 1) return ktir_set_error(KTIR_ERR_CUDA, "ktir_prompt_attention: no usable current device");
-  // at most this many tiles: every sequence may end in a part of one
-  const long long tiles = (d->tokens / (2 * p.tile_tokens) + d->batch) * d->kv_heads;
-  if (tiles > 0x7fffffffLL) return ktir_set_error(KTIR_ERR_UNSUPPORTED, "ktir_prompt_attention: too many tiles");
-  const unsigned grid = (unsigned)(tiles < sms ? tiles : sms);
+  // at most this many row tiles: every sequence may end in a part of one
+  const long long tiles = (d->tokens / p.tile_tokens + d->batch) * d->kv_heads;
+  if (tiles > 0x3fffffffLL) return ktir_set_error(KTIR_ERR_UNSUPPORTED, "ktir_prompt_attention: too many tiles");
+  p.token_magic = (uint32_t)(((1ULL << 32) + p.tile_tokens - 1) / p.tile_tokens - (p.tile_tokens == 1));
+  p.pair_magic = (uint32_t)(((1ULL << 32) + 2 * p.tile_tokens - 1) / (2 * p.tile_tokens));
+  p.parts = d->workspace && d->workspace_bytes >= ktir_prompt_attention_workspace() ? static_cast<float*>(d->workspace) : nullptr;
+  p.counters = reinterpret_cast<int*>(static_cast<char*>(d->workspace) + PARTS_BYTES);
+  // with a workspace the SMs left over share the keys, if there are enough of them
+  const unsigned grid = (unsigned)(tiles < sms && !(p.parts && d->kv_tokens > 4 * block) ? tiles : sms);
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   if (d->dim == 64)
     return bf16 ? launch<__nv_bfloat16, 64>(tq, tk, tv, p, grid, s) : launch<__half, 64>(tq, tk, tv, p, grid, s);

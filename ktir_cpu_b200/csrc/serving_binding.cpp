@@ -26,7 +26,8 @@ namespace {
 
 constexpr int MAX_DEVICES = 64;
 at::Tensor g_status[MAX_DEVICES];                                  // touched under the GIL only
-std::map<std::pair<int, cudaStream_t>, at::Tensor> g_workspace;
+using Key = std::pair<int, cudaStream_t>;
+std::map<Key, at::Tensor> g_decode, g_prompt;                      // workspaces by device and stream
 
 struct Failed {};   // a Python exception is set
 
@@ -48,10 +49,10 @@ int32_t* status_of(int dev) {
 // Zeroed scratch for calls on one stream, kept between them: calls on one stream
 // follow each other.  A call that is being captured gets its own, cleared inside
 // the graph, which may be replayed on any stream.
-at::Tensor workspace_of(int dev, cudaStream_t stream, int64_t bytes) {
+at::Tensor workspace_of(std::map<Key, at::Tensor>& kept, int dev, cudaStream_t stream, int64_t bytes) {
   const auto options = at::TensorOptions().dtype(at::kByte).device(at::kCUDA, dev);
   if (capturing()) return at::zeros({bytes}, options);
-  at::Tensor& t = g_workspace[{dev, stream}];
+  at::Tensor& t = kept[{dev, stream}];
   if (!t.defined() || t.numel() < bytes) t = at::zeros({bytes + bytes / 4}, options);
   return t;
 }
@@ -224,7 +225,7 @@ PyObject* paged_decode(PyObject* const* a) {
     d.kv_heads = (int32_t)kc->size(2);
     d.dim = (int32_t)q->size(2);
     const at::Tensor ws =
-        workspace_of(dev, stream, ktir_paged_decode_workspace(d.batch, d.heads, d.kv_heads, d.dim));
+        workspace_of(g_decode, dev, stream, ktir_paged_decode_workspace(d.batch, d.heads, d.kv_heads, d.dim));
     d.q = q->data_ptr();
     d.k_cache = kc->data_ptr();
     d.v_cache = vc->data_ptr();
@@ -275,7 +276,12 @@ PyObject* prompt_attention(PyObject* const* a) {
     if (lse.defined()) d.lse = lse.data_ptr<float>();
     d.offsets = offsets->data_ptr<int32_t>();
     d.kv_offsets = kv_offsets ? kv_offsets->data_ptr<int32_t>() : d.offsets;
-    d.status = status_of(q->get_device());
+    const int dev = q->get_device();
+    const cudaStream_t stream = c10::cuda::getCurrentCUDAStream(dev).stream();
+    const at::Tensor ws = workspace_of(g_prompt, dev, stream, ktir_prompt_attention_workspace());
+    d.workspace = ws.data_ptr();
+    d.workspace_bytes = ws.numel();
+    d.status = status_of(dev);
     d.batch = offsets->size(0) - 1;
     d.kv_tokens = k->size(0);
     strides(d.q_stride, *q);
@@ -287,7 +293,7 @@ PyObject* prompt_attention(PyObject* const* a) {
     d.dtype = dt;
     d.scale = scale_of(a[6], q->size(2));
     d.causal = flag(a[5]);
-    check(ktir_prompt_attention(&d, c10::cuda::getCurrentCUDAStream(q->get_device()).stream()));
+    check(ktir_prompt_attention(&d, stream));
   }
   return result(a[7], o, lse);
 }

@@ -168,7 +168,8 @@ class KtirPagedDecodeDesc(C.Structure):
 class KtirPromptDesc(C.Structure):
     _fields_ = [("q", C.c_void_p), ("k", C.c_void_p), ("v", C.c_void_p), ("out", C.c_void_p),
                 ("lse", C.c_void_p), ("offsets", C.c_void_p), ("kv_offsets", C.c_void_p),
-                ("status", C.c_void_p), ("batch", C.c_int64), ("tokens", C.c_int64),
+                ("status", C.c_void_p), ("workspace", C.c_void_p), ("workspace_bytes", C.c_int64),
+                ("batch", C.c_int64), ("tokens", C.c_int64),
                 ("kv_tokens", C.c_int64), ("q_stride", C.c_int64 * 2),
                 ("k_stride", C.c_int64 * 2), ("v_stride", C.c_int64 * 2),
                 ("out_stride", C.c_int64 * 2), ("heads", C.c_int32), ("kv_heads", C.c_int32),
@@ -245,6 +246,8 @@ def load_library(build_if_missing: bool = False) -> C.CDLL:
     lib.ktir_paged_decode.argtypes = [C.POINTER(KtirPagedDecodeDesc), vp]
     lib.ktir_paged_decode_workspace.argtypes = [C.c_int64, C.c_int32, C.c_int32, C.c_int32]
     lib.ktir_paged_decode_workspace.restype = C.c_int64
+    lib.ktir_prompt_attention_workspace.argtypes = []
+    lib.ktir_prompt_attention_workspace.restype = C.c_int64
     lib.ktir_prompt_attention.argtypes = [C.POINTER(KtirPromptDesc), vp]
     for name in EXPORTS:
         getattr(lib, name).restype = C.c_int if name != "ktir_last_error" else C.c_char_p

@@ -302,6 +302,44 @@ def test_prompt(typ, new, keys, heads, kv_heads, dim, causal):
     _check_prompt(typ, q, k, v, offsets, kv_offsets, causal, dim ** -0.5, out, lse)
 
 
+@pytest.mark.parametrize("typ,new,keys,heads,kv_heads,dim,causal", [
+    ("bf16", [64], [8192], 32, 8, 128, True),
+    ("f16", [16] * 4, [5000] * 4, 8, 2, 64, True),
+    ("bf16", [3, 70, 0, 1], [3000, 2001, 50, 4096], 6, 2, 128, True),
+    ("f16", [40, 100], [6000, 30], 4, 4, 128, False),
+    ("bf16", [200], [40], 2, 1, 64, True),
+    ("bf16", [1, 1], [20000, 7], 16, 1, 128, True),
+])
+def test_prompt_few_queries_over_many_keys(typ, new, keys, heads, kv_heads, dim, causal):
+    """The keys of a few queries are shared among the SMs; the same result every time."""
+    import torch
+    from ktir_cpu_b200 import check_status, prompt_attention
+    q, k, v, offsets, kv_offsets = _prompt_inputs(typ, new, keys, heads, kv_heads, dim, seed=sum(keys))
+    out, lse = prompt_attention(q, k, v, offsets, kv_offsets=kv_offsets, causal=causal, return_lse=True)
+    _check_prompt(typ, q, k, v, offsets, kv_offsets, causal, dim ** -0.5, out, lse)
+    for _ in range(50):
+        again, lse2 = prompt_attention(q, k, v, offsets, kv_offsets=kv_offsets, causal=causal, return_lse=True)
+        assert torch.equal(again, out) and torch.equal(lse2, lse)
+    check_status()
+
+
+def test_prompt_mixed_calls_in_turn():
+    """Calls that split keys, take row tiles singly and in pairs, one after the other."""
+    import torch
+    from ktir_cpu_b200 import check_status, prompt_attention
+    calls = []
+    for i, (new, keys) in enumerate([([64], [4000]), ([30] * 100, [30] * 100), ([700] * 9, [700] * 9), ([5], [900]),
+                                     ([81, 33, 300] * 5, [400] * 15)]):
+        q, k, v, offsets, kv_offsets = _prompt_inputs("bf16", new, keys, 8, 2, 128, seed=30 + i)
+        first, lse = prompt_attention(q, k, v, offsets, kv_offsets=kv_offsets, return_lse=True)
+        _check_prompt("bf16", q, k, v, offsets, kv_offsets, True, 128 ** -0.5, first, lse)
+        calls.append((q, k, v, offsets, kv_offsets, first))
+    for _ in range(20):
+        outs = [prompt_attention(*c[:4], kv_offsets=c[4]) for c in calls]
+        assert all(torch.equal(o, c[5]) for o, c in zip(outs, calls))
+    check_status()
+
+
 def test_prompt_many_short():
     from ktir_cpu_b200 import check_status, prompt_attention
     rng = random.Random(8)
