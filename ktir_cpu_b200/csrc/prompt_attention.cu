@@ -397,9 +397,12 @@ struct Order {
     }
     __syncwarp();
   }
-  // tile number `x`, not below the last one found: its sequence and place there
-  __device__ void find(int x, long long& b_out, int& i_out) {
-    if (table) {
+  // tile number `x`, not below the last one found: its sequence and place there.
+  // With a tile for every CTA their order does not matter (`any`): by sequence, then.
+  __device__ void find(int x, bool any, long long& b_out, int& i_out) {
+    if (any) {
+      weight = above = 0;
+    } else if (table) {
       while (weight > 0 && table[weight] <= x) above = table[weight--];
     } else {
       int hi = weight + 1, hi_count = above;   // count(hi) <= x
@@ -433,9 +436,9 @@ struct Order {
       int first = 0, mine = 0;
       if (b < p.d.batch) {
         const Seq s = seq(b);
-        const int all = heavier(s, lo);
-        mine = all - heavier(s, lo + 1);
-        first = divide(s.n + T - 1) - all;
+        const int tiles = divide(s.n + T - 1), all = any ? tiles : heavier(s, lo);
+        mine = any ? tiles : all - heavier(s, lo + 1);
+        first = tiles - all;
       }
       int incl = mine;
 #pragma unroll
@@ -599,7 +602,7 @@ __global__ void __launch_bounds__(THREADS, 1)
             if ((parts && (w || x >= all)) || y >= (singly ? rows : twos)) break;
             long long b;
             int i;
-            order.find((int)(y / d.kv_heads), b, i);
+            order.find((int)(y / d.kv_heads), parts, b, i);
             if (lane == 0 && b >= 0) {
               const int head = (int)(y % d.kv_heads);
               const Seq q = order.seq(b);
