@@ -734,80 +734,84 @@ __global__ void __launch_bounds__(THREADS, 1)
         for (int k = 0; ok && next_tile(k); ++k) {
           const Tile& t = B.tile[k % SCHED];
           if (leader) {
-            const bool shared = t.shared;
             const int mine = t.r[w].blocks, other = t.r[w ^ 1].blocks, blocks = max(mine, other);
-            // Both row tiles see every load arrive and give its place in the ring back
-            // (else one could take a phase of a barrier for another): a shared block after
-            // its product, the other's at once.
-            auto pass = [&]() -> bool {
-              if (!next_load()) return false;
-              mbar_arrive(smem_u32(&B.empty[stage]));
-              advance();
-              return true;
-            };
-            auto issue_s = [&](int j) -> bool {
-              if (!shared && w == 1 && j < other && !pass()) return false;
-              if (shared || j < mine) {
+            auto run = [&](auto SHARED) {       // the two apart: the loop of one is short
+              constexpr bool shared = decltype(SHARED)::value;
+              // Both row tiles see every load arrive and give its place in the ring back
+              // (else one could take a phase of a barrier for another): a shared block after
+              // its product, the other's at once.
+              auto pass = [&]() -> bool {
                 if (!next_load()) return false;
-                const uint32_t bar = smem_u32(&B.empty[stage]);
-                if (j < mine) {
-                  if (j == 0) {
-                    if (!wait(smem_u32(&B.q_full[w]), q_phase, abort)) return false;
-                    q_phase ^= 1;
-                  }
-                  // the block before is in registers
-                  if (!wait(smem_u32(&B.s_free[w]), s_phase, abort)) return false;
-                  s_phase ^= 1;
-                  tc_fence_after();
-                  const uint64_t kb = k_desc + (uint64_t)(stage * (C::TILE >> 4));
-#pragma unroll
-                  for (int kk = 0; kk < D / 16; ++kk)
-                    mma_f16(S, q_desc + (((kk >> 2) * C::Q_PANEL + (kk & 3) * 32) >> 4),
-                            kb + (((kk >> 2) * C::PANEL + (kk & 3) * 32) >> 4), idesc_s, kk != 0);
-                  mma_commit(smem_u32(&B.s_full[w]));
-                  mma_commit(bar);
-                  if (j + 1 == mine) mma_commit(smem_u32(&B.q_empty[w]));
-                } else {
-                  mbar_arrive(bar);
-                }
+                mbar_arrive(smem_u32(&B.empty[stage]));
                 advance();
-              }
-              if (!shared && w == 0 && j < other && !pass()) return false;
-              return true;
-            };
-            auto issue_pv = [&](int j) -> bool {
-              if (!shared && w == 1 && j < other && !pass()) return false;
-              if (shared || j < mine) {
-                if (!next_load()) return false;
-                const uint32_t bar = smem_u32(&B.empty[stage]);
-                if (j < mine) {
-                  if (j == 0) {                       // O of the tile before has been read
-                    if (!wait(smem_u32(&B.o_free[w]), o_phase, abort)) return false;
-                    o_phase ^= 1;
-                  }
-                  if (!wait(smem_u32(&B.p_full[w]), p_phase, abort)) return false;
-                  p_phase ^= 1;
-                  tc_fence_after();
-                  const uint64_t v = v_desc + (uint64_t)(stage * (C::TILE >> 4));
+                return true;
+              };
+              auto issue_s = [&](int j) -> bool {
+                if (!shared && w == 1 && j < other && !pass()) return false;
+                if (shared || j < mine) {
+                  if (!next_load()) return false;
+                  const uint32_t bar = smem_u32(&B.empty[stage]);
+                  if (j < mine) {
+                    if (j == 0) {
+                      if (!wait(smem_u32(&B.q_full[w]), q_phase, abort)) return false;
+                      q_phase ^= 1;
+                    }
+                    // the block before is in registers
+                    if (!wait(smem_u32(&B.s_free[w]), s_phase, abort)) return false;
+                    s_phase ^= 1;
+                    tc_fence_after();
+                    const uint64_t kb = k_desc + (uint64_t)(stage * (C::TILE >> 4));
 #pragma unroll
-                  for (int kk = 0; kk < BK / 16; ++kk)
-                    mma_f16_ts(O, P + kk * 8, v + (uint64_t)((kk * 16 * 128) >> 4), idesc_pv,
-                               kk == 0 ? (uint32_t)(j != 0) : 1u);
-                  mma_commit(smem_u32(&B.pv_done[w]));
-                  mma_commit(bar);
-                } else {
-                  mbar_arrive(bar);
+                    for (int kk = 0; kk < D / 16; ++kk)
+                      mma_f16(S, q_desc + (((kk >> 2) * C::Q_PANEL + (kk & 3) * 32) >> 4),
+                              kb + (((kk >> 2) * C::PANEL + (kk & 3) * 32) >> 4), idesc_s, kk != 0);
+                    mma_commit(smem_u32(&B.s_full[w]));
+                    mma_commit(bar);
+                    if (j + 1 == mine) mma_commit(smem_u32(&B.q_empty[w]));
+                  } else {
+                    mbar_arrive(bar);
+                  }
+                  advance();
                 }
-                advance();
+                if (!shared && w == 0 && j < other && !pass()) return false;
+                return true;
+              };
+              auto issue_pv = [&](int j) -> bool {
+                if (!shared && w == 1 && j < other && !pass()) return false;
+                if (shared || j < mine) {
+                  if (!next_load()) return false;
+                  const uint32_t bar = smem_u32(&B.empty[stage]);
+                  if (j < mine) {
+                    if (j == 0) {                       // O of the tile before has been read
+                      if (!wait(smem_u32(&B.o_free[w]), o_phase, abort)) return false;
+                      o_phase ^= 1;
+                    }
+                    if (!wait(smem_u32(&B.p_full[w]), p_phase, abort)) return false;
+                    p_phase ^= 1;
+                    tc_fence_after();
+                    const uint64_t v = v_desc + (uint64_t)(stage * (C::TILE >> 4));
+#pragma unroll
+                    for (int kk = 0; kk < BK / 16; ++kk)
+                      mma_f16_ts(O, P + kk * 8, v + (uint64_t)((kk * 16 * 128) >> 4), idesc_pv,
+                                 kk == 0 ? (uint32_t)(j != 0) : 1u);
+                    mma_commit(smem_u32(&B.pv_done[w]));
+                    mma_commit(bar);
+                  } else {
+                    mbar_arrive(bar);
+                  }
+                  advance();
+                }
+                if (!shared && w == 0 && j < other && !pass()) return false;
+                return true;
+              };
+              for (int j = 0; ok && j < 2 && j < blocks; ++j) ok = issue_s(j);
+              for (int j = 0; ok && j < blocks; ++j) {
+                ok = issue_pv(j);
+                if (ok && j + 2 < blocks) ok = issue_s(j + 2);
               }
-              if (!shared && w == 0 && j < other && !pass()) return false;
-              return true;
             };
-            for (int j = 0; ok && j < 2 && j < blocks; ++j) ok = issue_s(j);
-            for (int j = 0; ok && j < blocks; ++j) {
-              ok = issue_pv(j);
-              if (ok && j + 2 < blocks) ok = issue_s(j + 2);
-            }
+            if (t.shared) run(std::true_type());
+            else run(std::false_type());
           }
           ok = __all_sync(0xffffffffu, ok);
           done_tile(k);
@@ -956,20 +960,20 @@ __global__ void __launch_bounds__(THREADS, 1)
         unpack2(add2(add2(l4[0], l4[1]), add2(l4[2], l4[3])), a, b);
         l += a + b;
         ++n_s;
-        // the last block's V, cleared by one warp (of the first row tile that uses it)
-        if (tail && j + 1 == blocks && (warp & 3) == 3) {
-          ok = __all_sync(0xffffffffu, wait(smem_u32(&B.tail[tail_stage]), tail_phase, abort));
-          if (!ok) break;
-          uint8_t* v = smem_raw + (ring + tail_stage * C::TILE - smem_u32(smem_raw));
-          // whole 128-byte rows of each panel: the swizzle permutes within a row
-          for (int i = (r_t.keys - j * BK) * 8 + lane; i < BK * 8; i += 32)
+      }
+      // the last block's V, cleared by one warp (of the first row tile that uses it)
+      if (ok && tail && (warp & 3) == 3) {
+        ok = __all_sync(0xffffffffu, wait(smem_u32(&B.tail[tail_stage]), tail_phase, abort));
+        if (!ok) break;
+        uint8_t* v = smem_raw + (ring + tail_stage * C::TILE - smem_u32(smem_raw));
+        // whole 128-byte rows of each panel: the swizzle permutes within a row
+        for (int i = (r_t.keys - (blocks - 1) * BK) * 8 + lane; i < BK * 8; i += 32)
 #pragma unroll
-            for (int c = 0; c < C::PANELS; ++c)
-              *reinterpret_cast<uint4*>(v + c * C::PANEL + i * 16) = make_uint4(0, 0, 0, 0);
-          fence_proxy_async();
-          __syncwarp();
-          if (lane == 0) mbar_arrive(smem_u32(&B.full[tail_stage]));
-        }
+          for (int c = 0; c < C::PANELS; ++c)
+            *reinterpret_cast<uint4*>(v + c * C::PANEL + i * 16) = make_uint4(0, 0, 0, 0);
+        fence_proxy_async();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(smem_u32(&B.full[tail_stage]));
       }
       loads += t.shared ? 2 * max(t.r[0].blocks, t.r[1].blocks) : 2 * (t.r[0].blocks + t.r[1].blocks);
       if (!ok) break;
