@@ -323,6 +323,17 @@ def test_prompt_few_queries_over_many_keys(typ, new, keys, heads, kv_heads, dim,
     check_status()
 
 
+def test_prompt_many_tiles_of_many_keys():
+    """More weights of tiles than a table of them holds: some of the heads, all tokens."""
+    import torch
+    from ktir_cpu_b200 import check_status, prompt_attention
+    q, k, v, offsets, kv_offsets = _prompt_inputs("f16", [700, 9], [45000, 9], 128, 1, 64, seed=41)
+    out, lse = prompt_attention(q, k, v, offsets, kv_offsets=kv_offsets, return_lse=True)
+    check_status()
+    for h in (0, 77):
+        _check_prompt("f16", q[:, h:h + 1], k, v, offsets, kv_offsets, True, 0.125, out[:, h:h + 1], lse[:, h:h + 1])
+
+
 def test_prompt_mixed_calls_in_turn():
     """Calls that split keys, take row tiles singly and in pairs, one after the other."""
     import torch
