@@ -542,22 +542,23 @@ __global__ void __launch_bounds__(THREADS, 1)
       const int half = p.tile_tokens;
       int heaviest = 0, singles = 0, pairs = 0;
       bool any_bad = false;
+      const int ends = blockIdx.x == 0 ? d.offsets[0] | (d.offsets[d.batch] ^ (int)d.tokens) : 0;   // 0 if they cover the tokens
       for (long long b = lane; b < d.batch; b += 32) {
         bool bad;
         const Seq s = sequence(d, b, bad);
         if (b < CACHED) B.lengths[b] = make_int2(s.n, s.m);
         any_bad |= bad;
         if (s.n) heaviest = max(heaviest, (s.m + BK - 1) / BK);
-        singles += (s.n + half - 1) / half;
-        pairs += (s.n + 2 * half - 1) / (2 * half);
+        const int tiles = (int)((unsigned)(s.n + half - 1) / (unsigned)half);
+        singles += tiles;
+        pairs += (tiles + 1) / 2;
       }
       if (blockIdx.x == 0) {
-        if (lane == 0) any_bad |= d.offsets[0] != 0 || d.offsets[d.batch] != d.tokens;
-        if (any_bad) atomicOr(d.status, KTIR_STATUS_BAD_INDEX);
+        if (any_bad || (lane == 0 && ends)) atomicOr(d.status, KTIR_STATUS_BAD_INDEX);
       }
       __syncwarp();
       heaviest = (int)__reduce_max_sync(0xffffffffu, (unsigned)heaviest);
-      const long long rows = (long long)warp_sum(singles) * d.kv_heads, twos = (long long)warp_sum(pairs) * d.kv_heads;
+      const int rows = warp_sum(singles) * d.kv_heads, twos = warp_sum(pairs) * d.kv_heads;     // below 2^30
       const int G = (int)gridDim.x;
       // no more row tiles than CTAs: one each, and what is left over shares their keys.
       // A stretch costs its blocks, joining S of them about as much as S blocks.
@@ -565,7 +566,7 @@ __global__ void __launch_bounds__(THREADS, 1)
       int splits = 1;
       if (parts && rows > 0 && p.parts) {
         while (splits * splits < heaviest) ++splits;
-        splits = max(1, min(splits, (int)(min(G, MAX_PARTS) / rows)));
+        splits = max(1, min(splits, min(G, MAX_PARTS) / rows));
       }
       // Singles where a CTA has few row tiles, each then next to one of another weight
       // (7 pieces of prompts, 195 row tiles: 43 us against 55 in pairs), or where pairs
@@ -573,7 +574,7 @@ __global__ void __launch_bounds__(THREADS, 1)
       // against 67).  Else pairs: their shared blocks save L2 traffic (8192 tokens: 477
       // us against 573).
       const bool singly = parts || rows <= 2 * G || 2 * twos - rows > (2 * twos) / 3;
-      const long long all = parts ? rows * splits : singly ? (rows + 1) / 2 : twos;
+      const int all = parts ? rows * splits : singly ? (rows + 1) / 2 : twos;
       Order<BK> order = {p, B.lengths, lane, singly ? half : 2 * half, singly ? p.token_magic : p.pair_magic, heaviest, 0, nullptr};
 
       for (int next = 0;; ++next) {
@@ -583,11 +584,11 @@ __global__ void __launch_bounds__(THREADS, 1)
           break;
         // rounds of G (two of them at once for singles), back and forth: a heavy one here
         // is followed by a light one
-        const long long x = (long long)next * G + ((next & 1) ? G - 1 - blockIdx.x : blockIdx.x);
-        const long long first = parts ? x : singly ? 2LL * next * G + blockIdx.x : x;
+        const int x = next * G + ((next & 1) ? G - 1 - blockIdx.x : blockIdx.x);
+        const int first = !parts && singly ? 2 * next * G + blockIdx.x : x;
         Tile& t = B.tile[s];
         // a CTA may have a tile in the last round after having none before it
-        const bool stop = (long long)next * G >= all;
+        const bool stop = next * G >= all;
         if (lane == 0) {
           t.stop = stop;
           t.shared = !singly;
@@ -598,21 +599,22 @@ __global__ void __launch_bounds__(THREADS, 1)
         __syncwarp();
         if (!stop) {
           for (int w = 0; w < 2; ++w) {
-            const long long y = parts ? x / splits : singly && w ? first + 2 * (G - 1 - blockIdx.x) + 1 : first;
+            const int y = parts ? x / splits : singly && w ? first + 2 * (G - 1 - blockIdx.x) + 1 : first;
             if ((parts && (w || x >= all)) || y >= (singly ? rows : twos)) break;
             long long b;
             int i;
-            order.find((int)(y / d.kv_heads), parts, b, i);
+            const int index = (int)((unsigned)y / (unsigned)d.kv_heads);
+            order.find(index, parts, b, i);
             if (lane == 0 && b >= 0) {
-              const int head = (int)(y % d.kv_heads);
+              const int head = y - index * d.kv_heads;
               const Seq q = order.seq(b);
               row_tile<BK>(p, b, q, i * order.T, head, t.r[w]);
               if (!singly) row_tile<BK>(p, b, q, i * order.T + half, head, t.r[1]);
               if (splits > 1) {               // this CTA's stretch of the keys
                 RowTile& r = t.r[0];
                 t.splits = splits;
-                t.split = (int)(x % splits);
-                t.unit = (int)y;
+                t.split = x - y * splits;
+                t.unit = y;
                 const int per = (r.blocks + splits - 1) / splits, from = min(r.blocks, t.split * per);
                 r.blocks = min(per, r.blocks - from);
                 r.key0 += from * BK;
