@@ -5,14 +5,18 @@
 // table and applied in f32; one rounding to the element type at the end.
 //
 // Bound by memory: each of q, k, v is read once and written once.  One block per
-// token; dim / 16 threads share a head vector, each with two 16-byte vectors
+// token (or several short ones, see below); dim / 16 threads share a head vector, each with two 16-byte vectors
 // that hold whole pairs: vectors j and j + rot/16 of the rotated part when pairs
 // are (i, i + rot/2), vectors 2j and 2j+1 when they are (2i, 2i+1).  A thread
 // keeps its cosines and sines in registers and walks over the token's heads,
 // three vectors on their way at once, the first ones asked for before the
-// position, the slot and the table's row are there.  Blocks of 64 threads, 32 of
-// them per SM, keep the most copies in flight: 24576 tokens of 32 + 8 + 8 heads
-// of 128 take 93 us = 6.6 TB/s (128 threads: 106 us, one vector at a time: 98).
+// position, the slot and the table's row are there.  Blocks of 64 threads, 12 of
+// them on an SM at once, keep the most copies in flight: 24576 tokens of 32 + 8 + 8
+// heads of 128 take 93 us = 6.6 TB/s (128 threads: 106 us, one vector at a time: 98).
+// Where a token has less than three vectors for each thread of a block, and there
+// are more tokens than blocks fit at once, a block takes as many tokens as it has
+// threads for: 20344 tokens of 6 + 1 + 1 heads of 64 11.8 us against 28.9, of 15 +
+// 3 + 3 heads 25.3 against 34.1.
 #include "serve_common.cuh"
 
 using namespace ktir::serve;
@@ -20,11 +24,14 @@ using namespace ktir::serve;
 namespace {
 
 constexpr int UNROLL = 3;      // head vectors of a thread on their way at once
+constexpr int RESIDENT = 12;   // blocks of 64 threads on an SM at once, by their registers
 
 struct AppendParams {
   KtirKvAppendDesc d;
   long long slots_total;
   int vector_table;      // rows of the table start on 16-byte boundaries
+  int lanes;             // head vectors of a token in flight at once
+  int each;              // tokens of a block
 };
 
 template <typename T>
@@ -73,14 +80,15 @@ __device__ __forceinline__ uint4 rotate_pairs(const uint4& a, const float (&c)[8
   return r;
 }
 
-template <typename T, int THREADS>
-__global__ void __launch_bounds__(THREADS) k_kv_append(const __grid_constant__ AppendParams p) {
+template <typename T, int THREADS, bool SEVERAL>
+__global__ void __launch_bounds__(THREADS, SEVERAL ? RESIDENT : 0) k_kv_append(const __grid_constant__ AppendParams p) {
   const KtirKvAppendDesc& d = p.d;
-  const long long t = blockIdx.x;
   const int parts = d.dim >> 4;                 // threads per head vector
-  const int lanes = THREADS / parts;            // head vectors in flight per block
-  const int hl = threadIdx.x / parts, j = threadIdx.x - hl * parts;
-  if (hl >= lanes) return;
+  const int lanes = SEVERAL ? p.lanes : THREADS / parts;     // head vectors of a token in flight
+  const int vec = threadIdx.x / parts, j = threadIdx.x - vec * parts;
+  const int sub = SEVERAL ? vec / lanes : 0, hl = SEVERAL ? vec - sub * lanes : vec;
+  const long long t = SEVERAL ? (long long)blockIdx.x * p.each + sub : blockIdx.x;
+  if (SEVERAL ? sub >= p.each || t >= d.tokens : hl >= lanes) return;
   const int rparts = d.rot >> 4;
   const bool turn = j < rparts;
   // this thread's two vectors of a head vector, rotated or copied
@@ -112,7 +120,7 @@ __global__ void __launch_bounds__(THREADS) k_kv_append(const __grid_constant__ A
     }
     if (h0 == hl) {                             // the vectors are on their way meanwhile
       if (bad) {
-        if (threadIdx.x == 0) atomicOr(d.status, KTIR_STATUS_BAD_INDEX);
+        if (hl == 0 && j == 0) atomicOr(d.status, KTIR_STATUS_BAD_INDEX);
         return;
       }
       if (turn) {
@@ -190,16 +198,20 @@ extern "C" int ktir_kv_append(const KtirKvAppendDesc* d, void* stream) {
   const __int128 total = (__int128)d->num_pages * d->page_size;
   p.slots_total = total > 0x7fffffffLL ? 0x80000000LL : (long long)total;
   p.vector_table = aligned16(d->table) && !(d->table_stride & 3);
-  const unsigned grid = (unsigned)d->tokens;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
-  // with no more tokens than SMs a larger block is quicker (one token 2.4 us against
-  // 3.2), with more a smaller one (200 tokens 2.65 us against 3.2)
+  const int vectors = (d->q ? d->heads : 0) + 2 * d->kv_heads, across = 64 / (d->dim >> 4);
+  const int sms = sm_count();
+  const bool few = d->tokens <= sms, several = d->tokens > (int64_t)RESIDENT * sms && vectors < UNROLL * across;
+  p.lanes = (vectors + UNROLL - 1) / UNROLL;
+  p.each = several ? across / p.lanes : 1;
+  const unsigned grid = (unsigned)((d->tokens + p.each - 1) / p.each);
   const bool f16 = d->dtype == KTIR_F16;
   const cudaError_t e =
-      d->tokens <= sm_count()
-          ? (f16 ? launch_pdl(k_kv_append<__half, 128>, grid, 128, 0, s, p)
-                 : launch_pdl(k_kv_append<__nv_bfloat16, 128>, grid, 128, 0, s, p))
-          : (f16 ? launch_pdl(k_kv_append<__half, 64>, grid, 64, 0, s, p)
-                 : launch_pdl(k_kv_append<__nv_bfloat16, 64>, grid, 64, 0, s, p));
+      few ? (f16 ? launch_pdl(k_kv_append<__half, 128, false>, grid, 128, 0, s, p)
+                 : launch_pdl(k_kv_append<__nv_bfloat16, 128, false>, grid, 128, 0, s, p))
+      : several ? (f16 ? launch_pdl(k_kv_append<__half, 64, true>, grid, 64, 0, s, p)
+                       : launch_pdl(k_kv_append<__nv_bfloat16, 64, true>, grid, 64, 0, s, p))
+                : (f16 ? launch_pdl(k_kv_append<__half, 64, false>, grid, 64, 0, s, p)
+                       : launch_pdl(k_kv_append<__nv_bfloat16, 64, false>, grid, 64, 0, s, p));
   return launched(e, "ktir_kv_append: launch failed");
 }

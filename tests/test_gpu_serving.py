@@ -105,6 +105,39 @@ def test_append_reports_bad_indices():
     assert torch.equal(vc[1, 0], v[0]) and not vc[1, 1:].any()
 
 
+# more tokens than blocks of one fit on the GPU at once, of few heads: several share a block
+@pytest.mark.parametrize("typ,tokens,heads,kv_heads,dim,rot,page,interleaved,head_major", [
+    ("bf16", 2003, 6, 1, 64, 64, 32, False, False),
+    ("f16", 4001, 15, 3, 64, 32, 16, True, True),
+    ("bf16", 2500, 1, 1, 16, 16, 1, False, False),
+    ("f16", 1999, 2, 1, 256, 0, 8, False, False),
+    ("bf16", 1801, 13, 5, 128, 128, 16, False, True),
+])
+def test_append_several_tokens_per_block(typ, tokens, heads, kv_heads, dim, rot, page, interleaved, head_major):
+    test_append(typ, tokens, heads, kv_heads, dim, rot, page, interleaved, head_major)
+
+
+def test_append_several_tokens_per_block_bad_indices():
+    import torch
+    from ktir_cpu_b200 import check_status, kv_append, rotary_table
+    gen = _gen(5)
+    k, v = (_randn(gen, "bf16", 2500, 1, 64) for _ in range(2))
+    kc, vc = (torch.zeros(100, 25, 1, 64, dtype=torch.bfloat16, device="cuda") for _ in range(2))
+    slots = torch.arange(2500, dtype=torch.int32, device="cuda")
+    positions = slots % 10
+    bad = torch.tensor([0, 7, 1234, 2499], device="cuda")
+    slots[bad[:2]] = 2500
+    positions[bad[2]] = 10
+    positions[bad[3]] = -1
+    kv_append(k, v, kc, vc, slots, positions=positions, table=rotary_table(10, 64))
+    with pytest.raises(IndexError):
+        check_status()
+    got = vc.reshape(2500, 1, 64)
+    kept = torch.ones(2500, dtype=torch.bool, device="cuda")
+    kept[bad] = False
+    assert torch.equal(got[kept], v[kept]) and not got[bad].any() and not kc.reshape(2500, 64)[bad].any()
+
+
 # -- decode -----------------------------------------------------------------------
 
 def _decode_inputs(typ, lengths, heads, kv_heads, dim, page, head_major=False, seed=0, scale_q=1.0):
