@@ -15,12 +15,13 @@
 // into equal stretches, one per group of CTAs; the CTAs of a group take the
 // head tiles over the same stretch (so a page's heads, neighbours in a
 // token-major cache, are read at the same time).  The work is even however the
-// lengths differ.  Within a CTA each of the four warps owns 16 keys of every
-// tile, with its own ring of copies in flight, its own running m, l and o: the
-// warps meet only where a sequence ends.  A stretch that holds part of a
-// sequence leaves (m, l, o) in the workspace, and the last of the CTAs that
-// share the sequence joins the parts in the order of the list (so the result
-// does not depend on which was last).
+// lengths differ.  A few sequences get groups of their own instead, whole or in
+// even parts, where that makes the largest part little longer.  Within a CTA each
+// of the four warps owns 16 keys of every tile, with its own ring of copies in
+// flight, its own running m, l and o: the warps meet only where a sequence ends.
+// A stretch that holds part of a sequence leaves (m, l, o) in the workspace, and
+// the last of the CTAs that share the sequence joins the parts in the order of the
+// list (so the result does not depend on which was last).
 //
 // Precision: scores, m, l and o in f32; the weights p are rounded to the
 // element type for the second product (as the values are), at most one half
@@ -39,6 +40,8 @@ constexpr int TILE = WARPS * KPW;          // keys per tile
 constexpr int ROWS = 16;                   // query heads per head tile at most
 constexpr int MAX_CTAS = 512;              // of a launch that splits sequences
 constexpr int MIN_TILES = 2;               // per stretch: both in flight at once
+constexpr int FIT_BATCH = 64;              // sequences of a launch that may get CTAs of their own,
+constexpr int FIT_TILES = 10;              // and tiles of an even stretch then
 constexpr int LOOK = 3;                    // tiles between a look into the page table and the copy
 constexpr float RESCALE_THRESHOLD = 8.0f;  // log2 units
 constexpr int PART_STRIDE = ROWS * (128 + 2);   // floats of a part: o, then (m, l) per row
@@ -137,6 +140,7 @@ __global__ void __launch_bounds__(THREADS, Cfg<D>::CTAS_PER_SM)
   extern __shared__ __align__(128) uint8_t smem[];
   __shared__ long long s_scan[WARPS];
   __shared__ long long s_start[2];                     // sequence, tile in it
+  __shared__ int s_own[2];                             // CTA groups of the sequence, where it has its own
   __shared__ float2 s_ml[WARPS][ROWS];
   __shared__ int s_last;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
@@ -154,62 +158,171 @@ __global__ void __launch_bounds__(THREADS, Cfg<D>::CTAS_PER_SM)
   pdl_launch();
   pdl_wait();
 
-  // this stretch of the list: an exclusive scan over runs of sequences
-  const long long per = (d.batch + THREADS - 1) / THREADS;
-  const long long r0 = min((long long)d.batch, tid * per), r1 = min((long long)d.batch, r0 + per);
-  long long mine = 0;
-  for (long long b = r0; b < r1; ++b) {
-    const int len = d.lengths[b];
-    if (len < 0 || len > most) {
-      if (blockIdx.x == 0) atomicOr(d.status, KTIR_STATUS_BAD_INDEX);
-    } else {
-      mine += (len + TILE - 1) / TILE;
-    }
-  }
-  long long incl = mine;
-#pragma unroll
-  for (int w = 1; w < 32; w <<= 1) {
-    const long long o = __shfl_up_sync(0xffffffffu, incl, w);
-    if (lane >= w) incl += o;
-  }
-  if (lane == 31) s_scan[warp] = incl;
-  __syncthreads();
-  long long before = 0, total = 0;
-#pragma unroll
-  for (int w = 0; w < WARPS; ++w) {
-    if (w < warp) before += s_scan[w];
-    total += s_scan[w];
-  }
   // sequences without keys give zeros
-  for (long long b = grp; b < d.batch; b += p.groups) {
-    if (length_of(b) == 0) {
-      for (int i = tid; i < nrows * C::CHUNKS; i += THREADS) {
-        const int r = i / C::CHUNKS, c = i - r * C::CHUNKS;
-        *reinterpret_cast<uint4*>(static_cast<T*>(d.out) + b * d.out_stride[0] +
-                                  (head0 + r) * d.out_stride[1] + c * 8) = make_uint4(0, 0, 0, 0);
+  auto zeros = [&]() {
+    for (long long b = grp; b < d.batch; b += p.groups) {
+      if (length_of(b) == 0) {
+        for (int i = tid; i < nrows * C::CHUNKS; i += THREADS) {
+          const int r = i / C::CHUNKS, c = i - r * C::CHUNKS;
+          *reinterpret_cast<uint4*>(static_cast<T*>(d.out) + b * d.out_stride[0] +
+                                    (head0 + r) * d.out_stride[1] + c * 8) = make_uint4(0, 0, 0, 0);
+        }
+        if (d.lse && tid < nrows) d.lse[b * d.heads + head0 + tid] = -INFINITY;
       }
-      if (d.lse && tid < nrows) d.lse[b * d.heads + head0 + tid] = -INFINITY;
+    }
+  };
+
+  // This CTA's stretch of the list: tiles [t_begin, t_end), the first one tile `first`
+  // of sequence `start`, whose tiles begin at `base`.
+  long long t_begin, t_end, base, start, ng = 0, total = 0;
+  int first;
+  bool fits = false;
+  constexpr int FREE = NT == 1 ? 4 : 6;       // tiles that one CTA takes as fast as several join their parts
+  // this CTA's part of a sequence that CTA groups own0 .. own0 + own - 1 have to themselves
+  auto take = [&](int tiles, int own0, int own) {
+    const int least = (unsigned)tiles / (unsigned)own, left = tiles - least * own, piece = grp - own0;
+    base = 0;
+    first = piece * least + min(piece, left);
+    t_begin = first;
+    t_end = first + least + (piece < left ? 1 : 0);
+    if (tid == 0) {
+      s_own[0] = own0;
+      s_own[1] = own0 + own - 1;
+    }
+  };
+  if (d.batch == 1) {                         // nothing to count (77 keys: 4.5 us against 5.2, 400: 6.6 against 7.9)
+    const int len = d.lengths[0];
+    const bool bad = len < 0 || len > most;
+    if (bad && blockIdx.x == 0 && tid == 0) atomicOr(d.status, KTIR_STATUS_BAD_INDEX);
+    if (bad || len == 0) {
+      zeros();
+      return;
+    }
+    const int tiles = (int)(((unsigned)len + TILE - 1) / TILE);
+    const int own = tiles <= FREE ? 1 : min(p.groups, tiles > 16 ? (tiles + 1) / 2 : tiles);
+    if (grp >= own) return;
+    fits = true;
+    start = 0;
+    take(tiles, 0, own);
+  } else if (d.batch <= min(FIT_BATCH, p.groups)) {
+    // Few sequences: each gets CTAs of its own if that costs at most three tiles more
+    // than even stretches (ending one sequence and beginning another costs as much: 7
+    // sequences of 700 keys, 5 heads of 64: 7.5 us against 10.3).  One of few tiles is
+    // not split, since joining parts takes about as long as three of them.
+    const int each = d.batch > 32 ? 2 : 1;
+    unsigned t[2] = {0, 0};
+    bool none = false, bad = false;
+#pragma unroll
+    for (int x = 0; x < 2; ++x) {
+      const long long b = lane * each + x;
+      if (x < each && b < d.batch) {
+        const int len = d.lengths[b];
+        if (len < 0 || len > most) bad = true;
+        else t[x] = ((unsigned)len + TILE - 1) / TILE;
+        none |= t[x] == 0;
+      }
+    }
+    if (bad && blockIdx.x == 0 && warp == 0) atomicOr(d.status, KTIR_STATUS_BAD_INDEX);
+    if (__any_sync(0xffffffffu, none)) zeros();
+    const unsigned sum = __reduce_add_sync(0xffffffffu, t[0] + t[1]);     // at most 64 x 2^25
+    const unsigned longest = __reduce_max_sync(0xffffffffu, max(t[0], t[1]));
+    // 16 parts are joined at once
+    unsigned size = max((sum + p.groups - 1) / p.groups, longest > 16 ? 2u : 1u);
+    auto pieces = [&](unsigned tiles, unsigned size, float over) -> unsigned {
+      return tiles <= max(size, (unsigned)FREE) ? (tiles ? 1u : 0u)
+                                                : (unsigned)(((float)(min(tiles, 8191u) + size) - 0.5f) * over);
+    };
+    int more = 0;
+    if (size <= FIT_TILES) {
+      unsigned two[2];                         // what sizes size .. size + 3 take, two to a word
+#pragma unroll
+      for (unsigned x = 0; x < 2; ++x) {
+        const unsigned a = size + 2 * x, b = a + 1;
+        const float oa = __frcp_rn((float)a), ob = __frcp_rn((float)b);
+        two[x] = __reduce_add_sync(0xffffffffu, min(511u, pieces(t[0], a, oa) + pieces(t[1], a, oa)) +
+                                                    (min(511u, pieces(t[0], b, ob) + pieces(t[1], b, ob)) << 16));
+      }
+      const unsigned limit = min(p.groups, 510);
+#pragma unroll
+      for (int x = 3; x >= 0; --x)
+        if (((two[x >> 1] >> (16 * (x & 1))) & 0xffffu) <= limit) {
+          fits = true;
+          more = x;
+        }
+    }
+    if (fits) {
+      size += more;
+      const float over = __frcp_rn((float)size);
+      const int n0 = (int)pieces(t[0], size, over), mine = n0 + (int)pieces(t[1], size, over);
+      int incl = mine;
+#pragma unroll
+      for (int w = 1; w < 32; w <<= 1) {
+        const int o = __shfl_up_sync(0xffffffffu, incl, w);
+        if (lane >= w) incl += o;
+      }
+      const unsigned hit = __ballot_sync(0xffffffffu, grp >= incl - mine && grp < incl);
+      if (!hit) return;
+      const int from = __ffs(hit) - 1;
+      const int at = incl - mine, second = grp >= at + n0 ? 1 : 0;       // of the lane's two sequences
+      start = __shfl_sync(0xffffffffu, lane * each + second, from);
+      const int own0 = __shfl_sync(0xffffffffu, at + (second ? n0 : 0), from);
+      const int own = __shfl_sync(0xffffffffu, second ? mine - n0 : n0, from);
+      const int tiles = (int)__shfl_sync(0xffffffffu, second ? t[1] : t[0], from);
+      take(tiles, own0, own);
     }
   }
-  const long long want = (total + MIN_TILES - 1) / MIN_TILES;
-  const long long ng = min((long long)p.groups, want);
-  if (grp >= ng) return;
-  const long long t_begin = total * grp / ng, t_end = total * (grp + 1) / ng;
-  const int n = (int)(t_end - t_begin);
-  const long long excl = before + incl - mine;
-  if (t_begin >= excl && t_begin < excl + mine) {
-    long long at = excl;
+  if (!fits) {
+    // even stretches: an exclusive scan over runs of sequences
+    const long long run = (d.batch + THREADS - 1) / THREADS;
+    const long long r0 = min((long long)d.batch, tid * run), r1 = min((long long)d.batch, r0 + run);
+    long long mine = 0;
     for (long long b = r0; b < r1; ++b) {
-      const int nt = (length_of(b) + TILE - 1) / TILE;
-      if (t_begin < at + nt) {
-        s_start[0] = b;
-        s_start[1] = t_begin - at;
-        break;
+      const int len = d.lengths[b];
+      if (len < 0 || len > most) {
+        if (blockIdx.x == 0) atomicOr(d.status, KTIR_STATUS_BAD_INDEX);
+      } else {
+        mine += (len + TILE - 1) / TILE;
       }
-      at += nt;
     }
+    long long incl = mine;
+#pragma unroll
+    for (int w = 1; w < 32; w <<= 1) {
+      const long long o = __shfl_up_sync(0xffffffffu, incl, w);
+      if (lane >= w) incl += o;
+    }
+    if (lane == 31) s_scan[warp] = incl;
+    __syncthreads();
+    long long before = 0;
+#pragma unroll
+    for (int w = 0; w < WARPS; ++w) {
+      if (w < warp) before += s_scan[w];
+      total += s_scan[w];
+    }
+    if (d.batch > min(FIT_BATCH, p.groups)) zeros();      // else done above
+    const long long want = (total + MIN_TILES - 1) / MIN_TILES;
+    ng = min((long long)p.groups, want);
+    if (grp >= ng) return;
+    t_begin = total * grp / ng;
+    t_end = total * (grp + 1) / ng;
+    const long long excl = before + incl - mine;
+    if (t_begin >= excl && t_begin < excl + mine) {
+      long long at = excl;
+      for (long long b = r0; b < r1; ++b) {
+        const int nt = (length_of(b) + TILE - 1) / TILE;
+        if (t_begin < at + nt) {
+          s_start[0] = b;
+          s_start[1] = t_begin - at;
+          break;
+        }
+        at += nt;
+      }
+    }
+    __syncthreads();
+    start = s_start[0];
+    first = (int)s_start[1];
+    base = t_begin - first;
   }
-  __syncthreads();
+  const int n = (int)(t_end - t_begin);
 
   auto open = [&](Cursor& c, long long b) {   // the next sequence from b on that has keys
     c.b = b;
@@ -222,10 +335,9 @@ __global__ void __launch_bounds__(THREADS, Cfg<D>::CTAS_PER_SM)
     if (++c.t == c.nt) open(c, c.b + 1);
   };
   Cursor get, use;
-  open(get, s_start[0]);
-  get.t = (int)s_start[1];
+  open(get, start);
+  get.t = first;
   use = get;
-  long long base = t_begin - get.t;           // first tile of use's sequence in the list
 
   const uint32_t ring = (uint32_t)__cvta_generic_to_shared(smem) + warp * (C::STAGES * C::STAGE);
   float* join = reinterpret_cast<float*>(smem + C::RING);
@@ -462,7 +574,7 @@ __global__ void __launch_bounds__(THREADS, Cfg<D>::CTAS_PER_SM)
     clear();
     if (!whole) {
       // stretches that share the sequence: those of its first to its last tile
-      const long long g0 = ((base + 1) * ng - 1) / total, g1 = (end * ng - 1) / total;
+      const long long g0 = fits ? s_own[0] : ((base + 1) * ng - 1) / total, g1 = fits ? s_own[1] : (end * ng - 1) / total;
       if (tid == 0) {
         int* counter = p.counters + b * p.ht + ht;
         const int before = atomicAdd(counter, 1);
@@ -602,7 +714,7 @@ extern "C" int ktir_paged_decode(const KtirPagedDecodeDesc* d, void* stream) {
   if (slots > MAX_CTAS) slots = MAX_CTAS;
   long long groups = slots / p.ht;
   const __int128 tiles = (__int128)d->batch * ((d->max_pages * d->page_size + TILE - 1) / TILE);
-  if (groups > (tiles + MIN_TILES - 1) / MIN_TILES) groups = (long long)((tiles + MIN_TILES - 1) / MIN_TILES);
+  if (groups > tiles) groups = (long long)tiles;
   if (groups < 1) groups = 1;
   p.groups = (int)groups;
   const unsigned grid = (unsigned)(groups * p.ht);

@@ -190,6 +190,46 @@ def test_decode_many_sequences():
     _check_decode("bf16", *x, 0.3, out, lse)
 
 
+# how the keys are shared out: one sequence, whole or in parts; sequences with CTAs of their own, one or
+# two to a lane that counts; too many tiles or too many sequences for that
+@pytest.mark.parametrize("lengths", [
+    [0], [1], [64], [256], [257], [384], [385], [1024], [1025], [30000],
+    [640, 0, 65, 1000, 256, 257, 1, 3000],
+    [130 + 37 * (b % 9) for b in range(32)],
+    [(b * 61) % 300 for b in range(33)],
+    [(b * 127) % 500 for b in range(64)],
+    [1 + (b * 43) % 200 for b in range(65)],
+    [3000 + 100 * b for b in range(20)],
+    [5000, 3, 0, 9],
+])
+@pytest.mark.parametrize("typ,heads,kv_heads,dim", [("bf16", 8, 2, 128), ("f16", 3, 1, 64), ("bf16", 32, 2, 64)])
+def test_decode_shares_of_ctas(lengths, typ, heads, kv_heads, dim):
+    from ktir_cpu_b200 import check_status, paged_decode
+    x = _decode_inputs(typ, lengths, heads, kv_heads, dim, 16, seed=len(lengths))
+    out, lse = paged_decode(*x, return_lse=True)
+    again, lse2 = paged_decode(*x, return_lse=True)
+    check_status()
+    assert out.equal(again) and lse.equal(lse2)
+    _check_decode(typ, *x, dim ** -0.5, out, lse)
+
+
+@pytest.mark.parametrize("bad", [-3, 10 ** 6])
+@pytest.mark.parametrize("batch", [1, 6, 40, 70])
+def test_decode_bad_lengths(bad, batch):
+    import torch
+    from ktir_cpu_b200 import check_status, paged_decode
+    x = _decode_inputs("bf16", [100 + 50 * b for b in range(batch)], 8, 2, 64, 16, seed=batch)
+    lengths = x[-1].clone()
+    lengths[batch // 2] = bad
+    out, lse = paged_decode(*x[:-1], lengths, return_lse=True)
+    with pytest.raises(IndexError):
+        check_status()
+    assert not out[batch // 2].any() and (lse[batch // 2] == -float("inf")).all()
+    lengths[batch // 2] = 0
+    _check_decode("bf16", *x[:-1], lengths, 64 ** -0.5, out, lse)
+    check_status()
+
+
 @pytest.mark.parametrize("typ", ["bf16", "f16"])
 def test_decode_peaked_and_growing_scores(typ):
     """Scores in the hundreds, the largest at the end: the running maximum moves
