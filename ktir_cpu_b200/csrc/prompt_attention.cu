@@ -601,10 +601,11 @@ __global__ void __launch_bounds__(THREADS, 1)
           for (int w = 0; w < 2; ++w) {
             const int y = parts ? x / splits : singly && w ? first + 2 * (G - 1 - blockIdx.x) + 1 : first;
             if ((parts && (w || x >= all)) || y >= (singly ? rows : twos)) break;
-            long long b;
+            long long b = 0;
             int i;
             const int index = (int)((unsigned)y / (unsigned)d.kv_heads);
-            order.find(index, parts, b, i);
+            if (d.batch == 1) i = (singly ? rows : twos) / d.kv_heads - 1 - index;    // its last tile is the heaviest
+            else order.find(index, parts, b, i);
             if (lane == 0 && b >= 0) {
               const int head = y - index * d.kv_heads;
               const Seq q = order.seq(b);
@@ -628,7 +629,7 @@ __global__ void __launch_bounds__(THREADS, 1)
         __syncwarp();
         if (lane == 0) mbar_arrive(smem_u32(&B.sched_full[s]));
         if (stop) break;
-        if (next == 0 && all > 2 * G) order.tabulate(B.weights, heaviest);    // worth it for a few more
+        if (next == 0 && all > 2 * G && d.batch > 1) order.tabulate(B.weights, heaviest);    // worth it for a few more
       }
     } else if (warp == 9) {
       // ---------------- TMA ----------------
