@@ -44,6 +44,11 @@
 // Precision: S, O, m and l in f32; P is rounded to the element type for the
 // second product (tcgen05 wants one type for both operands), half an ulp per
 // weight; l adds the unrounded weights.
+// Measured, 8192 tokens of 32 heads over 8, causal: dim 128 459 us in a short burst
+// (1,200 TFLOP/s) and 531 under the power cap, dim 64 365 us.  Of a block's 2,100
+// cycles (80 keys, both row tiles) the exponentials take 1,300; both groups of softmax
+// warps run in step, so nothing else overlaps them.  A change of tiles costs 4,500
+// cycles: the last product, the outputs, the next tile's S.
 // Every wait is bounded; one that runs out raises the CTA's abort flag, every
 // role then leaves its loop, waits for its own copies and products, and the
 // CTA still frees its TMEM.
@@ -560,19 +565,30 @@ __global__ void __launch_bounds__(THREADS, 1)
       heaviest = (int)__reduce_max_sync(0xffffffffu, (unsigned)heaviest);
       const int rows = warp_sum(singles) * d.kv_heads, twos = warp_sum(pairs) * d.kv_heads;     // below 2^30
       const int G = (int)gridDim.x;
-      // no more row tiles than CTAs: one each, and what is left over shares their keys.
-      // A stretch costs its blocks, joining S of them about as much as S blocks.
+      // No more row tiles than CTAs: one each, and what is left over shares their keys,
+      // S CTAs to a row tile.  The longest stretch costs ceil(blocks / S) blocks, and
+      // joining costs about J of them for every four parts (64 KiB each at dim 128, from
+      // L2 through one SM).  64 queries over 400 keys, 32 heads over 8, dim 128: whole
+      // 10.8 us, in three parts 15.6; over 2000 keys whole 26.5, in four parts 20.3.
       const bool parts = rows <= G;
       int splits = 1;
       if (parts && rows > 0 && p.parts) {
-        while (splits * splits < heaviest) ++splits;
-        splits = max(1, min(splits, min(G, MAX_PARTS) / rows));
+        constexpr int J = D == 128 ? 8 : 4;
+        const int cap = min(G, MAX_PARTS) / rows;
+        for (int r = 1, best = heaviest; cap > 1 && r * J < best; ++r) {
+          const int S = min(4 * r, cap), cost = (heaviest + S - 1) / S + r * J;
+          if (cost < best) {
+            best = cost;
+            splits = S;
+          }
+          if (4 * r >= cap) break;
+        }
       }
       // Singles where a CTA has few row tiles, each then next to one of another weight
-      // (7 pieces of prompts, 195 row tiles: 43 us against 55 in pairs), or where pairs
+      // (7 pieces of prompts, 195 row tiles: 36 us against 44 in pairs), or where pairs
       // would leave more than a third of them empty (200 prompts of 32 tokens: 46 us
-      // against 67).  Else pairs: their shared blocks save L2 traffic (8192 tokens: 477
-      // us against 573).
+      // against 59).  Else pairs: their shared blocks save L2 traffic (8192 tokens: 459
+      // us against 489).
       const bool singly = parts || rows <= 2 * G || 2 * twos - rows > (2 * twos) / 3;
       const int all = parts ? rows * splits : singly ? (rows + 1) / 2 : twos;
       Order<BK> order = {p, B.lengths, lane, singly ? half : 2 * half, singly ? p.token_magic : p.pair_magic, heaviest, 0, nullptr};
@@ -987,7 +1003,7 @@ __global__ void __launch_bounds__(THREADS, 1)
       T* out = static_cast<T*>(d.out) + tok * d.out_stride[0] + head * d.out_stride[1];
       // 64 outputs of the warp's 32 rows: every lane's own row to shared memory, then
       // eight lanes a row from there (a row at a time from one lane, a store would
-      // touch 32 rows: 4,600 cycles a tile against 1,300)
+      // touch 32 rows: 4,600 cycles a tile against 3,300)
       const uint32_t keep = __ballot_sync(0xffffffffu, store);
       auto store_rows = [&](int i, const uint32_t (&v)[32]) {
         uint8_t* mine = staged + lane * C::OUT_ROW;
