@@ -18,9 +18,10 @@
 //   pairs    two that follow each other in a sequence, sharing its K and V blocks
 //   singles  two of any sequences and heads, each with blocks of its own, where
 //            most sequences have but one row tile per head
-//   parts    no more row tiles than SMs: one per CTA, or, where its keys are many,
-//            a stretch of them; the stretches' (m, l, O) are left in the workspace
-//            and the last CTA of a row tile joins them in their order
+//   parts    no more row tiles than SMs: one per CTA, half of its keys to each group
+//            of softmax warps, or, where its keys are many, a stretch of them; the
+//            stretches' (m, l, O) are left in the workspace and the last CTA of a row
+//            tile joins them in their order
 //
 // Roles, meeting only at mbarriers:
 //   warps 0-3, 4-7  the softmax of row tile 0 and 1, one row per thread:
@@ -70,6 +71,7 @@ constexpr int SCHED = 4;             // tiles announced ahead
 constexpr int WEIGHTS = 512;         // weights whose tile counts a CTA keeps there
 constexpr int CACHED = 256;          // sequences whose lengths a CTA keeps in shared memory
 constexpr int MAX_PARTS = 160;       // CTAs of a launch that splits keys
+constexpr int HALVE = 3;             // blocks from which a CTA's two groups of softmax warps share a row tile
 constexpr int PART_FLOATS = 128 * BQ + 2 * BQ;      // O [dim][row], then (m, l) per row
 constexpr int64_t PARTS_BYTES = (int64_t)MAX_PARTS * PART_FLOATS * 4;
 constexpr int SCHED_READERS = 11;    // 8 softmax warps, two MMA, TMA
@@ -109,6 +111,7 @@ struct RowTile {
 struct Tile {
   int stop;
   int shared;     // both row tiles use the same K and V blocks
+  int halves;     // row tile 1 is the second half of row tile 0's keys
   int splits;     // CTAs that share row tile 0, each with a stretch of its keys,
   int split;      // which of them this is
   int unit;       // and the row tile's number
@@ -133,7 +136,7 @@ struct Shared {
   uint64_t tail[MAX_STAGES];        // a V block with rows past the last key has arrived
   uint64_t drain[2];
   uint64_t sched_full[SCHED], sched_empty[SCHED];
-  uint64_t part_in, part_out;
+  uint64_t meet, part_in, part_out;
   Tile tile[SCHED];
   int2 lengths[CACHED];             // tokens and keys of the first sequences
   int last;
@@ -509,7 +512,8 @@ __global__ void __launch_bounds__(THREADS, 1)
       mbar_init(smem_u32(&B.tail[s]), 1);
     }
     for (int w = 0; w < 2; ++w) mbar_init(smem_u32(&B.drain[w]), 1);
-    mbar_init(smem_u32(&B.part_in), 4);
+    mbar_init(smem_u32(&B.meet), 8);
+    mbar_init(smem_u32(&B.part_in), 8);
     mbar_init(smem_u32(&B.part_out), 1);
     for (int s = 0; s < SCHED; ++s) {
       mbar_init(smem_u32(&B.sched_full[s]), 1);
@@ -565,15 +569,16 @@ __global__ void __launch_bounds__(THREADS, 1)
       heaviest = (int)__reduce_max_sync(0xffffffffu, (unsigned)heaviest);
       const int rows = warp_sum(singles) * d.kv_heads, twos = warp_sum(pairs) * d.kv_heads;     // below 2^30
       const int G = (int)gridDim.x;
-      // No more row tiles than CTAs: one each, and what is left over shares their keys,
-      // S CTAs to a row tile.  The longest stretch costs ceil(blocks / S) blocks, and
-      // joining costs about J of them for every four parts (64 KiB each at dim 128, from
-      // L2 through one SM).  64 queries over 400 keys, 32 heads over 8, dim 128: whole
-      // 10.8 us, in three parts 15.6; over 2000 keys whole 26.5, in four parts 20.3.
+      // No more row tiles than CTAs: one each, its keys shared by the two groups of
+      // softmax warps (512 tokens, 32 heads over 8, dim 128: 12.1 us against 13.5), and
+      // what CTAs are left over share them too, S to a row tile.  The longest stretch
+      // costs ceil(blocks / S) blocks, and joining costs about J of them for every four
+      // parts (64 KiB each at dim 128, from L2 through one SM).  64 queries over 400
+      // keys: whole 9.9 us, in three parts 15.6; over 2000 keys whole 21.5, in four 19.5.
       const bool parts = rows <= G;
       int splits = 1;
       if (parts && rows > 0 && p.parts) {
-        constexpr int J = D == 128 ? 8 : 4;
+        constexpr int J = D == 128 ? 12 : 6;
         const int cap = min(G, MAX_PARTS) / rows;
         for (int r = 1, best = heaviest; cap > 1 && r * J < best; ++r) {
           const int S = min(4 * r, cap), cost = (heaviest + S - 1) / S + r * J;
@@ -608,6 +613,7 @@ __global__ void __launch_bounds__(THREADS, 1)
         if (lane == 0) {
           t.stop = stop;
           t.shared = !singly;
+          t.halves = 0;
           t.splits = 1;                       // an empty tile has no part in another's
           t.split = t.unit = 0;
           for (int w = 0; w < 2; ++w) t.r[w].tokens = t.r[w].blocks = t.r[w].keys = 0;
@@ -637,6 +643,16 @@ __global__ void __launch_bounds__(THREADS, 1)
                 r.key0 += from * BK;
                 r.keys -= from * BK;
                 r.seen -= from * BK;
+              }
+              if (parts && t.r[0].blocks >= HALVE) {      // for both groups of softmax warps
+                RowTile &r = t.r[0], &o = t.r[1];
+                o = r;
+                r.blocks = (r.blocks + 1) / 2;
+                o.blocks -= r.blocks;
+                o.key0 += r.blocks * BK;
+                o.keys -= r.blocks * BK;
+                o.seen -= r.blocks * BK;
+                t.halves = 1;
               }
             }
             if (!singly) break;
@@ -864,8 +880,9 @@ __global__ void __launch_bounds__(THREADS, 1)
       const Tile& t = B.tile[k % SCHED];
       const RowTile& r_t = t.r[w];
       const int splits = t.splits;
-      // of a split row tile both groups of softmax warps join, half of the outputs each
-      const RowTile& o_t = t.r[splits > 1 ? 0 : w];
+      // both groups of softmax warps join the stretches of a row tile, half of the outputs each
+      const bool joined = splits > 1 || t.halves;
+      const RowTile& o_t = t.r[joined ? 0 : w];
       const bool store = real && token < o_t.tokens;
       const int blocks = r_t.blocks;
       const int limit = d.causal ? r_t.seen + token : r_t.keys;      // keys this row sees
@@ -1026,30 +1043,84 @@ __global__ void __launch_bounds__(THREADS, 1)
         if (!__all_sync(0xffffffffu, wait(smem_u32(&B.pv_done[w]), (n_s - 1) & 1, abort))) break;
         tc_fence_after();
       }
-      if (splits > 1) {
-        // this stretch's O [dim][row], m and l; the last CTA of the row tile joins them
-        if (w == 0) {
-          float* part = p.parts + (long long)(unit * splits + split) * PART_FLOATS;
-          if (blocks) {
-#pragma unroll 1
-            for (int i = 0; i < D; i += 32) {
-              uint32_t r[32];
-              tmem_ld32_wait(O + i, r);
+      if (joined) {
+        constexpr int EACH = D / 2;                    // outputs per group
+        // Every thread reads its row of both row tiles' O, with their m and l (left where
+        // Q was: its products are complete, and a CTA has one tile when keys are shared).
+        float2* row_ml = reinterpret_cast<float2*>(smem_raw + (sQ - smem_u32(smem_raw)));
+        auto ml_at = [&](int w) -> float2& { return row_ml[w * (C::Q_TILE / 8) + row]; };
+        ml_at(w) = make_float2(blocks ? m : -INFINITY, blocks ? l : 0.f);
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(smem_u32(&B.meet));
+        if (!__all_sync(0xffffffffu, wait(smem_u32(&B.meet), 0, abort))) break;
+        tc_fence_after();
+        const float2 ml0 = ml_at(0), ml1 = ml_at(1);
+        m = fmaxf(ml0.x, ml1.x);
+        const float at_most = m == -INFINITY ? 0.f : m;
+        const float f0 = ex2(ml0.x - at_most), f1 = ex2(ml1.x - at_most);
+        l = ml0.y * f0 + ml1.y * f1;
+        const uint32_t O0 = at_lane + C::O_COL;
+        const bool any1 = __any_sync(0xffffffffu, ml1.x != -INFINITY);
+        auto both = [&](int i, float (&o)[32]) {        // 32 columns of f0 O_0 + f1 O_1
+          uint32_t r[32];
+          tmem_ld32_wait(O0 + i, r);
 #pragma unroll
-              for (int x = 0; x < 32; ++x) part[(i + x) * BQ + row] = __uint_as_float(r[x]);
+          for (int x = 0; x < 32; ++x) o[x] = ml0.x == -INFINITY ? 0.f : __uint_as_float(r[x]) * f0;
+          if (any1) {
+            tmem_ld32_wait(O0 + C::O_STEP + i, r);
+#pragma unroll
+            for (int x = 0; x < 32; ++x) o[x] += ml1.x == -INFINITY ? 0.f : __uint_as_float(r[x]) * f1;
+          }
+        };
+        auto store_half = [&](const uint32_t (&v)[32]) {
+          if constexpr (EACH == 64) {
+            store_rows(w * 64, v);
+          } else if (store) {
+#pragma unroll
+            for (int x = 0; x < 16; x += 4)
+              *reinterpret_cast<uint4*>(out + w * 32 + 2 * x) = make_uint4(v[x], v[x + 1], v[x + 2], v[x + 3]);
+          }
+        };
+        if (splits == 1) {
+          const float inv = l == 0.f ? 0.f : 1.f / l;
+          uint32_t v[32];
+#pragma unroll
+          for (int i = 0; i < EACH; i += 32) {
+            float o[32];
+            both(w * EACH + i, o);
+#pragma unroll
+            for (int x = 0; x < 16; ++x) v[i / 2 + x] = Elem<T>::from2(o[2 * x] * inv, o[2 * x + 1] * inv);
+          }
+          store_half(v);
+          if (store && d.lse && w == 0) d.lse[tok * d.heads + head] = l == 0.f ? -INFINITY : (m + log2f(l)) * LN2;
+          continue;
+        }
+        // this stretch's O [dim][row], m and l; the last CTA of the row tile joins them
+        {
+          float* part = p.parts + (long long)(unit * splits + split) * PART_FLOATS;
+          if (__any_sync(0xffffffffu, m != -INFINITY)) {
+#pragma unroll 1
+            for (int i = 0; i < EACH; i += 32) {
+              float o[32];
+              both(w * EACH + i, o);
+#pragma unroll
+              for (int x = 0; x < 32; ++x) part[(w * EACH + i + x) * BQ + row] = o[x];
             }
           }
-          reinterpret_cast<float2*>(part + 128 * BQ)[row] = make_float2(m, l);
+          if (w == 0) reinterpret_cast<float2*>(part + 128 * BQ)[row] = make_float2(m, l);
           __threadfence();
           __syncwarp();
           if (lane == 0) mbar_arrive(smem_u32(&B.part_in));
-          if (!__all_sync(0xffffffffu, wait(smem_u32(&B.part_in), 0, abort))) break;
           if (tid == 0) {
-            B.last = atomicAdd(p.counters + unit, 1) == splits - 1;
-            if (B.last) p.counters[unit] = 0;
-            __threadfence();
-            mbar_arrive(smem_u32(&B.part_out));
+            if (wait(smem_u32(&B.part_in), 0, abort)) {
+              B.last = atomicAdd(p.counters + unit, 1) == splits - 1;
+              if (B.last) p.counters[unit] = 0;
+              __threadfence();
+              mbar_arrive(smem_u32(&B.part_out));
+            }
           }
+          __syncwarp();
         }
         if (!__all_sync(0xffffffffu, wait(smem_u32(&B.part_out), 0, abort))) break;
         if (!B.last) continue;
@@ -1065,7 +1136,6 @@ __global__ void __launch_bounds__(THREADS, 1)
           sum += ml.y * ex2(ml.x - sub);
         }
         const float inv = sum == 0.f ? 0.f : 1.f / sum;
-        constexpr int EACH = D / 2;                    // outputs per group
         uint32_t v[32];
 #pragma unroll
         for (int i = 0; i < EACH; i += 32) {
@@ -1092,13 +1162,7 @@ __global__ void __launch_bounds__(THREADS, 1)
 #pragma unroll
           for (int x = 0; x < 16; ++x) v[(i & 32) / 2 + x] = Elem<T>::from2(o[2 * x], o[2 * x + 1]);
         }
-        if constexpr (EACH == 64) {
-          store_rows(w * 64, v);
-        } else if (store) {
-#pragma unroll
-          for (int x = 0; x < 16; x += 4)
-            *reinterpret_cast<uint4*>(out + w * 32 + 2 * x) = make_uint4(v[x], v[x + 1], v[x + 2], v[x + 3]);
-        }
+        store_half(v);
         if (store && d.lse && w == 0) d.lse[tok * d.heads + head] = sum == 0.f ? -INFINITY : (top + log2f(sum)) * LN2;
         continue;
       }

@@ -434,6 +434,22 @@ def test_prompt_many_short():
     _check_prompt("bf16", *x, True, 0.2, out, lse)
 
 
+# few row tiles: a CTA's halves of the keys, around the blocks (80 keys at dim 128, 128 at dim 64) where that begins
+@pytest.mark.parametrize("keys", [160, 161, 240, 241, 256, 257, 320, 385, 1280, 1281])
+@pytest.mark.parametrize("typ,new,heads,kv_heads,dim,causal", [
+    ("bf16", 5, 4, 2, 128, True),
+    ("f16", 130, 3, 1, 64, True),
+    ("f16", 40, 6, 6, 128, False),
+    ("bf16", 300, 2, 2, 64, True),        # more queries than some have keys: rows that see none
+])
+def test_prompt_halves_of_keys(keys, typ, new, heads, kv_heads, dim, causal):
+    from ktir_cpu_b200 import check_status, prompt_attention
+    q, k, v, offsets, kv_offsets = _prompt_inputs(typ, [new], [keys], heads, kv_heads, dim, seed=keys)
+    out, lse = prompt_attention(q, k, v, offsets, kv_offsets=kv_offsets, causal=causal, return_lse=True)
+    check_status()
+    _check_prompt(typ, q, k, v, offsets, kv_offsets, causal, dim ** -0.5, out, lse)
+
+
 @pytest.mark.parametrize("typ,dim", [("bf16", 128), ("f16", 64), ("f16", 128)])
 @pytest.mark.parametrize("rising", [True, False])
 def test_prompt_peaked_scores(typ, dim, rising):
