@@ -200,6 +200,9 @@ def test_decode_many_sequences():
     [(b * 127) % 500 for b in range(64)],
     [1 + (b * 43) % 200 for b in range(65)],
     [3000 + 100 * b for b in range(20)],
+    [0, 0] + [(b * 53) % 700 for b in range(90)] + [0] * 5,
+    [769 * (b % 2) + b for b in range(150)],
+    [768 - b for b in range(300)],
     [5000, 3, 0, 9],
 ])
 @pytest.mark.parametrize("typ,heads,kv_heads,dim", [("bf16", 8, 2, 128), ("f16", 3, 1, 64), ("bf16", 32, 2, 64)])
