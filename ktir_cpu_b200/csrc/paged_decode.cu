@@ -483,7 +483,7 @@ __global__ void __launch_bounds__(THREADS, Cfg<D>::CTAS_PER_SM)
       float top[2];
 #pragma unroll
       for (int x = 0; x < 4; ++x)
-        s[h][x] = at + 8 * (x >> 1) < left ? (s[h][x] + s2[h][x]) * sl : -INFINITY;
+        s[h][x] = at + 8 * (x >> 1) < left ? __fmul_rn(s[h][x] + s2[h][x], sl) : -INFINITY;
 #pragma unroll
       for (int x = 0; x < 2; ++x) {
         top[x] = fmaxf(s[h][x], s[h][x + 2]);
@@ -492,7 +492,7 @@ __global__ void __launch_bounds__(THREADS, Cfg<D>::CTAS_PER_SM)
         top[x] = fmaxf(top[x], __shfl_xor_sync(0xffffffffu, top[x], 16));
       }
       if (__any_sync(0xffffffffu,
-                     top[0] > m[h][0] + RESCALE_THRESHOLD || top[1] > m[h][1] + RESCALE_THRESHOLD)) {
+                     top[0] - m[h][0] > RESCALE_THRESHOLD || top[1] - m[h][1] > RESCALE_THRESHOLD)) {
 #pragma unroll
         for (int x = 0; x < 2; ++x) {
           const float mn = fmaxf(m[h][x], top[x]);

@@ -611,3 +611,67 @@ def test_prompt_then_decode_agree():
         one = paged_decode(turned[i:i + 1], kc, vc, pages, torch.tensor([i + 1], dtype=torch.int32, device="cuda"))
         assert (one[0].double() - whole[i].double()).abs().max() <= bound
     check_status()
+
+
+# -- scores far from 0 ---------------------------------------------------------------
+
+def _far(typ, keys, dim, best):
+    """Integer vectors: every score is exact in 32 bits, key `best`'s the largest by
+    more than 2^20, and its product with scale log2(e) is not."""
+    import torch
+    q = torch.full((1, 1, dim), 3 * 4096., device="cuda").to(S.dtype_of(typ))
+    k = torch.full((keys, 1, dim), 1024., device="cuda").to(S.dtype_of(typ))
+    k[best] = 5 * 4096.
+    return q, k, _randn(_gen(keys), typ, keys, 1, dim)
+
+
+@pytest.mark.parametrize("typ", ["bf16", "f16"])
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("keys,best", [(1, 0), (90, 3), (300, 0), (300, 150), (3000, 2999)])
+@pytest.mark.parametrize("scale", [None, 0.1, 0.3])
+def test_far_scores(typ, dim, keys, best, scale):
+    """One score stands out by so much that every other weight is below 2^-1000: the
+    output is that key's value, to the bit."""
+    import torch
+    from ktir_cpu_b200 import check_status, paged_decode, prompt_attention
+    q, k, v = _far(typ, keys, dim, best)
+    for sign in (1, -1):           # the largest score of all, or the others far below 0
+        qs, ks = (q, k) if sign > 0 else (-q, torch.where(k == k[best], 1.0, 5 * 4096.).to(k.dtype))
+        if keys == 1:
+            ks = k
+        ends = torch.tensor([0, 1, keys], dtype=torch.int32, device="cuda")
+        out = prompt_attention(qs, ks, v, ends[:2], kv_offsets=ends[::2].contiguous(), scale=scale)
+        assert torch.equal(out[0, 0], v[best, 0])
+        pages = torch.arange(keys, dtype=torch.int32, device="cuda")[None]
+        out = paged_decode(qs, ks[:, None], v[:, None], pages, ends[2:], scale=scale)
+        assert torch.equal(out[0, 0], v[best, 0])
+    check_status()
+
+
+@pytest.mark.parametrize("typ", ["bf16", "f16"])
+@pytest.mark.parametrize("size", [3000.0, 9000.0])
+def test_far_scores_close_together(typ, size):
+    """Scores of 2^27 and more, a few units apart: how the weights fall is open within
+    the scores' own rounding, but they sum to 1.  With values of 1, each output is a sum
+    of weights rounded to the element type over the sum of the unrounded ones, then
+    rounded: 1 within two unit roundoffs, the sums' 2 n 2^-24 and, in f16, 2^-25 for each
+    weight below the normal range."""
+    import torch
+    from ktir_cpu_b200 import check_status, paged_decode, prompt_attention
+    n, dim = 500, 64
+    gen = _gen(int(size))
+    base = torch.randn(1, 1, dim, generator=gen, device="cuda").sign() * size
+    q = base.expand(n, 4, dim).to(S.dtype_of(typ))
+    k = base.expand(n, 1, dim).to(S.dtype_of(typ)).clone()
+    k[torch.arange(n, device="cuda"), 0, torch.arange(n, device="cuda") % dim] = 0
+    v = torch.ones(n, 1, dim, dtype=k.dtype, device="cuda")
+    bound = 2 * S.U[typ] + 2 * n * S.E + (n * 2.0 ** -25 if typ == "f16" else 0.0)
+    ends = torch.tensor([0, n], dtype=torch.int32, device="cuda")
+    for scale in (0.3, 0.1, 1.0):
+        for keys in (k, k * torch.linspace(0.99, 1.01, n, device="cuda")[:, None, None].to(k.dtype)):
+            out = prompt_attention(q, keys, v, ends, scale=scale).double()
+            assert ((out - 1).abs() <= bound).all()
+            pages = torch.arange(n, dtype=torch.int32, device="cuda")[None]
+            out = paged_decode(q[:1], keys[:, None], v[:, None], pages, ends[1:], scale=scale).double()
+            assert ((out - 1).abs() <= bound).all()
+    check_status()
