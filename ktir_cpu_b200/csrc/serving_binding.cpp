@@ -157,7 +157,7 @@ PyObject* kv_append(PyObject* const* a) {
   const int dt = dtype_of(*k);
   if (dt < 0 || !k->is_cuda() || !vectors(*k, *k, 3) || !vectors(*v, *k, 3) || !vectors(*kc, *k, 4) ||
       !vectors(*vc, *k, 4) || !v->sizes().equals(k->sizes()) || !vc->sizes().equals(kc->sizes()) ||
-      kc->size(2) != k->size(1) || kc->size(3) != k->size(2) || !index(*slots, *k, k->size(0)))
+      kc->size(2) != k->size(1) || kc->size(2) < 1 || kc->size(3) != k->size(2) || !index(*slots, *k, k->size(0)))
     return wrong();
   if ((bool)pos != (bool)table || (out && !q)) return wrong();
   if (table && (!index(*pos, *k, k->size(0)) || table->dim() != 2 || table->scalar_type() != at::kFloat ||
@@ -171,8 +171,9 @@ PyObject* kv_append(PyObject* const* a) {
   KtirKvAppendDesc d = {};
   d.tokens = k->size(0);
   d.kv_heads = (int32_t)k->size(1);
-  d.heads = q ? (int32_t)q->size(1) : d.kv_heads;
-  if (d.tokens > 0 && d.kv_heads > 0 && d.heads > 0) {
+  const bool turn_q = q && q->size(1) > 0;        // none to rotate: keys and values are written all the same
+  d.heads = turn_q ? (int32_t)q->size(1) : d.kv_heads;
+  if (d.tokens > 0) {
     const c10::cuda::CUDAGuard guard(k->device());
     d.k = k->data_ptr();
     d.v = v->data_ptr();
@@ -186,7 +187,7 @@ PyObject* kv_append(PyObject* const* a) {
     strides(d.vc_stride, *vc);
     d.num_pages = kc->size(0);
     d.page_size = kc->size(1);
-    if (q) {
+    if (turn_q) {
       d.q = q->data_ptr();
       d.q_out = o.data_ptr();
       strides(d.q_stride, *q);

@@ -134,6 +134,8 @@ def _wrong_append(k, v, k_cache, v_cache, slots, q, positions, table, q_out):
     _cache(what, "v_cache", v_cache, k)
     _same_shape(what, "v", v, k, "k")
     tokens, kv_heads, dim = k.shape
+    if not kv_heads:
+        _fail(ValueError, what, "k and v have no heads")
     if k_cache.shape != v_cache.shape or tuple(k_cache.shape[2:]) != (kv_heads, dim):
         _fail(ValueError, what, f"caches must be [pages, page_size, {kv_heads}, {dim}], got "
                                 f"{tuple(k_cache.shape)} and {tuple(v_cache.shape)}")

@@ -675,3 +675,22 @@ def test_far_scores_close_together(typ, size):
             out = paged_decode(q[:1], keys[:, None], v[:, None], pages, ends[1:], scale=scale).double()
             assert ((out - 1).abs() <= bound).all()
     check_status()
+
+
+# -- sizes of zero ---------------------------------------------------------------------
+
+def test_append_without_heads():
+    """Queries without heads: keys and values are written all the same.  Keys without
+    heads are refused: no output is returned that nothing wrote."""
+    import torch
+    from ktir_cpu_b200 import check_status, kv_append
+    gen = _gen(50)
+    k, v = _randn(gen, "bf16", 3, 2, 64), _randn(gen, "bf16", 3, 2, 64)
+    kc, vc = (torch.zeros(2, 4, 2, 64, dtype=torch.bfloat16, device="cuda") for _ in range(2))
+    slots = torch.tensor([5, 0, 2], dtype=torch.int32, device="cuda")
+    out = kv_append(k, v, kc, vc, slots, q=k[:, :0])
+    assert out.shape == (3, 0, 64)
+    assert torch.equal(kc.flatten(0, 1)[slots.long()], k) and torch.equal(vc.flatten(0, 1)[slots.long()], v)
+    with pytest.raises(ValueError, match="no heads"):
+        kv_append(k[:, :0], v[:, :0], kc[:, :, :0], vc[:, :, :0], slots, q=k)
+    check_status()
