@@ -434,7 +434,10 @@ int ktir_host_download(const KtirHostXfer* x, int n, const KtirHostCopy* extra, 
  * (x_2i, x_2i+1) when interleaved, of a vector's first `rot` elements by
  * table[position][i] = cos and table[position][rot/2 + i] = sin, in f32,
  * rounded once; the elements after `rot` are copied.  rot = 0: plain copy, no
- * positions or table needed.  The slots of one call are distinct. */
+ * positions or table needed.  The slots of one call are distinct.  A token whose
+ * slot is past the cache is not written to it; one whose position is not in the
+ * table isn't either, and its q_out is zero.  The position of padding is not
+ * reported. */
 typedef struct {
   const void* q; const void* k; const void* v;   /* [tokens][heads][dim]; q may be null */
   void* q_out;

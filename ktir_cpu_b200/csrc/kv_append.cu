@@ -100,9 +100,11 @@ __global__ void __launch_bounds__(THREADS, SEVERAL ? RESIDENT : 0) k_kv_append(c
   pdl_wait();
   const int slot = d.slots[t];
   const int pos = rparts ? d.positions[t] : 0;
-  const bool bad = slot >= p.slots_total || (rparts && (pos < 0 || pos >= d.table_rows));
+  // A bad slot leaves the token's key and value out, a bad position makes its query
+  // zeros as well (never what the memory held before).
+  const bool lost = rparts && (pos < 0 || pos >= d.table_rows);
+  const bool kept = slot >= 0 && slot < p.slots_total && !lost;
   float c[8], s[8];
-  const bool kept = slot >= 0 && !bad;
   const long long page = kept ? slot / d.page_size : 0;
   const long long place = kept ? slot - page * d.page_size : 0;
   for (int h0 = hl; h0 < n; h0 += UNROLL * lanes) {
@@ -119,11 +121,8 @@ __global__ void __launch_bounds__(THREADS, SEVERAL ? RESIDENT : 0) k_kv_append(c
       }
     }
     if (h0 == hl) {                             // the vectors are on their way meanwhile
-      if (bad) {
-        if (hl == 0 && j == 0) atomicOr(d.status, KTIR_STATUS_BAD_INDEX);
-        return;
-      }
-      if (turn) {
+      if (!kept && slot >= 0 && hl == 0 && j == 0) atomicOr(d.status, KTIR_STATUS_BAD_INDEX);
+      if (turn && !lost) {
         const float* row = d.table + (long long)pos * d.table_stride + 8 * j;
         if (p.vector_table) {
 #pragma unroll
@@ -145,7 +144,9 @@ __global__ void __launch_bounds__(THREADS, SEVERAL ? RESIDENT : 0) k_kv_append(c
       const int h = h0 + u * lanes;
       if (h >= n || (h >= hq && !kept)) continue;
       uint4 x = a[u], y = b[u];
-      if (turn && h < hk) {
+      if (lost) {
+        x = y = make_uint4(0, 0, 0, 0);
+      } else if (turn && h < hk) {
         if (d.interleaved) {
           x = rotate_pairs<T>(a[u], c, s, 0);
           y = rotate_pairs<T>(b[u], c, s, 4);

@@ -168,7 +168,10 @@ def kv_append(k, v, k_cache, v_cache, slots, q=None, positions=None, table=None,
     ``rotary_table``) and `positions` [tokens] int32, the first rot elements of
     every key are rotated by their position, in pairs (i, i + rot/2) or, when
     `interleaved`, (2i, 2i+1).  q [tokens, heads, dim], when given, is rotated
-    likewise and returned (into `q_out`, which may be q itself)."""
+    likewise and returned (into `q_out`, which may be q itself).  A token whose slot
+    is past the cache is not written to it; one whose position is not in the table
+    isn't either, and its query comes back as zeros (both reported by
+    ``check_status``; the position of padding is not)."""
     r = _ext().kv_append(k, v, k_cache, v_cache, slots, q, positions, table, interleaved, q_out)
     if r is NotImplemented:
         _wrong_append(k, v, k_cache, v_cache, slots, q, positions, table, q_out)

@@ -694,3 +694,55 @@ def test_append_without_heads():
     with pytest.raises(ValueError, match="no heads"):
         kv_append(k[:, :0], v[:, :0], kc[:, :, :0], vc[:, :, :0], slots, q=k)
     check_status()
+
+
+def _fill_free_memory(value=7.0):
+    """Whatever is allocated next holds `value` until something is written."""
+    import torch
+    for n in (10, 14, 18, 22):
+        blocks = [torch.full((1 << n,), value, dtype=torch.bfloat16, device="cuda") for _ in range(8)]
+        del blocks
+
+
+@pytest.mark.parametrize("tokens,kv_heads", [(6, 2), (2500, 1)])       # one token per block, and several
+@pytest.mark.parametrize("rot", [0, 32, 64])
+def test_append_bad_indices_leave_no_row_unwritten(tokens, kv_heads, rot):
+    """A query does not depend on its token's slot; one without a position is zero."""
+    import torch
+    from ktir_cpu_b200 import check_status, kv_append, rotary_table
+    gen = _gen(51)
+    q, k, v = (_randn(gen, "bf16", tokens, kv_heads, 64) for _ in range(3))
+    page = 25
+    kc, vc = (torch.zeros(tokens // page + 1, page, kv_heads, 64, dtype=torch.bfloat16, device="cuda") for _ in range(2))
+    slots = torch.arange(tokens, dtype=torch.int32, device="cuda")
+    positions = slots % 10
+    args = dict(positions=positions, table=rotary_table(10, rot)) if rot else {}
+    want = kv_append(k, v, kc.clone(), vc.clone(), slots, q=q, **args)
+    check_status()
+
+    # padding without a position: nothing to report
+    slots[1], slots[2], positions[2] = -1, -1, -1
+    _fill_free_memory()
+    got = kv_append(k, v, kc, vc, slots, q=q, **args)
+    check_status()
+    if rot:
+        assert not got[2].any()
+    same = torch.ones(tokens, dtype=torch.bool, device="cuda")
+    same[2] = not rot
+    assert torch.equal(got[same], want[same])
+
+    slots[0] = kc.shape[0] * page                   # past the cache
+    positions[3], positions[4] = 10, -1             # not in the table
+    kc.zero_(), vc.zero_()
+    _fill_free_memory()
+    got = kv_append(k, v, kc, vc, slots, q=q, **args)
+    with pytest.raises(IndexError):
+        check_status()
+    if rot:
+        assert not got[2:5].any()
+        same[3:5] = False
+    assert torch.equal(got[same], want[same])
+    written = same & (slots >= 0)
+    written[0] = False
+    assert torch.equal(vc.flatten(0, 1)[:tokens][written], v[written])
+    assert not vc.flatten(0, 1)[:tokens][~written].any() and not kc.flatten(0, 1)[:tokens][~written].any()
