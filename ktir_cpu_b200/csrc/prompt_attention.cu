@@ -144,6 +144,7 @@ struct Shared {
   int weights[WEIGHTS];             // tiles of at least this weight
   uint32_t tmem_base;
   int abort_flag;
+  int gaps;                         // offsets out of their range, or tokens outside all sequences
 };
 
 
@@ -498,6 +499,7 @@ __global__ void __launch_bounds__(THREADS, 1)
 
   if (tid == 0) {
     B.abort_flag = 0;
+    B.gaps = 0;
     for (int w = 0; w < 2; ++w) {
       mbar_init(smem_u32(&B.q_full[w]), 1);
       mbar_init(smem_u32(&B.q_empty[w]), 1);
@@ -552,7 +554,7 @@ __global__ void __launch_bounds__(THREADS, 1)
       const int half = p.tile_tokens;
       int heaviest = 0, singles = 0, pairs = 0;
       bool any_bad = false;
-      const int ends = blockIdx.x == 0 ? d.offsets[0] | (d.offsets[d.batch] ^ (int)d.tokens) : 0;   // 0 if they cover the tokens
+      const int ends = d.offsets[0] | (d.offsets[d.batch] ^ (int)d.tokens);   // 0 if they cover the tokens
       for (long long b = lane; b < d.batch; b += 32) {
         bool bad;
         const Seq s = sequence(d, b, bad);
@@ -563,8 +565,10 @@ __global__ void __launch_bounds__(THREADS, 1)
         singles += tiles;
         pairs += (tiles + 1) / 2;
       }
-      if (blockIdx.x == 0) {
-        if (any_bad || (lane == 0 && ends)) atomicOr(d.status, KTIR_STATUS_BAD_INDEX);
+      any_bad = __any_sync(0xffffffffu, any_bad || ends);
+      if (lane == 0) {
+        B.gaps = any_bad;
+        if (any_bad && blockIdx.x == 0) atomicOr(d.status, KTIR_STATUS_BAD_INDEX);
       }
       __syncwarp();
       heaviest = (int)__reduce_max_sync(0xffffffffu, (unsigned)heaviest);
@@ -1205,6 +1209,24 @@ __global__ void __launch_bounds__(THREADS, 1)
         for (int i = 0; i < D; i += 64) store_rows(i, v);
       }
       if (store && d.lse) d.lse[tok * d.heads + head] = l == 0.f ? -INFINITY : (m + log2f(l)) * LN2;
+    }
+    // Bad offsets: tokens of no sequence get zeros, not what the memory held before.
+    // Nothing else writes them.
+    if (B.gaps && !*abort) {
+      for (long long at = (long long)blockIdx.x * 256 + tid; at < d.tokens; at += (long long)gridDim.x * 256) {
+        bool covered = false;
+        for (long long b = 0; b < d.batch && !covered; ++b) {
+          bool bad;
+          const long long n = sequence(d, b, bad).n, from = at - d.offsets[b];
+          covered = from >= 0 && from < n;
+        }
+        if (covered) continue;
+        for (int h = 0; h < d.heads; ++h) {
+          T* out = static_cast<T*>(d.out) + at * d.out_stride[0] + h * d.out_stride[1];
+          for (int i = 0; i < D; i += 8) *reinterpret_cast<uint4*>(out + i) = make_uint4(0, 0, 0, 0);
+          if (d.lse) d.lse[at * d.heads + h] = -INFINITY;
+        }
+      }
     }
   }
   tc_fence_before();

@@ -245,8 +245,8 @@ def prompt_attention(q, k, v, offsets, kv_offsets=None, causal=True, scale=None,
     - 1 (default: offsets).  A causal mask is aligned at the end: query i of n
     sees keys j <= i + m - n of m, so later pieces of a prompt attend to its
     earlier ones.  heads is a multiple of kv_heads, scale defaults to dim **
-    -0.5.  Returns out [tokens, heads, dim], zero where a query sees no key; with
-    `return_lse` also the f32 [tokens, heads] logarithm of each row's sum of
+    -0.5.  Returns out [tokens, heads, dim], zero where a query sees no key (and, if
+    offsets are bad, where it belongs to no sequence); with `return_lse` also the f32 [tokens, heads] logarithm of each row's sum of
     exponentials."""
     r = _ext().prompt_attention(q, k, v, offsets, kv_offsets, causal, scale, out, return_lse)
     if r is NotImplemented:

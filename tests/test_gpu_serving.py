@@ -746,3 +746,33 @@ def test_append_bad_indices_leave_no_row_unwritten(tokens, kv_heads, rot):
     written[0] = False
     assert torch.equal(vc.flatten(0, 1)[:tokens][written], v[written])
     assert not vc.flatten(0, 1)[:tokens][~written].any() and not kc.flatten(0, 1)[:tokens][~written].any()
+
+
+@pytest.mark.parametrize("heads,kv_heads,dim", [(4, 2, 128), (3, 1, 64), (64, 2, 64)])
+@pytest.mark.parametrize("offsets,kv_offsets,valid", [
+    ([0, 50, 111], [0, 60, 110], [0]),               # past the tokens
+    ([0, 50, 20, 100], [0, 60, 80, 110], []),        # falling: rows 20 to 49 are two sequences', either may stay
+    ([-1, 50, 100], [0, 60, 110], [1]),
+    ([0, 50, 100], [0, 60, 300], [0]),               # keys past their tokens
+    ([0, 50, 100], [0, 120, 110], []),
+    ([7, 50, 90], [0, 60, 110], [0, 1]),             # tokens before the first sequence and after the last
+    ([0, 0, 0], [0, 60, 110], []),
+])
+def test_prompt_bad_offsets_leave_no_row_unwritten(heads, kv_heads, dim, offsets, kv_offsets, valid):
+    import torch
+    from ktir_cpu_b200 import check_status, prompt_attention
+    q, k, v, _, _ = _prompt_inputs("bf16", [100], [110], heads, kv_heads, dim, seed=52)
+    index = lambda x: torch.tensor(x, dtype=torch.int32, device="cuda")  # noqa: E731
+    _fill_free_memory()
+    out, lse = prompt_attention(q, k, v, index(offsets), kv_offsets=index(kv_offsets), return_lse=True)
+    with pytest.raises(IndexError):
+        check_status()
+    free = torch.ones(100, dtype=torch.bool, device="cuda")
+    for b, (lo, hi, k0, k1) in enumerate(zip(offsets, offsets[1:], kv_offsets, kv_offsets[1:])):
+        if 0 <= lo <= hi <= 100 and 0 <= k0 <= k1 <= 110:
+            free[lo:hi] = False
+        if b in valid:
+            _check_prompt("bf16", q[lo:hi], k[k0:k1], v[k0:k1], index([0, hi - lo]), index([0, k1 - k0]), True,
+                          dim ** -0.5, out[lo:hi], lse[lo:hi])
+    assert not out[free].any() and (lse[free] == -math.inf).all()
+    check_status()
