@@ -25,8 +25,9 @@
 //
 // Precision: scores, m, l and o in f32; the weights p are rounded to the
 // element type for the second product (as the values are), at most one half
-// ulp each.  m moves only when the maximum grows by more than 2^8, so p stays
-// below 2^8 and the largest p of a row is at least 1.
+// ulp each (in f16 2^-32 of a row's largest where that is more).  m moves only when
+// the maximum grows by more than 2^8, so the largest p of a row lies between 1 and 2^8,
+// and in f16, where m is kept 2^7 lower (Elem::LIFT), between 2^7 and 2^15.
 #include "serve_common.cuh"
 
 using namespace ktir::serve;
@@ -492,10 +493,11 @@ __global__ void __launch_bounds__(THREADS, Cfg<D>::CTAS_PER_SM)
         top[x] = fmaxf(top[x], __shfl_xor_sync(0xffffffffu, top[x], 16));
       }
       if (__any_sync(0xffffffffu,
-                     top[0] - m[h][0] > RESCALE_THRESHOLD || top[1] - m[h][1] > RESCALE_THRESHOLD)) {
+                     top[0] - m[h][0] > RESCALE_THRESHOLD + Elem<T>::LIFT ||
+                         top[1] - m[h][1] > RESCALE_THRESHOLD + Elem<T>::LIFT)) {
 #pragma unroll
         for (int x = 0; x < 2; ++x) {
-          const float mn = fmaxf(m[h][x], top[x]);
+          const float mn = fmaxf(m[h][x], top[x] - Elem<T>::LIFT);
           const float f = mn == -INFINITY ? 1.f : ex2(m[h][x] - mn);
           m[h][x] = mn;
           l[h][x] *= f;

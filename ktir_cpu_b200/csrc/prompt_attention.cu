@@ -41,10 +41,12 @@
 // TMEM holds S, P and O of both row tiles apart, which at dim 128 leaves room for
 // blocks of 80 keys (128 at dim 64).
 // The running maximum moves only when a row's maximum exceeds it by more than
-// 2^8; O's rows are then rescaled in TMEM, after the product before.
+// 2^8; O's rows are then rescaled in TMEM, after the product before.  In f16 it is kept
+// 2^7 lower than it is (Elem::LIFT).
 // Precision: S, O, m and l in f32; P is rounded to the element type for the
 // second product (tcgen05 wants one type for both operands), half an ulp per
-// weight; l adds the unrounded weights.
+// weight (in f16 2^-32 of a row's largest where that is more); l adds the unrounded
+// weights.
 // Measured, 8192 tokens of 32 heads over 8, causal: dim 128 459 us in a short burst
 // (1,200 TFLOP/s) and 531 under the power cap, dim 64 365 us.  Of a block's 2,100
 // cycles (80 keys, both row tiles) the exponentials take 1,300; both groups of softmax
@@ -955,13 +957,16 @@ __global__ void __launch_bounds__(THREADS, 1)
 #pragma unroll
           for (int x = 0; x < 4; ++x) m4[x] = max3(m4[x], s[i + x], s[i + 4 + x]);
         const float s_top = fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3])), top = __fmul_rn(s_top, c);
-        const bool move = top - m > RESCALE_THRESHOLD;     // also from -inf (m + 8 may round to m + 16)
+        const bool move = top - m > RESCALE_THRESHOLD + Elem<T>::LIFT;     // also from -inf (m + 8 may round to m + 16)
         bool done = j == 0;                                // PV of the block before
         if (__any_sync(0xffffffffu, move || from != 0.f)) {
-          const float f = move ? ex2(m - top) : 1.f;
+          float f = 1.f;
           if (move) {
-            m = top;
-            from = fabsf(m) >= FAR ? -s_top : 0.f;
+            const bool is_far = fabsf(top) >= FAR;
+            const float mn = is_far ? top : top - Elem<T>::LIFT;
+            f = ex2(m - mn);
+            m = mn;
+            from = is_far ? -s_top : 0.f;
           }
           l *= f;
           if (j) {

@@ -21,6 +21,11 @@ constexpr float LN2 = 0.6931471805599453f;
 template <typename T> struct Elem;
 template <> struct Elem<__half> {
   static constexpr bool BF16 = false;
+  // log2 of what softmax weights are scaled up by (and their sum with them): f16 has no
+  // more than 2^-24 below 1, and many small weights of a long row count.  From 1 to 2^8
+  // of themselves, the largest of a row's weights are then 2^7 to 2^15, and one is lost
+  // from 2^-32 of the largest down (131,072 keys: 2^-15 of the sum, unscaled 2^-8).
+  static constexpr float LIFT = 7.0f;
   static __device__ __forceinline__ float2 to2(uint32_t v) {
     return __half22float2(*reinterpret_cast<const __half2*>(&v));
   }
@@ -31,6 +36,7 @@ template <> struct Elem<__half> {
 };
 template <> struct Elem<__nv_bfloat16> {
   static constexpr bool BF16 = true;
+  static constexpr float LIFT = 0.0f;         // as much range as f32
   static __device__ __forceinline__ float2 to2(uint32_t v) {
     return make_float2(__uint_as_float(v << 16), __uint_as_float(v & 0xffff0000u));
   }

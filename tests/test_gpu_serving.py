@@ -776,3 +776,40 @@ def test_prompt_bad_offsets_leave_no_row_unwritten(heads, kv_heads, dim, offsets
                           dim ** -0.5, out[lo:hi], lse[lo:hi])
     assert not out[free].any() and (lse[free] == -math.inf).all()
     check_status()
+
+
+@pytest.mark.parametrize("first", [True, False])      # the largest weight's key
+@pytest.mark.parametrize("heads", [1, 160, 600])      # shared out over the keys, and not
+@pytest.mark.parametrize("dim", [64, 128])
+def test_f16_many_small_weights(dim, heads, first):
+    """131,071 keys of weight 2^-25.5 beside one of weight 1: 0.0028 of the sum, each
+    weight below what f16 holds next to 1.  A weight is good to 2^-32 of the largest."""
+    import torch
+    from ktir_cpu_b200 import check_status, paged_decode, prompt_attention
+    n, page = 131072, 64
+    at = 0 if first else n - 1
+    q = torch.zeros(1, heads, dim, dtype=torch.float16, device="cuda")
+    q[..., 0] = 1
+    k = torch.zeros(n, 1, dim, dtype=torch.float16, device="cuda")
+    k[..., 0] = -25.5
+    k[at] = 0
+    v = torch.ones_like(k)
+    v[at] = 0
+    scale = math.log(2.0)
+    small = (n - 1) * 2.0 ** -25.5
+    want = small / (1 + small)
+    score = (dim + 4) * S.E * 25.5 * scale + 2.0 ** -21
+    bound = S.U["f16"] * want + (S.U["f16"] + 2 * score + 2 * S.E * n) * want + 2.0 ** -32 * n + 2.0 ** -25
+    lim = score + S.E * n + 2 * S.E
+    ends = torch.tensor([0, 1, n], dtype=torch.int32, device="cuda")
+    shared = lambda x: x.expand(-1, heads, -1)  # noqa: E731
+    out, lse = prompt_attention(q, shared(k), shared(v), ends[:2], kv_offsets=ends[::2].contiguous(), scale=scale,
+                                return_lse=True)
+    assert ((out.double() - want).abs() <= bound).all(), float((out.double() - want).abs().max() / bound)
+    assert ((lse.double() - math.log1p(small)).abs() <= lim).all()
+    paged = lambda x: x.view(n // page, page, 1, dim).expand(-1, -1, heads, -1)  # noqa: E731
+    out, lse = paged_decode(q, paged(k), paged(v), torch.arange(n // page, dtype=torch.int32, device="cuda")[None],
+                            ends[2:], scale=scale, return_lse=True)
+    assert ((out.double() - want).abs() <= bound).all(), float((out.double() - want).abs().max() / bound)
+    assert ((lse.double() - math.log1p(small)).abs() <= lim).all()
+    check_status()
