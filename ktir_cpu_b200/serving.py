@@ -46,7 +46,9 @@ def _ext():
 
 def check_status(device=None) -> None:
     """Wait for `device` (default: the current one) and raise for what the
-    serving operators have reported there since the last check."""
+    serving operators have reported there since the last check: RuntimeError if a
+    wait inside a kernel ran out (some of the outputs since then were given up),
+    else IndexError for an index out of range."""
     dev = torch.cuda.current_device() if device is None else torch.device(device).index
     if dev is None:
         dev = torch.cuda.current_device()
@@ -58,10 +60,11 @@ def check_status(device=None) -> None:
     if v:
         t.zero_()
         torch.cuda.synchronize(dev)
+    index = "a page, slot, position, length or offset of a serving operator is out of range"
+    if v & R.STATUS_TIMEOUT:             # the graver one: an IndexError alone would let the outputs pass
+        raise RuntimeError("device wait timed out" + (f"; and {index}" if v & R.STATUS_BAD_INDEX else ""))
     if v & R.STATUS_BAD_INDEX:
-        raise IndexError("a page, slot, position, length or offset of a serving operator is out of range")
-    if v & R.STATUS_TIMEOUT:
-        raise RuntimeError("device wait timed out")
+        raise IndexError(index)
 
 
 # -- what is wrong with a call that did not pass its operator's check ----------------

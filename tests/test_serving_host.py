@@ -142,3 +142,36 @@ def test_cpu_tensors_are_refused():
         prompt_attention(x, x, x, i)
     with pytest.raises(ValueError, match="CUDA"):
         kv_append(x, x, c, c, i)
+
+
+class _FakeBinding:
+    """The binding's status word of one device, in host memory."""
+
+    def __init__(self, value):
+        import torch
+        self.word = torch.tensor([value], dtype=torch.int32)
+
+    def status(self, dev):
+        return self.word
+
+
+@pytest.mark.parametrize("bits,kind,text", [
+    (0, None, None), ("bad", IndexError, "out of range"), ("timeout", RuntimeError, "timed out"),
+    ("both", RuntimeError, "timed out.*out of range"),
+])
+def test_check_status_reports_every_bit(monkeypatch, bits, kind, text):
+    torch = pytest.importorskip("torch")
+    from ktir_cpu_b200 import runtime as R
+    from ktir_cpu_b200 import serving
+    value = {0: 0, "bad": R.STATUS_BAD_INDEX, "timeout": R.STATUS_TIMEOUT,
+             "both": R.STATUS_BAD_INDEX | R.STATUS_TIMEOUT}[bits]
+    fake = _FakeBinding(value)
+    monkeypatch.setattr(serving, "_EXT", fake)
+    monkeypatch.setattr(torch.cuda, "synchronize", lambda dev=None: None)
+    if kind is None:
+        serving.check_status(0)
+    else:
+        with pytest.raises(kind, match=text):
+            serving.check_status(0)
+    assert int(fake.word) == 0
+    serving.check_status(0)
