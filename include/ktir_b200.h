@@ -493,7 +493,9 @@ int ktir_paged_decode(const KtirPagedDecodeDesc* desc, void* stream);
  * -inf), as does one of no sequence, where offsets are out of range.  lse as above, [tokens][heads].  dim 64 or 128; heads / kv_heads at
  * most 128.  With a workspace (ktir_prompt_attention_workspace() bytes, zero
  * before its first use, its own for calls that may overlap) few queries over
- * many keys share the keys among the SMs. */
+ * many keys share the keys among the SMs.  Should KTIR_STATUS_TIMEOUT be set,
+ * outputs of calls since the word was clear were given up, and their workspace
+ * must be cleared before its next use. */
 typedef struct {
   const void* q;                 /* [tokens][heads][dim] */
   const void* k; const void* v;  /* [kv_tokens][kv_heads][dim] */

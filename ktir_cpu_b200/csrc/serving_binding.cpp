@@ -314,6 +314,15 @@ PyObject* status(PyObject* const* a) {
   return THPVariable_Wrap(g_status[dev]);
 }
 
+// the kept workspaces of a device are given up: the next calls get cleared ones
+PyObject* forget(PyObject* const* a) {
+  const long dev = PyLong_AsLong(a[0]);
+  if (dev == -1 && PyErr_Occurred()) throw Failed();
+  for (auto* kept : {&g_decode, &g_prompt})
+    for (auto it = kept->begin(); it != kept->end();) it = it->first.first == dev ? kept->erase(it) : std::next(it);
+  Py_RETURN_NONE;
+}
+
 // no C++ exception leaves a call
 template <PyObject* (*F)(PyObject* const*), int N>
 PyObject* entry(PyObject*, PyObject* const* args, Py_ssize_t n) {
@@ -340,6 +349,7 @@ PyMethodDef g_methods[] = {
     {"paged_decode", method<paged_decode, 8>(), METH_FASTCALL, nullptr},
     {"prompt_attention", method<prompt_attention, 9>(), METH_FASTCALL, nullptr},
     {"status", method<status, 1>(), METH_FASTCALL, nullptr},
+    {"forget", method<forget, 1>(), METH_FASTCALL, nullptr},
     {nullptr, nullptr, 0, nullptr}};
 
 PyModuleDef g_module = {PyModuleDef_HEAD_INIT, "_serving", nullptr, -1, g_methods, nullptr, nullptr, nullptr, nullptr};

@@ -62,6 +62,7 @@ def check_status(device=None) -> None:
         torch.cuda.synchronize(dev)
     index = "a page, slot, position, length or offset of a serving operator is out of range"
     if v & R.STATUS_TIMEOUT:             # the graver one: an IndexError alone would let the outputs pass
+        _ext().forget(dev)               # the call that was given up may have left counters part-counted
         raise RuntimeError("device wait timed out" + (f"; and {index}" if v & R.STATUS_BAD_INDEX else ""))
     if v & R.STATUS_BAD_INDEX:
         raise IndexError(index)

@@ -813,3 +813,25 @@ def test_f16_many_small_weights(dim, heads, first):
     assert ((out.double() - want).abs() <= bound).all(), float((out.double() - want).abs().max() / bound)
     assert ((lse.double() - math.log1p(small)).abs() <= lim).all()
     check_status()
+
+
+def test_workspaces_after_a_reported_timeout():
+    """The status word as a wait that ran out leaves it: the kept workspaces go, and the
+    next calls, split and not, are right."""
+    import torch
+    from ktir_cpu_b200 import check_status, paged_decode, prompt_attention, runtime, serving
+    q, k, v, offsets, kv_offsets = _prompt_inputs("bf16", [64], [8192], 8, 2, 128, seed=53)
+    x = _decode_inputs("bf16", [3000, 40], 8, 2, 128, 16, seed=53)
+    want, want2 = prompt_attention(q, k, v, offsets, kv_offsets=kv_offsets), paged_decode(*x)
+    check_status()
+    device = torch.cuda.current_device()
+    before = torch.cuda.memory_allocated()
+    serving._ext().status(device).fill_(runtime.STATUS_TIMEOUT)
+    with pytest.raises(RuntimeError, match="timed out"):
+        check_status()
+    # parts of both operators: 16 rows of 130 floats twice for 512 CTAs, 128 rows of 130 for 160
+    assert before - torch.cuda.memory_allocated() >= 4 * 130 * (512 * 2 * 16 + 160 * 128)
+    for _ in range(3):
+        assert torch.equal(prompt_attention(q, k, v, offsets, kv_offsets=kv_offsets), want)
+        assert torch.equal(paged_decode(*x), want2)
+    check_status()

@@ -150,6 +150,10 @@ class _FakeBinding:
     def __init__(self, value):
         import torch
         self.word = torch.tensor([value], dtype=torch.int32)
+        self.forgotten = []
+
+    def forget(self, dev):
+        self.forgotten.append(dev)
 
     def status(self, dev):
         return self.word
@@ -175,3 +179,17 @@ def test_check_status_reports_every_bit(monkeypatch, bits, kind, text):
             serving.check_status(0)
     assert int(fake.word) == 0
     serving.check_status(0)
+
+
+@pytest.mark.parametrize("timeout", [False, True])
+def test_workspaces_are_given_up_after_a_timeout(monkeypatch, timeout):
+    """A split call that was given up leaves counters that a later call would take for its own."""
+    torch = pytest.importorskip("torch")
+    from ktir_cpu_b200 import runtime as R
+    from ktir_cpu_b200 import serving
+    fake = _FakeBinding(R.STATUS_TIMEOUT if timeout else R.STATUS_BAD_INDEX)
+    monkeypatch.setattr(serving, "_EXT", fake)
+    monkeypatch.setattr(torch.cuda, "synchronize", lambda dev=None: None)
+    with pytest.raises(RuntimeError if timeout else IndexError):
+        serving.check_status(3)
+    assert fake.forgotten == ([3] if timeout else [])
