@@ -80,10 +80,16 @@ struct Arg {
   const at::Tensor& operator*() const { return *t; }
 };
 
-// a tensor of head vectors of the call's type and device, without a gradient to lose
+// a gradient, or a tangent of forward mode, that the operators would lose
+bool differentiated(const at::Tensor& t) {
+  return (t.requires_grad() && at::GradMode::is_enabled()) ||
+         (c10::AutogradState::get_tls_state().get_fw_grad_mode() && t._fw_grad(0).defined());
+}
+
+// a tensor of head vectors of the call's type and device
 bool vectors(const at::Tensor& t, const at::Tensor& like, int dims) {
   return t.dim() == dims && t.scalar_type() == like.scalar_type() && t.device() == like.device() &&
-         t.stride(dims - 1) == 1 && !(t.requires_grad() && at::GradMode::is_enabled());
+         t.stride(dims - 1) == 1 && !differentiated(t);
 }
 
 // an int32 index array of n entries on the call's device
@@ -161,7 +167,7 @@ PyObject* kv_append(PyObject* const* a) {
     return wrong();
   if ((bool)pos != (bool)table || (out && !q)) return wrong();
   if (table && (!index(*pos, *k, k->size(0)) || table->dim() != 2 || table->scalar_type() != at::kFloat ||
-                table->device() != k->device() || table->stride(1) != 1))
+                table->device() != k->device() || table->stride(1) != 1 || differentiated(*table)))
     return wrong();
   at::Tensor o;
   if (q) {

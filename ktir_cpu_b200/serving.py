@@ -80,6 +80,13 @@ def _kind(what, t):
         _fail(NotImplementedError, what, f"needs float16 or bfloat16, got {t.dtype}")
 
 
+def _no_gradient(what, name, t):
+    if t.requires_grad and torch.is_grad_enabled():
+        _fail(RuntimeError, what, f"{name} requires a gradient, which this operator does not have")
+    if torch._C._is_fwd_grad_enabled() and torch.autograd.forward_ad.unpack_dual(t).tangent is not None:
+        _fail(RuntimeError, what, f"{name} has a forward-mode tangent, which this operator does not carry on")
+
+
 def _vectors(what, name, t, like, layout):
     """A tensor of head vectors, of the call's type and device."""
     if t.dim() != layout.count(",") + 1:
@@ -88,8 +95,7 @@ def _vectors(what, name, t, like, layout):
         _fail(ValueError, what, f"{name} must be {like.dtype} on {like.device}, got {t.dtype} on {t.device}")
     if t.stride(-1) != 1:
         _fail(NotImplementedError, what, f"{name}'s head vectors must be contiguous")
-    if t.requires_grad and torch.is_grad_enabled():
-        _fail(RuntimeError, what, f"{name} requires a gradient, which this operator does not have")
+    _no_gradient(what, name, t)
 
 
 def _heads(what, name, t, like):
@@ -150,6 +156,7 @@ def _wrong_append(k, v, k_cache, v_cache, slots, q, positions, table, q_out):
         _index(what, "positions", positions, (tokens,), k)
         if table.dim() != 2 or table.dtype != torch.float32 or table.device != k.device or table.stride(1) != 1:
             _fail(ValueError, what, f"table must be f32 [positions, rot] on {k.device}, rows contiguous")
+        _no_gradient(what, "table", table)
     if q is not None:
         _heads(what, "q", q, k)
         if q.shape[0] != tokens or q.shape[2] != dim:

@@ -835,3 +835,35 @@ def test_workspaces_after_a_reported_timeout():
         assert torch.equal(prompt_attention(q, k, v, offsets, kv_offsets=kv_offsets), want)
         assert torch.equal(paged_decode(*x), want2)
     check_status()
+
+
+def test_gradients_and_tangents_are_refused():
+    """Neither a gradient nor a forward-mode tangent is lost without a word."""
+    import torch
+    import torch.autograd.forward_ad as fw
+    from ktir_cpu_b200 import check_status, kv_append, paged_decode, prompt_attention, rotary_table
+    q, kc, vc, pages, lengths = _decode_inputs("bf16", [40, 20], 4, 2, 64, 16, seed=54)
+    k, v = kc[0, :2].clone(), vc[0, :2].clone()
+    off = torch.tensor([0, 2], dtype=torch.int32, device="cuda")
+    table = rotary_table(8, 64)
+    calls = {
+        "append": lambda q, k, v, kc, vc, t: kv_append(k, v, kc, vc, off, q=q, positions=off, table=t),
+        "decode": lambda q, k, v, kc, vc, t: paged_decode(q, kc, vc, pages, lengths),
+        "prompt": lambda q, k, v, kc, vc, t: prompt_attention(q, k, v, off),
+    }
+    takes = {"append": (0, 1, 2, 3, 4, 5), "decode": (0, 3, 4), "prompt": (0, 1, 2)}
+    for name, call in calls.items():
+        for at in takes[name]:
+            args = [q, k, v, kc, vc, table]
+            with fw.dual_level():
+                args[at] = fw.make_dual(args[at], torch.ones_like(args[at]))
+                with pytest.raises(RuntimeError, match="tangent"):
+                    call(*args)
+                with fw._set_fwd_grad_enabled(False):
+                    call(*args)
+            args[at] = [q, k, v, kc, vc, table][at].clone().requires_grad_()
+            with pytest.raises(RuntimeError, match="gradient"):
+                call(*args)
+            with torch.no_grad():
+                call(*args)
+    check_status()
