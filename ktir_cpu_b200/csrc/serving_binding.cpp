@@ -134,6 +134,11 @@ at::Tensor fresh(at::IntArrayRef sizes, at::ScalarType type, at::Device device) 
   return at::Tensor(at::detail::empty_cuda(sizes, type, device, c10::nullopt));
 }
 
+// a caller's tensor that was written: autograd sees that what it saved of it has changed
+void written(const at::Tensor& t) {
+  if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
+}
+
 // out (given, or new) of q's shape
 bool output(const Arg& out, const at::Tensor& q, at::Tensor& o) {
   if (out) {
@@ -210,6 +215,9 @@ PyObject* kv_append(PyObject* const* a) {
     d.interleaved = flag(a[8]);
     d.dtype = dt;
     check(ktir_kv_append(&d, c10::cuda::getCurrentCUDAStream(k->get_device()).stream()));
+    written(*kc);
+    written(*vc);
+    if (turn_q && out) written(o);
   }
   if (!q) Py_RETURN_NONE;
   return result(a[9], o, at::Tensor());
@@ -261,6 +269,7 @@ PyObject* paged_decode(PyObject* const* a) {
     d.dtype = dt;
     d.scale = scale_of(a[5], q->size(2));
     check(ktir_paged_decode(&d, stream));
+    if (out) written(o);
   }
   return result(a[6], o, lse);
 }
@@ -308,6 +317,7 @@ PyObject* prompt_attention(PyObject* const* a) {
     d.scale = scale_of(a[6], q->size(2));
     d.causal = flag(a[5]);
     check(ktir_prompt_attention(&d, stream));
+    if (out) written(o);
   }
   return result(a[7], o, lse);
 }

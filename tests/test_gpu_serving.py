@@ -867,3 +867,33 @@ def test_gradients_and_tangents_are_refused():
             with torch.no_grad():
                 call(*args)
     check_status()
+
+
+def test_written_tensors_are_seen_as_changed():
+    """Caches and given outputs count as written in place, inputs do not; a tensor saved
+    for a gradient and written since is found out."""
+    import torch
+    from ktir_cpu_b200 import check_status, kv_append, paged_decode, prompt_attention
+    q, kc, vc, pages, lengths = _decode_inputs("bf16", [40, 20], 4, 2, 64, 16, seed=55)
+    k, v = kc[0, :2].clone(), vc[0, :2].clone()
+    off = torch.tensor([0, 2], dtype=torch.int32, device="cuda")
+    out, q_out = torch.empty_like(q), torch.empty_like(q)
+    read, write = (q, k, v, pages, lengths, off), (kc, vc, q_out, out)
+    for call, moves in [(lambda: kv_append(k, v, kc, vc, off, q=q, q_out=q_out), (1, 1, 1, 0)),
+                        (lambda: kv_append(k, v, kc, vc, off), (1, 1, 0, 0)),
+                        (lambda: paged_decode(q, kc, vc, pages, lengths, out=out), (0, 0, 0, 1)),
+                        (lambda: prompt_attention(q, k, v, off, out=out), (0, 0, 0, 1))]:
+        was_read, was = [t._version for t in read], [t._version for t in write]
+        call()
+        assert [t._version for t in read] == was_read
+        assert [t._version - w for t, w in zip(write, was)] == list(moves)
+    weight = torch.ones(64, dtype=torch.bfloat16, device="cuda", requires_grad=True)
+    loss = (kc * weight).sum()
+    kv_append(k, v, kc, vc, off)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        loss.backward()
+    with torch.inference_mode():
+        c = torch.zeros_like(kc)
+        kv_append(k, v, c, c.clone(), off)
+    kv_append(k, v, c, c.clone(), off)              # inference tensors keep no count
+    check_status()
