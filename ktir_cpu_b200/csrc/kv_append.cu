@@ -194,6 +194,8 @@ extern "C" int ktir_kv_append(const KtirKvAppendDesc* d, void* stream) {
       !aligned16(d->v_cache))
     return ktir_set_error(KTIR_ERR_UNSUPPORTED,
                           "ktir_kv_append: head vectors must start on 16-byte boundaries");
+  if ((d->q && !apart(d->qo_stride, te, 2)) || !apart(d->kc_stride, ce, 3) || !apart(d->vc_stride, ce, 3))
+    return ktir_set_error(KTIR_ERR_ARG, "ktir_kv_append: places of a cache, or rows of q_out, share memory");
   AppendParams p;
   p.d = *d;
   const __int128 total = (__int128)d->num_pages * d->page_size;

@@ -718,6 +718,8 @@ extern "C" int ktir_paged_decode(const KtirPagedDecodeDesc* d, void* stream) {
       !aligned16(d->k_cache) || !aligned16(d->v_cache) || !aligned16(d->out) || !aligned16(d->workspace))
     return ktir_set_error(KTIR_ERR_UNSUPPORTED,
                           "ktir_paged_decode: head vectors must start on 16-byte boundaries");
+  if (!apart(d->out_stride, qe, 2))
+    return ktir_set_error(KTIR_ERR_ARG, "ktir_paged_decode: rows of out share memory");
   if (d->workspace_bytes < ktir_paged_decode_workspace(d->batch, d->heads, d->kv_heads, d->dim))
     return ktir_set_error(KTIR_ERR_ARG, "ktir_paged_decode: workspace too small");
   const int sms = sm_count();

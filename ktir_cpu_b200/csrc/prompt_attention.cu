@@ -1333,6 +1333,8 @@ extern "C" int ktir_prompt_attention(const KtirPromptDesc* d, void* stream) {
       !aligned16(d->k) || !aligned16(d->v) || !aligned16(d->out) || !aligned16(d->workspace))
     return ktir_set_error(KTIR_ERR_UNSUPPORTED,
                           "ktir_prompt_attention: head vectors must start on 16-byte boundaries");
+  if (!apart(d->out_stride, qe, 2))
+    return ktir_set_error(KTIR_ERR_ARG, "ktir_prompt_attention: rows of out share memory");
   const bool bf16 = d->dtype == KTIR_BF16;
   PromptParams p;
   p.d = *d;

@@ -85,6 +85,13 @@ inline bool vector_strides(const int64_t* stride, const int64_t* extent, int n) 
   return true;
 }
 
+// a written tensor's entries lie apart (an expanded axis has stride 0)
+inline bool apart(const int64_t* stride, const int64_t* extent, int n) {
+  for (int i = 0; i < n; ++i)
+    if (extent[i] > 1 && stride[i] == 0) return false;
+  return true;
+}
+
 constexpr int MAX_DEVICES = 64;
 
 // the current device, or -1

@@ -897,3 +897,21 @@ def test_written_tensors_are_seen_as_changed():
         kv_append(k, v, c, c.clone(), off)
     kv_append(k, v, c, c.clone(), off)              # inference tensors keep no count
     check_status()
+
+
+def test_outputs_that_share_memory_are_refused():
+    import torch
+    from ktir_cpu_b200 import check_status, kv_append, paged_decode, prompt_attention
+    q, kc, vc, pages, lengths = _decode_inputs("bf16", [40, 20], 4, 2, 64, 16, seed=56)
+    k, v = kc[0, :2].clone(), vc[0, :2].clone()
+    off = torch.tensor([0, 2], dtype=torch.int32, device="cuda")
+    for call in [lambda: paged_decode(q, kc, vc, pages, lengths, out=q[:1].clone().expand(2, -1, -1)),
+                 lambda: prompt_attention(q, k, v, off, out=q[:, :1].clone().expand(-1, 4, -1)),
+                 lambda: kv_append(k, v, kc, vc, off, q=q, q_out=q[:1].clone().expand(2, -1, -1)),
+                 lambda: kv_append(k, v, kc[:1].expand(9, -1, -1, -1), vc[:1].expand(9, -1, -1, -1), off)]:
+        with pytest.raises(ValueError, match="share memory"):
+            call()
+    one = q[:1].clone()
+    assert torch.equal(paged_decode(q[:1], kc, vc, pages[:1], lengths[:1], out=one.as_strided((1, 4, 64), (0, 64, 1))),
+                       paged_decode(q[:1], kc, vc, pages[:1], lengths[:1]))
+    check_status()

@@ -193,3 +193,25 @@ def test_workspaces_are_given_up_after_a_timeout(monkeypatch, timeout):
     with pytest.raises(RuntimeError if timeout else IndexError):
         serving.check_status(3)
     assert fake.forgotten == ([3] if timeout else [])
+
+
+def test_written_tensors_do_not_share_memory():
+    """Outputs and caches with an expanded axis are refused (many tokens, one place);
+    one entry along it needs no stride."""
+    from ktir_cpu_b200 import runtime as R
+    lib = R.load_library()
+    for call, make, names in [
+        (lib.ktir_kv_append, lambda **c: _append_desc(q=1 << 20, q_out=1 << 20, **c), ("qo_stride", "kc_stride", "vc_stride")),
+        (lib.ktir_paged_decode, _decode_desc, ("out_stride",)),
+        (lib.ktir_prompt_attention, _prompt_desc, ("out_stride",)),
+    ]:
+        for name in names:
+            d = make()
+            for other in ("q_stride", "qo_stride"):
+                if hasattr(d, other):
+                    getattr(d, other)[0], getattr(d, other)[1] = 1024, 128
+            for axis in range(len(getattr(d, name))):
+                was, getattr(d, name)[axis] = getattr(d, name)[axis], 0
+                assert call(C.byref(d), None) == ARG, (name, axis)
+                assert b"share memory" in lib.ktir_last_error()
+                getattr(d, name)[axis] = was
