@@ -461,9 +461,11 @@ int ktir_kv_append(const KtirKvAppendDesc* desc, void* stream);
  * pages[b][0 ..].  A sequence of length 0 gives zeros (lse -inf).  lse, when
  * given, receives the natural logarithm of each row's sum of exponentials,
  * [batch][heads] f32.  dim 64 or 128.  workspace: device memory of at least
- * ktir_paged_decode_workspace() bytes, zero before its first use and left so
- * that the next call on the same stream may use it; two calls that may overlap
- * need workspaces of their own. */
+ * ktir_paged_decode_workspace() bytes, zero before its first use (its first
+ * KTIR_PAGED_DECODE_PARTS_BYTES may hold anything) and left so that the next
+ * call on the same stream may use it; two calls that may overlap need
+ * workspaces of their own. */
+#define KTIR_PAGED_DECODE_PARTS_BYTES 8519680
 typedef struct {
   const void* q;                 /* [batch][heads][dim] */
   const void* k_cache; const void* v_cache;
@@ -492,10 +494,12 @@ int ktir_paged_decode(const KtirPagedDecodeDesc* desc, void* stream);
  * of the prompt was read earlier); a query that sees no key gives zeros (lse
  * -inf), as does one of no sequence, where offsets are out of range.  lse as above, [tokens][heads].  dim 64 or 128; heads / kv_heads at
  * most 128.  With a workspace (ktir_prompt_attention_workspace() bytes, zero
- * before its first use, its own for calls that may overlap) few queries over
- * many keys share the keys among the SMs.  Should KTIR_STATUS_TIMEOUT be set,
+ * before its first use but for the first KTIR_PROMPT_PARTS_BYTES, its own for
+ * calls that may overlap) few queries over many keys share the keys among the
+ * SMs.  Should KTIR_STATUS_TIMEOUT be set,
  * outputs of calls since the word was clear were given up, and their workspace
  * must be cleared before its next use. */
+#define KTIR_PROMPT_PARTS_BYTES 10649600
 typedef struct {
   const void* q;                 /* [tokens][heads][dim] */
   const void* k; const void* v;  /* [kv_tokens][kv_heads][dim] */

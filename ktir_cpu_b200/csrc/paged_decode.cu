@@ -48,6 +48,7 @@ constexpr int LOOK = 3;                    // tiles between a look into the page
 constexpr float RESCALE_THRESHOLD = 8.0f;  // log2 units
 constexpr int PART_STRIDE = ROWS * (128 + 2);   // floats of a part: o, then (m, l) per row
 constexpr int64_t PARTS_BYTES = (int64_t)MAX_CTAS * 2 * PART_STRIDE * 4;
+static_assert(PARTS_BYTES == KTIR_PAGED_DECODE_PARTS_BYTES);
 
 struct DecodeParams {
   KtirPagedDecodeDesc d;

@@ -76,6 +76,7 @@ constexpr int MAX_PARTS = 160;       // CTAs of a launch that splits keys
 constexpr int HALVE = 3;             // blocks from which a CTA's two groups of softmax warps share a row tile
 constexpr int PART_FLOATS = 128 * BQ + 2 * BQ;      // O [dim][row], then (m, l) per row
 constexpr int64_t PARTS_BYTES = (int64_t)MAX_PARTS * PART_FLOATS * 4;
+static_assert(PARTS_BYTES == KTIR_PROMPT_PARTS_BYTES);
 constexpr int SCHED_READERS = 11;    // 8 softmax warps, two MMA, TMA
 constexpr float RESCALE_THRESHOLD = 8.0f;   // log2 units
 constexpr float FAR = 16777216.0f;          // 2^24: a maximum from here on is rounded to whole log2 units

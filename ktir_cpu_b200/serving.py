@@ -7,7 +7,8 @@
 
 They work on torch CUDA tensors (f16 or bf16, sums in f32), run on the current
 stream of the tensors' device, allocate nothing but their outputs and a
-workspace per stream, wait for nothing and can be captured into a CUDA graph.
+workspace per stream (and per stream of a capture), wait for nothing and can be
+captured into a CUDA graph.
 A cache is any pair of tensors [pages, page_size, kv_heads, dim] whose head
 vectors are contiguous and start on 16-byte boundaries; a page may be stored
 token by token or head by head (a transposed view).  Index tensors are int32.

@@ -915,3 +915,97 @@ def test_outputs_that_share_memory_are_refused():
     assert torch.equal(paged_decode(q[:1], kc, vc, pages[:1], lengths[:1], out=one.as_strided((1, 4, 64), (0, 64, 1))),
                        paged_decode(q[:1], kc, vc, pages[:1], lengths[:1]))
     check_status()
+
+
+# -- captured calls ------------------------------------------------------------------
+
+def _nodes(graph):
+    """(kernels, bytes cleared, other nodes) of a captured graph."""
+    import ctypes as C
+    rt = C.CDLL("libcudart.so.12")
+
+    class Memset(C.Structure):
+        _fields_ = [("dst", C.c_void_p), ("pitch", C.c_size_t), ("value", C.c_uint), ("element", C.c_uint),
+                    ("width", C.c_size_t), ("height", C.c_size_t)]
+
+    raw, n = C.c_void_p(graph.raw_cuda_graph()), C.c_size_t(0)
+    assert rt.cudaGraphGetNodes(raw, None, C.byref(n)) == 0
+    nodes = (C.c_void_p * n.value)()
+    assert rt.cudaGraphGetNodes(raw, nodes, C.byref(n)) == 0
+    kernels = cleared = others = 0
+    for node in nodes:
+        kind, m = C.c_int(), Memset()
+        assert rt.cudaGraphNodeGetType(C.c_void_p(node), C.byref(kind)) == 0
+        if kind.value == 0:
+            kernels += 1
+        elif kind.value == 2:
+            assert rt.cudaGraphMemsetNodeGetParams(C.c_void_p(node), C.byref(m)) == 0
+            cleared += m.element * m.width * m.height
+        else:
+            others += 1
+    return kernels, cleared, others
+
+
+def test_captured_calls_do_nothing_but_their_kernels():
+    """One kernel a call, and one clear of the counters for all calls of an operator."""
+    import torch
+    from ktir_cpu_b200 import check_status, kv_append, paged_decode, prompt_attention
+    q, kc, vc, pages, lengths = _decode_inputs("bf16", [300, 77, 5], 8, 2, 128, 16, seed=57)
+    k, v = kc[0, :3].clone(), vc[0, :3].clone()
+    p = _prompt_inputs("bf16", [64, 9], [3000, 9], 8, 2, 128, seed=57)
+    slots = torch.tensor([-1, -1, -1], dtype=torch.int32, device="cuda")
+    want, want2 = paged_decode(q, kc, vc, pages, lengths), prompt_attention(*p[:4], kv_offsets=p[4])
+    graph = torch.cuda.CUDAGraph(keep_graph=True)
+    with torch.cuda.graph(graph):
+        for _ in range(6):
+            turned = kv_append(k, v, kc, vc, slots, q=q)
+            got = paged_decode(turned, kc, vc, pages, lengths)
+            got2 = prompt_attention(*p[:4], kv_offsets=p[4])
+    kernels, cleared, others = _nodes(graph)
+    assert (kernels, others) == (18, 0)
+    assert cleared == 3 * 2 * 4 + 160 * 4            # sequences x head tiles; row tiles that share keys
+    graph.instantiate()
+    for _ in range(3):
+        graph.replay()
+        assert torch.equal(got, want) and torch.equal(got2, want2)
+    check_status()
+
+
+@pytest.mark.parametrize("order", [1, -1])
+def test_captured_calls_of_many_sizes(order):
+    """Calls that split sequences and row tiles and calls that do not, of rising and
+    falling sizes, in one graph and on two streams of it: what a graph's later calls
+    allocate may lie where its earlier ones had their workspace."""
+    import torch
+    from ktir_cpu_b200 import check_status, paged_decode, prompt_attention
+    decodes = [_decode_inputs("bf16", n, 8, 2, 128, 16, seed=58)
+               for n in ([5000], [3000, 17, 400], [2000] * 40, [900] * 200, [0, 6000])][::order]
+    prompts = [_prompt_inputs("bf16", new, keys, 8, 2, 128, seed=59)
+               for new, keys in (([64], [8192]), ([5], [900]), ([30] * 60, [30] * 60), ([16] * 4, [5000] * 4))][::order]
+    attend = lambda p: prompt_attention(*p[:4], kv_offsets=p[4])  # noqa: E731
+    want = [paged_decode(*x) for x in decodes], [attend(p) for p in prompts]
+    side = torch.cuda.Stream()
+    graph = torch.cuda.CUDAGraph()
+    for _ in range(2):                               # the second capture after the first has been replayed
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            main = torch.cuda.current_stream()
+            side.wait_stream(main)
+            got = [], []
+            for i in range(5):
+                got[0].append(paged_decode(*decodes[i]))
+                got[1].append(attend(prompts[i % 4]))
+                with torch.cuda.stream(side):
+                    got[0].append(paged_decode(*decodes[4 - i]))
+                    got[1].append(attend(prompts[3 - i % 4]))
+            main.wait_stream(side)
+        for _ in range(20):
+            for t in got[0] + got[1]:
+                t.zero_()
+            graph.replay()
+            eager = paged_decode(*decodes[0]), attend(prompts[0])
+            for i in range(5):
+                assert torch.equal(got[0][2 * i], want[0][i]) and torch.equal(got[0][2 * i + 1], want[0][4 - i])
+                assert torch.equal(got[1][2 * i], want[1][i % 4]) and torch.equal(got[1][2 * i + 1], want[1][3 - i % 4])
+            assert torch.equal(eager[0], want[0][0]) and torch.equal(eager[1], want[1][0])
+    check_status()
