@@ -1,5 +1,6 @@
 """Compile the CUDA library (libktir_b200.so) in-tree for sm_100a, and the
-serving operators' Python binding (_serving.so), which calls it.
+serving operators' Python binding (_serving.so), which calls it, where torch is
+installed.
 
     python -m ktir_cpu_b200.build          # or build() from Python
 
@@ -9,6 +10,8 @@ nvcc cross-compiles without a GPU, so this runs on CPU-only hosts too.
 from __future__ import annotations
 
 import glob
+import importlib.metadata
+import importlib.util
 import os
 import shutil
 import subprocess
@@ -40,17 +43,38 @@ def _newer(target, deps) -> bool:
     return all(os.path.getmtime(p) <= t for p in deps)
 
 
+def _torch():
+    """The installed torch's folder, or None; it is not imported."""
+    spec = importlib.util.find_spec("torch")
+    return spec.submodule_search_locations[0] if spec else None
+
+
+def _made_for() -> str:
+    """What a binding fits: it is compiled against torch's and Python's own headers."""
+    return f"torch {importlib.metadata.version('torch')}, python {sys.version_info[0]}.{sys.version_info[1]}"
+
+
+def _stamp() -> str:
+    return os.path.join(HERE, "_build", "serving.txt")
+
+
+def _binding_up_to_date(headers) -> bool:
+    if not _newer(BINDING, [BINDING_SRC] + headers) or not os.path.exists(_stamp()):
+        return False
+    with open(_stamp()) as f:
+        return f.read() == _made_for()
+
+
 def up_to_date() -> bool:
     headers = glob.glob(os.path.join(HERE, "..", "include", "*.h"))
     return _newer(LIB, sources() + glob.glob(os.path.join(CSRC, "*.cuh")) + headers) and \
-        _newer(BINDING, [BINDING_SRC] + headers)
+        (_torch() is None or _binding_up_to_date(headers))
 
 
 def _compile_binding():
     """The binding's object file and the process that compiles it."""
     import sysconfig
-    import torch
-    inc = os.path.join(os.path.dirname(torch.__file__), "include")
+    inc = os.path.join(_torch(), "include")
     obj = os.path.join(HERE, "_build", "serving_binding.o")
     includes = [inc, os.path.join(inc, "torch", "csrc", "api", "include"), sysconfig.get_paths()["include"],
                 os.path.join(os.path.dirname(os.path.dirname(os.path.realpath(_nvcc()))), "include")]
@@ -61,14 +85,15 @@ def _compile_binding():
 
 
 def _link_binding(obj):
-    import torch
     cmd = ["g++", "-shared", "-o", BINDING + ".tmp", obj, "-L", HERE, "-l:" + os.path.basename(LIB),
            "-Wl,-rpath,$ORIGIN"]
-    cmd += ["-L", os.path.join(os.path.dirname(torch.__file__), "lib")]
+    cmd += ["-L", os.path.join(_torch(), "lib")]
     # torch's libraries are in the process by the time the binding is imported
     cmd += ["-ltorch_python", "-ltorch_cpu", "-ltorch", "-lc10", "-lc10_cuda"]
     subprocess.check_call(cmd)
     os.replace(BINDING + ".tmp", BINDING)
+    with open(_stamp(), "w") as f:
+        f.write(_made_for())
 
 
 def build(force: bool = False, verbose: bool = False) -> str:
@@ -87,8 +112,10 @@ def build(force: bool = False, verbose: bool = False) -> str:
             cmd.insert(1, "-Xptxas=-v")
         procs.append((src, subprocess.Popen(cmd, stdout=subprocess.PIPE, stderr=subprocess.STDOUT)))
         objs.append(obj)
-    binding_obj, binding = _compile_binding()
-    procs.append((BINDING_SRC, binding))
+    binding_obj = None
+    if _torch():                          # the library alone needs none
+        binding_obj, binding = _compile_binding()
+        procs.append((BINDING_SRC, binding))
     failed = []
     for src, p in procs:
         out, _ = p.communicate()
@@ -101,7 +128,8 @@ def build(force: bool = False, verbose: bool = False) -> str:
     tmp_lib = LIB + ".tmp"
     subprocess.check_call([nvcc, *ARCH, "-shared", "-o", tmp_lib, *objs, "-lcudart"])
     os.replace(tmp_lib, LIB)
-    _link_binding(binding_obj)
+    if binding_obj:
+        _link_binding(binding_obj)
     return LIB
 
 
