@@ -80,6 +80,8 @@ def whole_text(layers, embedding, tokens, table):
 
 
 def main(steps=32, n_layers=2, prompts=(37, 5, 120, 64, 1), seed=0):
+    if steps < 1 or min(prompts) < 1:
+        raise ValueError("needs at least one step, and prompts of at least one token")
     device = torch.device("cuda")
     gen = torch.Generator(device=device).manual_seed(seed)
     layers = [Layer(gen, device) for _ in range(n_layers)]
@@ -124,19 +126,17 @@ def main(steps=32, n_layers=2, prompts=(37, 5, 120, 64, 1), seed=0):
         position.add_(1)
         return out
 
-    for b, t in enumerate(new.tolist()):
-        texts[b].append(t)
-    step()                                                   # once outside the graph
-    history = [new.clone()]
-    graph = torch.cuda.CUDAGraph()
-    saved = new.clone(), position.clone()
-    with torch.cuda.graph(graph):
-        last = step()
-    new.copy_(saved[0])
-    position.copy_(saved[1])
-    for _ in range(steps - 2):
-        graph.replay()
-        history.append(new.clone())
+    history, last = [new.clone()], logits[offsets[1:].long() - 1]
+    if steps > 1:
+        step()                                               # once outside the graph; its token is
+        new.copy_(history[0])                                # decoded again, and written again
+        position.copy_(index(prompts))
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            last = step()
+        for _ in range(steps - 1):
+            graph.replay()
+            history.append(new.clone())
     for tokens in history:
         for b, t in enumerate(tokens.tolist()):
             texts[b].append(t)

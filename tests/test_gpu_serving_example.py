@@ -25,3 +25,20 @@ def test_serving_example(steps, layers, prompts):
     # 4 at the end, in the worst case all of the size of the largest logit.
     bound = (8 * layers + 4) * 2.0 ** -8
     assert serve.main(steps, layers, prompts) <= bound
+
+
+@pytest.mark.parametrize("steps", [1, 2, 3])
+def test_serving_example_of_few_steps(steps):
+    """One step: the prompts' own logits.  Two: a single run of the graph."""
+    test_serving_example(steps, 2, (37, 5, 120, 64, 1))
+
+
+def test_serving_example_needs_a_step():
+    sys.path.insert(0, EXAMPLES)
+    try:
+        import serve
+    finally:
+        sys.path.remove(EXAMPLES)
+    for steps, prompts in [(0, (3, 4)), (2, (3, 0))]:
+        with pytest.raises(ValueError):
+            serve.main(steps, 1, prompts)
