@@ -74,7 +74,13 @@ def _fail(kind, what, text):
     raise kind(f"{what}: {text}")
 
 
-def _kind(what, t):
+def _tensor(what, name, t):
+    if not isinstance(t, torch.Tensor):
+        _fail(ValueError, what, f"{name} must be a tensor, got {type(t).__name__}")
+
+
+def _kind(what, name, t):
+    _tensor(what, name, t)
     if t.device.type != "cuda":
         _fail(ValueError, what, f"needs CUDA tensors, got one on {t.device}")
     if t.dtype not in _DTYPES:
@@ -90,6 +96,7 @@ def _no_gradient(what, name, t):
 
 def _vectors(what, name, t, like, layout):
     """A tensor of head vectors, of the call's type and device."""
+    _tensor(what, name, t)
     if t.dim() != layout.count(",") + 1:
         _fail(ValueError, what, f"{name} must be {layout}, got {tuple(t.shape)}")
     if t.dtype != like.dtype or t.device != like.device:
@@ -108,6 +115,7 @@ def _cache(what, name, t, like):
 
 
 def _index(what, name, t, shape, like):
+    _tensor(what, name, t)
     if t.dtype != torch.int32 or t.device != like.device or tuple(t.shape) != tuple(shape):
         _fail(ValueError, what, f"{name} must be int32 {list(shape)} on {like.device}, got {t.dtype} "
                                 f"{list(t.shape)} on {t.device}")
@@ -138,7 +146,7 @@ def rotary_table(max_positions, rot, base=10000.0, device="cuda"):
 
 def _wrong_append(k, v, k_cache, v_cache, slots, q, positions, table, q_out):
     what = "kv_append"
-    _kind(what, k)
+    _kind(what, "k", k)
     _heads(what, "k", k, k)
     _heads(what, "v", v, k)
     _cache(what, "k_cache", k_cache, k)
@@ -154,6 +162,7 @@ def _wrong_append(k, v, k_cache, v_cache, slots, q, positions, table, q_out):
     if (positions is None) != (table is None):
         _fail(ValueError, what, "positions and table go together")
     if table is not None:
+        _tensor(what, "table", table)
         _index(what, "positions", positions, (tokens,), k)
         if table.dim() != 2 or table.dtype != torch.float32 or table.device != k.device or table.stride(1) != 1:
             _fail(ValueError, what, f"table must be f32 [positions, rot] on {k.device}, rows contiguous")
@@ -192,7 +201,7 @@ def kv_append(k, v, k_cache, v_cache, slots, q=None, positions=None, table=None,
 
 def _wrong_decode(q, k_cache, v_cache, pages, lengths, out):
     what = "paged_decode"
-    _kind(what, q)
+    _kind(what, "q", q)
     _heads(what, "q", q, q)
     _cache(what, "k_cache", k_cache, q)
     _cache(what, "v_cache", v_cache, q)
@@ -201,6 +210,7 @@ def _wrong_decode(q, k_cache, v_cache, pages, lengths, out):
     if k_cache.shape != v_cache.shape or k_cache.shape[3] != dim or not kv_heads or heads % kv_heads:
         _fail(ValueError, what, f"caches must be [pages, page_size, kv_heads, {dim}] with kv_heads dividing "
                                 f"{heads}, got {tuple(k_cache.shape)} and {tuple(v_cache.shape)}")
+    _tensor(what, "pages", pages)
     if pages.dim() != 2:
         _fail(ValueError, what, f"pages must be [batch, max_pages], got {tuple(pages.shape)}")
     _index(what, "pages", pages, (batch, pages.shape[1]), q)
@@ -227,7 +237,7 @@ def paged_decode(q, k_cache, v_cache, pages, lengths, scale=None, out=None, retu
 
 def _wrong_prompt(q, k, v, offsets, kv_offsets, out):
     what = "prompt_attention"
-    _kind(what, q)
+    _kind(what, "q", q)
     _heads(what, "q", q, q)
     _heads(what, "k", k, q)
     _heads(what, "v", v, q)
@@ -236,6 +246,7 @@ def _wrong_prompt(q, k, v, offsets, kv_offsets, out):
     if k.shape != v.shape or k.shape[2] != dim or not kv_heads or heads % kv_heads:
         _fail(ValueError, what, f"k and v must be [kv_tokens, kv_heads, {dim}] with kv_heads dividing {heads}, "
                                 f"got {tuple(k.shape)} and {tuple(v.shape)}")
+    _tensor(what, "offsets", offsets)
     if offsets.dim() != 1 or offsets.shape[0] < 2:
         _fail(ValueError, what, f"offsets must be [batch + 1], got {tuple(offsets.shape)}")
     _index(what, "offsets", offsets, tuple(offsets.shape), q)

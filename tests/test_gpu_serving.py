@@ -1009,3 +1009,21 @@ def test_captured_calls_of_many_sizes(order):
                 assert torch.equal(got[1][2 * i], want[1][i % 4]) and torch.equal(got[1][2 * i + 1], want[1][3 - i % 4])
             assert torch.equal(eager[0], want[0][0]) and torch.equal(eager[1], want[1][0])
     check_status()
+
+
+def test_what_is_no_tensor_is_refused():
+    import torch
+    from ktir_cpu_b200 import kv_append, paged_decode, prompt_attention
+    q, kc, vc, pages, lengths = _decode_inputs("bf16", [40, 20], 4, 2, 64, 16, seed=60)
+    k = kc[0, :2]
+    off = torch.tensor([0, 2], dtype=torch.int32, device="cuda")
+    appends = [k, k, kc, vc, off, q, off, torch.zeros(8, 64, device="cuda")]
+    append = lambda *a: kv_append(*a[:5], q=a[5], positions=a[6], table=a[7], q_out=a[8])  # noqa: E731
+    for call, args in [(append, appends + [torch.empty_like(q)]), (lambda *a: paged_decode(*a[:5], out=a[5]),
+                                                                 [q, kc, vc, pages, lengths, torch.empty_like(q)]),
+                       (lambda *a: prompt_attention(*a[:5], out=a[5]), [k, k, k, off, off, torch.empty_like(k)])]:
+        call(*args)
+        for at in range(len(args)):
+            for wrong in (3, "k", [1, 2]):
+                with pytest.raises(ValueError, match="must be"):
+                    call(*args[:at], wrong, *args[at + 1:])

@@ -215,3 +215,16 @@ def test_written_tensors_do_not_share_memory():
                 assert call(C.byref(d), None) == ARG, (name, axis)
                 assert b"share memory" in lib.ktir_last_error()
                 getattr(d, name)[axis] = was
+
+
+@pytest.mark.parametrize("wrong", [None, 3, [1.0, 2.0]])
+def test_what_is_no_tensor_is_refused(wrong):
+    torch = pytest.importorskip("torch")
+    from ktir_cpu_b200 import kv_append, paged_decode, prompt_attention
+    x = torch.zeros(2, 4, 64, dtype=torch.bfloat16)
+    with pytest.raises(ValueError, match="k must be a tensor"):
+        kv_append(wrong, x, x, x, x)
+    with pytest.raises(ValueError, match="q must be a tensor"):
+        paged_decode(wrong, x, x, x, x)
+    with pytest.raises(ValueError, match="q must be a tensor"):
+        prompt_attention(wrong, x, x, x)
