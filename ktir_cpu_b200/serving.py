@@ -268,7 +268,13 @@ def prompt_attention(q, k, v, offsets, kv_offsets=None, causal=True, scale=None,
     - 1 (default: offsets).  A causal mask is aligned at the end: query i of n
     sees keys j <= i + m - n of m, so later pieces of a prompt attend to its
     earlier ones.  heads is a multiple of kv_heads, scale defaults to dim **
-    -0.5.  Returns out [tokens, heads, dim], zero where a query sees no key (and, if
+    -0.5.  A value row that is not finite reaches, besides the queries that see it,
+    some just before it, as 0 times it is not 0 in the product: the mask leaves out
+    whole blocks of keys only, 80 of them at dim 128 and 128 at dim 64, for tiles of
+    128 // (heads // kv_heads) tokens, so that queries less than the sum of the two
+    before it may be reached.  A key row does not, nor does either reach another
+    sequence.
+    Returns out [tokens, heads, dim], zero where a query sees no key (and, if
     offsets are bad, where it belongs to no sequence); with `return_lse` also the f32 [tokens, heads] logarithm of each row's sum of
     exponentials."""
     r = _ext().prompt_attention(q, k, v, offsets, kv_offsets, causal, scale, out, return_lse)

@@ -1027,3 +1027,61 @@ def test_what_is_no_tensor_is_refused():
             for wrong in (3, "k", [1, 2]):
                 with pytest.raises(ValueError, match="must be"):
                     call(*args[:at], wrong, *args[at + 1:])
+
+
+# -- reach of what is not finite, calls without a workspace, many sequences ----------------
+
+@pytest.mark.parametrize("n,heads,kv_heads,dim", [(256, 4, 1, 128), (256, 2, 2, 64), (3000, 8, 8, 128), (3000, 16, 4, 64)])
+@pytest.mark.parametrize("bad", [math.nan, math.inf])
+def test_prompt_reach_of_infinite_values(n, heads, kv_heads, dim, bad):
+    """A value row that is not finite reaches no row tile whose last block of keys ends
+    before it, and no other kv head."""
+    import torch
+    from ktir_cpu_b200 import check_status, prompt_attention
+    q, k, v, offsets, _ = _prompt_inputs("bf16", [n], [n], heads, kv_heads, dim, seed=61)
+    clean = prompt_attention(q, k, v, offsets)
+    group = heads // kv_heads
+    tile, block = 128 // group, 80 if dim == 128 else 128
+    for at in (n // 3, n // 2 + 17, n - 1):
+        v2 = v.clone()
+        v2[at, 0] = bad
+        got = prompt_attention(q, k, v2, offsets)
+        first = next(t for t in range(0, n, tile) if -(-min(n, t + tile) // block) * block > at)
+        assert at - first < tile + block
+        assert torch.equal(got[:first], clean[:first]) and torch.equal(got[:, group:], clean[:, group:])
+        assert not torch.isfinite(got[at:, :group]).any()
+    check_status()
+
+
+@pytest.mark.parametrize("new,keys,dim", [([64], [8192], 128), ([16] * 4, [5000] * 4, 64), ([300], [300], 64)])
+def test_prompt_without_a_workspace(new, keys, dim):
+    """The C entry with no workspace: the keys of few queries are not shared out."""
+    import ctypes
+    import torch
+    from ktir_cpu_b200 import runtime as R
+    q, k, v, offsets, kv_offsets = _prompt_inputs("bf16", new, keys, 8, 2, dim, seed=62)
+    out, lse = torch.empty_like(q), torch.empty(q.shape[:2], device="cuda")
+    status = torch.zeros(1, dtype=torch.int32, device="cuda")
+    d = R.KtirPromptDesc()
+    for name, t in (("q", q), ("k", k), ("v", v), ("out", out), ("lse", lse), ("offsets", offsets),
+                    ("kv_offsets", kv_offsets), ("status", status)):
+        setattr(d, name, t.data_ptr())
+    for name, t in (("q_stride", q), ("k_stride", k), ("v_stride", v), ("out_stride", out)):
+        getattr(d, name)[0], getattr(d, name)[1] = t.stride(0), t.stride(1)
+    d.batch, d.tokens, d.kv_tokens = len(new), q.shape[0], k.shape[0]
+    d.heads, d.kv_heads, d.dim, d.dtype, d.scale, d.causal = 8, 2, dim, R.BF16, dim ** -0.5, 1
+    stream = ctypes.c_void_p(torch.cuda.current_stream().cuda_stream)
+    assert R.load_library().ktir_prompt_attention(ctypes.byref(d), stream) == 0
+    torch.cuda.synchronize()
+    assert not int(status)
+    _check_prompt("bf16", q, k, v, offsets, kv_offsets, True, dim ** -0.5, out, lse)
+
+
+def test_prompt_thousands_of_sequences():
+    from ktir_cpu_b200 import check_status, prompt_attention
+    rng = random.Random(9)
+    new = [rng.choice([0, 0, 1, 1, 2, 9, 33, 150]) for _ in range(3000)]
+    x = _prompt_inputs("f16", new, new, 1, 1, 64, seed=63)
+    out, lse = prompt_attention(*x[:4], return_lse=True)
+    check_status()
+    _check_prompt("f16", *x, True, 0.125, out, lse)
