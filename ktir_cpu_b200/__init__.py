@@ -12,13 +12,19 @@ from .latency import HardwareConfig, LatencyCategory, LatencyReport
 from .parser import KTIRParser, KTIRParserBase
 
 __all__ = ["KTIRInterpreter", "KTIRParser", "KTIRParserBase", "HardwareConfig",
-           "LatencyCategory", "LatencyReport", "check_status", "kv_append", "paged_decode",
-           "prompt_attention", "rotary_table"]
+           "LatencyCategory", "LatencyReport"]
+
+# imported by name: a star import would bring torch with it
+_SERVING = ("check_status", "kv_append", "paged_decode", "prompt_attention", "rotary_table")
 
 
 def __getattr__(name):
     # the serving operators import torch; the interpreter's host side does not
-    if name in ("check_status", "kv_append", "paged_decode", "prompt_attention", "rotary_table"):
+    if name in _SERVING:
         from . import serving
         return globals().setdefault(name, getattr(serving, name))
     raise AttributeError(f"module {__name__!r} has no attribute {name!r}")
+
+
+def __dir__():
+    return sorted({*globals(), *_SERVING})
