@@ -493,7 +493,7 @@ int ktir_paged_decode(const KtirPagedDecodeDesc* desc, void* stream);
  * end: query i of n sees keys j <= i + m - n of m (m > n when the first part
  * of the prompt was read earlier); a query that sees no key gives zeros (lse
  * -inf), as does one of no sequence, where offsets are out of range.  lse as above, [tokens][heads].  dim 64 or 128; heads / kv_heads at
- * most 128.  With a workspace (ktir_prompt_attention_workspace() bytes, zero
+ * most 128; at most 2^20 sequences.  With a workspace (ktir_prompt_attention_workspace() bytes, zero
  * before its first use but for the first KTIR_PROMPT_PARTS_BYTES, its own for
  * calls that may overlap) few queries over many keys share the keys among the
  * SMs.  Should KTIR_STATUS_TIMEOUT be set,

@@ -348,6 +348,9 @@ struct Order {
   uint32_t magic;
   int weight;            // of the tile last found, at first the heaviest of all
   int above;             // tiles heavier than that
+  int upto;              // and tiles of at least that weight, once one has been found
+  long long from;        // sequences before this one have had all their tiles of the weight looked at,
+  int passed;            // this many: a walk over all tiles looks once at every sequence for each weight
   int* table;            // tiles of at least each weight, or null
 
   __device__ __forceinline__ int divide(int x) const {      // x / T, x >= 0
@@ -415,11 +418,15 @@ struct Order {
   __device__ void find(int x, bool any, long long& b_out, int& i_out) {
     if (any) {
       weight = above = 0;
+    } else if (x < upto) {
+      // of the weight last found
     } else if (table) {
       while (weight > 0 && table[weight] <= x) above = table[weight--];
+      upto = table[weight];
+      from = passed = 0;
     } else {
       int hi = weight + 1, hi_count = above;   // count(hi) <= x
-      int step = 1, lo = max(0, hi - 1), c = count(lo);
+      int step = 1, lo = max(0, hi - 1), c = count(lo), lo_count;
       while (c <= x && lo > 0) {
         hi = lo;
         hi_count = c;
@@ -427,11 +434,13 @@ struct Order {
         lo = max(0, hi - step);
         c = count(lo);
       }
-      while (hi - lo > 1) {                    // count(lo) > x >= count(hi)
+      lo_count = c;
+      while (hi - lo > 1) {                    // lo_count = count(lo) > x >= count(hi)
         const int mid = (lo + hi) >> 1;
         c = count(mid);
         if (c > x) {
           lo = mid;
+          lo_count = c;
         } else {
           hi = mid;
           hi_count = c;
@@ -439,12 +448,14 @@ struct Order {
       }
       weight = lo;
       above = hi_count;
+      upto = lo_count;
+      from = passed = 0;
     }
     const int lo = weight;
-    int r = x - above;
+    int r = x - above - passed;
     b_out = -1;
     i_out = 0;
-    for (long long b0 = 0; b0 < p.d.batch; b0 += 32) {
+    for (long long b0 = from; b0 < p.d.batch; b0 += 32) {
       const long long b = b0 + lane;
       int first = 0, mine = 0;
       if (b < p.d.batch) {
@@ -461,9 +472,11 @@ struct Order {
       }
       const unsigned hit = __ballot_sync(0xffffffffu, r >= incl - mine && r < incl);
       if (hit) {
-        const int from = __ffs(hit) - 1;
-        b_out = b0 + from;
-        i_out = __shfl_sync(0xffffffffu, first + r - (incl - mine), from);
+        const int at = __ffs(hit) - 1;
+        b_out = b0 + at;
+        i_out = __shfl_sync(0xffffffffu, first + r - (incl - mine), at);
+        from = b0;
+        passed = x - above - r;
         return;
       }
       r -= __shfl_sync(0xffffffffu, incl, 31);
@@ -604,7 +617,7 @@ __global__ void __launch_bounds__(THREADS, 1)
       // us against 489).
       const bool singly = parts || rows <= 2 * G || 2 * twos - rows > (2 * twos) / 3;
       const int all = parts ? rows * splits : singly ? (rows + 1) / 2 : twos;
-      Order<BK> order = {p, B.lengths, lane, singly ? half : 2 * half, singly ? p.token_magic : p.pair_magic, heaviest, 0, nullptr};
+      Order<BK> order = {p, B.lengths, lane, singly ? half : 2 * half, singly ? p.token_magic : p.pair_magic, heaviest, 0, 0, 0, 0, nullptr};
 
       for (int next = 0;; ++next) {
         const int s = next % SCHED;
@@ -1320,7 +1333,9 @@ extern "C" int ktir_prompt_attention(const KtirPromptDesc* d, void* stream) {
     return ktir_set_error(KTIR_ERR_UNSUPPORTED, "ktir_prompt_attention: needs f16 or bf16");
   if (d->dim != 64 && d->dim != 128)
     return ktir_set_error(KTIR_ERR_UNSUPPORTED, "ktir_prompt_attention: needs dim 64 or 128");
-  if (d->batch < 1 || d->batch > (1 << 24) || d->tokens < 0 || d->tokens > 0x7fffffffLL ||
+  if (d->batch > (1 << 20))      // every CTA looks at every sequence for each weight of a tile (40,000 of 20 tokens: 2.6 ms)
+    return ktir_set_error(KTIR_ERR_UNSUPPORTED, "ktir_prompt_attention: more than 2^20 sequences in a call");
+  if (d->batch < 1 || d->tokens < 0 || d->tokens > 0x7fffffffLL ||
       d->kv_tokens < 0 || d->kv_tokens > 0x7fffffffLL || d->heads < 1 || d->kv_heads < 1 ||
       d->heads % d->kv_heads || d->heads > (1 << 16))
     return ktir_set_error(KTIR_ERR_ARG, "ktir_prompt_attention: extent out of range");

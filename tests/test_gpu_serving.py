@@ -1085,3 +1085,52 @@ def test_prompt_thousands_of_sequences():
     out, lse = prompt_attention(*x[:4], return_lse=True)
     check_status()
     _check_prompt("f16", *x, True, 0.125, out, lse)
+
+
+def test_prompt_time_grows_with_the_sequences():
+    """Four times the sequences of few tokens take about four times as long, not sixteen;
+    and they are right at the batch's end."""
+    import torch
+    from ktir_cpu_b200 import check_status, prompt_attention
+
+    def timed(batch):
+        gen = _gen(batch)
+        new = torch.randint(1, 40, (batch,), generator=gen, device="cuda")
+        offsets = torch.cat([torch.zeros(1, dtype=torch.int64, device="cuda"), new.cumsum(0)]).int()
+        n = int(offsets[-1])
+        q, k, v = (_randn(gen, "bf16", n, h, 64) for h in (4, 2, 2))
+        prompt_attention(q, k, v, offsets)
+        best = math.inf
+        for _ in range(5):
+            a, b = (torch.cuda.Event(enable_timing=True) for _ in range(2))
+            a.record()
+            out, lse = prompt_attention(q, k, v, offsets, return_lse=True)
+            b.record()
+            torch.cuda.synchronize()
+            best = min(best, a.elapsed_time(b))
+        for at in (0, batch // 2, batch - 200):
+            ends = offsets[at:at + 201]
+            lo, hi = int(ends[0]), int(ends[-1])
+            _check_prompt("bf16", q[lo:hi], k[lo:hi], v[lo:hi], ends - lo, ends - lo, True, 0.125, out[lo:hi], lse[lo:hi])
+        return best
+
+    few, many = timed(5000), timed(20000)
+    check_status()
+    assert many < 8 * few, (few, many)
+
+
+@pytest.mark.parametrize("causal", [True, False])
+def test_prompt_many_weights_over_many_sequences(causal):
+    """More sequences than a block keeps the lengths of, of many key counts, some beyond
+    the table of weights: every tile is found once."""
+    import torch
+    from ktir_cpu_b200 import check_status, prompt_attention
+    rng = random.Random(11)
+    for longest in (600, 45000):
+        new = [rng.choice([0, 1, 3, 40, 130, 300]) for _ in range(400)]
+        keys = [n + rng.choice([0, 0, 5, 700]) if n else 0 for n in new]
+        new[333], keys[333] = 200, longest
+        q, k, v, offsets, kv_offsets = _prompt_inputs("bf16", new, keys, 2, 1, 128, seed=64)
+        out, lse = prompt_attention(q, k, v, offsets, kv_offsets=kv_offsets, causal=causal, return_lse=True)
+        check_status()
+        _check_prompt("bf16", q, k, v, offsets, kv_offsets, causal, 128 ** -0.5, out, lse)

@@ -228,3 +228,11 @@ def test_what_is_no_tensor_is_refused(wrong):
         paged_decode(wrong, x, x, x, x)
     with pytest.raises(ValueError, match="q must be a tensor"):
         prompt_attention(wrong, x, x, x)
+
+
+def test_prompt_batch_limit():
+    """The kernel looks at every sequence in every block: a call has a bound on them."""
+    from ktir_cpu_b200 import runtime as R
+    lib = R.load_library()
+    assert lib.ktir_prompt_attention(C.byref(_prompt_desc(batch=(1 << 20) + 1)), None) == UNSUPPORTED
+    assert b"2^20" in lib.ktir_last_error()
