@@ -1233,12 +1233,21 @@ __global__ void __launch_bounds__(THREADS, 1)
     // Nothing else writes them.
     if (B.gaps && !*abort) {
       for (long long at = (long long)blockIdx.x * 256 + tid; at < d.tokens; at += (long long)gridDim.x * 256) {
-        bool covered = false;
-        for (long long b = 0; b < d.batch && !covered; ++b) {
+        auto covers = [&](long long b) -> bool {
           bool bad;
           const long long n = sequence(d, b, bad).n, from = at - d.offsets[b];
-          covered = from >= 0 && from < n;
+          return from >= 0 && from < n;
+        };
+        // by halves, which finds it where offsets rise, else among all (among all for every
+        // token of 40,000 sequences of 20, the last ones in none: 57.6 ms against 7.7)
+        long long low = 0, high = d.batch;
+        while (high - low > 1) {
+          const long long mid = (low + high) >> 1;
+          if (d.offsets[mid] <= at) low = mid;
+          else high = mid;
         }
+        bool covered = covers(low);
+        for (long long b = 0; b < d.batch && !covered; ++b) covered = covers(b);
         if (covered) continue;
         for (int h = 0; h < d.heads; ++h) {
           T* out = static_cast<T*>(d.out) + at * d.out_stride[0] + h * d.out_stride[1];
