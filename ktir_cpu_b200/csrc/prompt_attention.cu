@@ -581,11 +581,6 @@ __global__ void __launch_bounds__(THREADS, 1)
         singles += tiles;
         pairs += (tiles + 1) / 2;
       }
-      any_bad = __any_sync(0xffffffffu, any_bad || ends);
-      if (lane == 0) {
-        B.gaps = any_bad;
-        if (any_bad && blockIdx.x == 0) atomicOr(d.status, KTIR_STATUS_BAD_INDEX);
-      }
       __syncwarp();
       heaviest = (int)__reduce_max_sync(0xffffffffu, (unsigned)heaviest);
       const int rows = warp_sum(singles) * d.kv_heads, twos = warp_sum(pairs) * d.kv_heads;     // below 2^30
@@ -677,6 +672,13 @@ __global__ void __launch_bounds__(THREADS, 1)
               }
             }
             if (!singly) break;
+          }
+        }
+        if (stop) {                           // not before the first tile: its way is the short prompts' time
+          any_bad = __any_sync(0xffffffffu, any_bad || ends);
+          if (lane == 0) {
+            B.gaps = any_bad;
+            if (any_bad && blockIdx.x == 0) atomicOr(d.status, KTIR_STATUS_BAD_INDEX);
           }
         }
         __syncwarp();
