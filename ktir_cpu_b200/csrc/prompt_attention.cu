@@ -498,6 +498,37 @@ __device__ __forceinline__ void row_tile(const PromptParams& p, long long b, con
   r.blocks = here > 0 && end > 0 ? (end + BK - 1) / BK : 0;
 }
 
+// Bad offsets: tokens of no sequence get zeros, not what the memory held before (nothing
+// else writes them).  256 threads of every CTA; a function of its own, out of the way of
+// the softmax's registers.
+template <typename T, int D>
+__device__ __noinline__ void fill_gaps(const PromptParams& p, int tid) {
+  const KtirPromptDesc& d = p.d;
+  for (long long at = (long long)blockIdx.x * 256 + tid; at < d.tokens; at += (long long)gridDim.x * 256) {
+    auto covers = [&](long long b) -> bool {
+      bool bad;
+      const long long n = sequence(d, b, bad).n, from = at - d.offsets[b];
+      return from >= 0 && from < n;
+    };
+    // by halves, which finds it where offsets rise, else among all (among all for every
+    // token of 40,000 sequences of 20, the last ones in none: 57.6 ms against 7.7)
+    long long low = 0, high = d.batch;
+    while (high - low > 1) {
+      const long long mid = (low + high) >> 1;
+      if (d.offsets[mid] <= at) low = mid;
+      else high = mid;
+    }
+    bool covered = covers(low);
+    for (long long b = 0; b < d.batch && !covered; ++b) covered = covers(b);
+    if (covered) continue;
+    for (int h = 0; h < d.heads; ++h) {
+      T* out = static_cast<T*>(d.out) + at * d.out_stride[0] + h * d.out_stride[1];
+      for (int i = 0; i < D; i += 8) *reinterpret_cast<uint4*>(out + i) = make_uint4(0, 0, 0, 0);
+      if (d.lse) d.lse[at * d.heads + h] = -INFINITY;
+    }
+  }
+}
+
 template <typename T, int D>
 __global__ void __launch_bounds__(THREADS, 1)
     k_prompt_attention(const __grid_constant__ CUtensorMap tq, const __grid_constant__ CUtensorMap tk,
@@ -1231,33 +1262,7 @@ __global__ void __launch_bounds__(THREADS, 1)
       }
       if (store && d.lse) d.lse[tok * d.heads + head] = l == 0.f ? -INFINITY : (m + log2f(l)) * LN2;
     }
-    // Bad offsets: tokens of no sequence get zeros, not what the memory held before.
-    // Nothing else writes them.
-    if (B.gaps && !*abort) {
-      for (long long at = (long long)blockIdx.x * 256 + tid; at < d.tokens; at += (long long)gridDim.x * 256) {
-        auto covers = [&](long long b) -> bool {
-          bool bad;
-          const long long n = sequence(d, b, bad).n, from = at - d.offsets[b];
-          return from >= 0 && from < n;
-        };
-        // by halves, which finds it where offsets rise, else among all (among all for every
-        // token of 40,000 sequences of 20, the last ones in none: 57.6 ms against 7.7)
-        long long low = 0, high = d.batch;
-        while (high - low > 1) {
-          const long long mid = (low + high) >> 1;
-          if (d.offsets[mid] <= at) low = mid;
-          else high = mid;
-        }
-        bool covered = covers(low);
-        for (long long b = 0; b < d.batch && !covered; ++b) covered = covers(b);
-        if (covered) continue;
-        for (int h = 0; h < d.heads; ++h) {
-          T* out = static_cast<T*>(d.out) + at * d.out_stride[0] + h * d.out_stride[1];
-          for (int i = 0; i < D; i += 8) *reinterpret_cast<uint4*>(out + i) = make_uint4(0, 0, 0, 0);
-          if (d.lse) d.lse[at * d.heads + h] = -INFINITY;
-        }
-      }
-    }
+    if (B.gaps && !*abort) fill_gaps<T, D>(p, tid);
   }
   tc_fence_before();
   __syncthreads();
