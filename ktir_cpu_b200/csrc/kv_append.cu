@@ -12,7 +12,7 @@
 // three vectors on their way at once, the first ones asked for before the
 // position, the slot and the table's row are there.  Blocks of 64 threads, 12 of
 // them on an SM at once, keep the most copies in flight: 24576 tokens of 32 + 8 + 8
-// heads of 128 take 93 us = 6.6 TB/s (128 threads: 106 us, one vector at a time: 98).
+// heads of 128 take 93 to 97 us = 6.6 to 6.4 TB/s (128 threads: 106 us, one vector at a time: 98).
 // Where a token has less than three vectors for each thread of a block, and there
 // are more tokens than blocks fit at once, a block takes as many tokens as it has
 // threads for: 20344 tokens of 6 + 1 + 1 heads of 64 11.8 us against 28.9, of 15 +

@@ -9,7 +9,9 @@
 // two products run on mma.sync (m16n8k16) with 16 keys, or 16 elements of the
 // values, as its rows and 8 query heads as its columns: x^T = K q^T, then o^T +=
 // V^T p^T (tcgen05's 64 or 128 rows would be mostly empty).  A head tile has 8
-// heads, or 16 where g is above 8; a larger g takes several.
+// heads, or 16 where g is above 8; a larger g takes several.  (32 sequences of 200 to
+// 4000 keys, 8 kv heads, floor 34.0 us: g = 4 43.7 us, 12 50.2, 16 52.4; dim 64, floor
+// 17.0: g = 8 29.5, 16 36.0, where the second tile's queries and outputs spill 80 bytes.)
 //
 // Split over the cache: the 64-key tiles of all sequences form one list, cut
 // into equal stretches, one per group of CTAs; the CTAs of a group take the
@@ -42,7 +44,11 @@ constexpr int ROWS = 16;                   // query heads per head tile at most
 constexpr int MAX_CTAS = 512;              // of a launch that splits sequences
 constexpr int MIN_TILES = 2;               // per stretch: both in flight at once
 constexpr int FIT_BATCH = 64;              // sequences of a launch that may get CTAs of their own,
-constexpr int FIT_TILES = 10;              // and tiles of an even stretch then
+// And tiles of an even stretch then.  8 sequences of 8.9 (and 16 of 6.5) tiles to a stretch,
+// 8 kv heads of 128: CTAs of their own 21.4 (17.4) us, even stretches 23.0 (19.6).  Above
+// that it goes either way: 8 sequences of 13.6 28.1 against 30.1, 32 of 13.3 29.3 against
+// 28.9, 16 of 10.9 (20 heads of 64) 22.6 against 22.3.
+constexpr int FIT_TILES = 10;
 constexpr unsigned SNAP = 12;              // tiles of a sequence that is not cut in two
 constexpr int LOOK = 3;                    // tiles between a look into the page table and the copy
 constexpr float RESCALE_THRESHOLD = 8.0f;  // log2 units

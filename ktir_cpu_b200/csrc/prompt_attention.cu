@@ -47,8 +47,8 @@
 // second product (tcgen05 wants one type for both operands), half an ulp per
 // weight (in f16 2^-32 of a row's largest where that is more); l adds the unrounded
 // weights.
-// Measured, 8192 tokens of 32 heads over 8, causal: dim 128 459 us in a short burst
-// (1,200 TFLOP/s) and 531 under the power cap, dim 64 365 us.  Of a block's 2,100
+// Measured, 8192 tokens of 32 heads over 8, causal: dim 128 449 us in a short burst
+// (1,220 TFLOP/s) and 505 to 520 under the power cap, dim 64 360 us.  Of a block's 2,100
 // cycles (80 keys, both row tiles) the exponentials take 1,300; both groups of softmax
 // warps run in step, so nothing else overlaps them.  A change of tiles costs 4,500
 // cycles: the last product, the outputs, the next tile's S.
@@ -637,10 +637,10 @@ __global__ void __launch_bounds__(THREADS, 1)
         }
       }
       // Singles where a CTA has few row tiles, each then next to one of another weight
-      // (7 pieces of prompts, 195 row tiles: 36 us against 44 in pairs), or where pairs
+      // (7 pieces of prompts, 200 row tiles: 37 us against 44 in pairs), or where pairs
       // would leave more than a third of them empty (200 prompts of 32 tokens: 46 us
-      // against 59).  Else pairs: their shared blocks save L2 traffic (8192 tokens: 459
-      // us against 489).
+      // against 59).  Else pairs: their shared blocks save L2 traffic (8192 tokens: 30
+      // us of 489).
       const bool singly = parts || rows <= 2 * G || 2 * twos - rows > (2 * twos) / 3;
       const int all = parts ? rows * splits : singly ? (rows + 1) / 2 : twos;
       Order<BK> order = {p, B.lengths, lane, singly ? half : 2 * half, singly ? p.token_magic : p.pair_magic, heaviest, 0, 0, 0, 0, nullptr};
